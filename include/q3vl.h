@@ -143,6 +143,79 @@ Q3_API int q3_attn_decode_paged(const void* q, const void* k_pages, const void* 
                          int64_t table_stride, int page_tokens, int num_pages, float scale,
                          void* workspace, size_t workspace_bytes, q3_stream_t stream);
 
+/* ---- ragged serving step over paged K/V -----------------------------------
+ * The decoder layer's attention (model_fused.py:107-129, :244-262) for a batch
+ * whose requests have different lengths: q_lens[b] new tokens of each request,
+ * packed one after the other, on past_lens[b] cached positions.  The reference
+ * and the paged calls above take one start position and one length for the
+ * whole batch.  Lengths, tables, slots and positions stay on the device, so a
+ * step can be captured and replayed with other lengths.  Pools and block
+ * tables as q3_kv_pages_* lays them out: [num_pages, Hkv, page_tokens, 128]
+ * bf16, page_tokens a multiple of 64; position t of request b in page
+ * block_table[b * table_stride + t / page_tokens], table_width entries a row.
+ * A bad length, table entry or slot is recorded in the device error word
+ * (0x90x plan, 0x911 slots, 0x92x decode, 0x93x prefill) and what it maps is
+ * skipped or clamped as said below; nothing is read or written out of range. */
+
+/* Block tables, slot map and positions from the lengths.  q_lens, past_lens
+ * int32 [B], 0 <= B <= 8192.  With free_pages (int32 [n_free]), request b gets
+ * ceil((past + q) / page_tokens) - ceil(past / page_tokens) pages from the list,
+ * in request order, written to its row of block_table behind the pages of its
+ * past positions (entries there are taken as empty); with NULL the table
+ * already maps every position.  Outputs: cu_q int32 [B + 1] first packed token
+ * of each request; kv_lens int32 [B] = past + q; counts int32 [2] = {packed
+ * tokens, pages taken}; for each of n_tokens packed rows requests int32,
+ * positions int64 (cache position + rope_delta[b], rope_delta int64 [B] or
+ * NULL) and slots int64 (page * page_tokens + offset).  Rows behind the last
+ * request get request -1, position 0, slot -1.  Errors recorded: 0x901 a
+ * negative length (taken as 0); 0x902 a position past the table (slot -1,
+ * kv_lens clamped); 0x903 no page (free list short: counts[1] > n_free, table
+ * entry -1; or the table's entry negative; slot -1); 0x904 more tokens than
+ * n_tokens (the last ones are dropped). */
+Q3_API int q3_ragged_plan(const int32_t* q_lens, const int32_t* past_lens, int B,
+                          int32_t* block_table, int64_t table_stride, int table_width,
+                          int page_tokens, const int32_t* free_pages, int n_free,
+                          const int64_t* rope_delta, int64_t n_tokens, int32_t* cu_q,
+                          int32_t* kv_lens, int32_t* requests, int64_t* positions, int64_t* slots,
+                          int32_t* counts, q3_stream_t stream);
+
+/* Per-head QK-RMSNorm, rotary positions and the K/V write of packed tokens
+ * (model_fused.py:107-129, :244-246; M-RoPE of transformers 5.5.0
+ * modeling_qwen3_vl.py:352-386).  qkv bf16 [n_tokens, (Hq + 2 Hkv) * 128] with
+ * row stride qkv_stride elements (a multiple of 8); positions int64: axis a of
+ * token i at positions[a * pos_axis_stride + i] (t, h, w; pos_axis_stride 0:
+ * one axis for all three); inv_freq f32 [64]; sections as q3_mrope_cos_sin.
+ * q_out [n_tokens, Hq, 128], row stride q_stride; the K and V rows of token i
+ * go to position slots[i] % page_tokens of page slots[i] / page_tokens.  fp32
+ * throughout with one rounding at the end (angles reduced in fp64).  A token
+ * whose slot is -1 is padding: nothing of it is read or written.  A slot
+ * outside the pool is recorded (0x911) and its token skipped. */
+Q3_API int q3_qkv_norm_rope_ragged(const void* qkv, int64_t qkv_stride, const void* q_norm_w,
+                                   const void* k_norm_w, const int64_t* positions,
+                                   int64_t pos_axis_stride, const float* inv_freq,
+                                   const int64_t* slots, void* q_out, int64_t q_stride,
+                                   void* k_pages, void* v_pages, int64_t n_tokens, int Hq, int Hkv,
+                                   int head_dim, int page_tokens, int64_t num_pages, int sec_h,
+                                   int sec_w, float eps, q3_stream_t stream);
+
+/* Attention of one new token per request (model_fused.py:248-262 at S = 1):
+ * q, out bf16 [B, Hq, 128] with row strides (elements; out_stride a multiple
+ * of 8); request b attends to positions [0, kv_lens[b]) (int32 [B] on the
+ * device); kv_lens[b] = 0 gives zeros.  Hq / Hkv <= 16.  Rows of the pools at
+ * or past kv_lens[b] may hold anything, NaN included.  The work is divided
+ * over the SMs by length on the device; partial results meet in the workspace
+ * (q3_attn_decode_ragged_workspace_bytes, 16-byte aligned; no state is kept in
+ * it between calls, but two calls that may overlap need one each).  A length
+ * outside 0 .. table_width * page_tokens is clamped (0x921); a table entry
+ * outside the pool is read as page 0 (0x922). */
+Q3_API size_t q3_attn_decode_ragged_workspace_bytes(int Hq, int Hkv);
+Q3_API int q3_attn_decode_ragged(const void* q, int64_t q_stride, const void* k_pages,
+                                 const void* v_pages, void* out, int64_t out_stride, int B, int Hq,
+                                 int Hkv, int head_dim, const int32_t* block_table,
+                                 int64_t table_stride, int table_width, int page_tokens,
+                                 int64_t num_pages, const int32_t* kv_lens, float scale,
+                                 void* workspace, size_t workspace_bytes, q3_stream_t stream);
+
 /* ---- vision tower (transformers 5.5.0 Qwen3VLVisionModel, which the
  * reference runs at vision.py:51-53, :74-76) --------------------------------
  * Tokens are patches in merge-block order.  The image table `imgs` is int32

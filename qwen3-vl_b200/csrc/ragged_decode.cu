@@ -1,0 +1,595 @@
+// Ragged serving step: attention of one new token per request, each request
+// over its own length of the paged K/V cache.
+//
+// The S = 1 eager attention of forward_layer (model_fused.py:248-262) for a
+// batch whose requests have different lengths (the reference, and the paged
+// kernel of attn_decode.cu, take one length for the whole batch):
+//   out[b, h] = softmax(q[b, h] . K_b^T * scale) V_b over positions
+//   [0, kv_lens[b]), K/V head h / (Hq / Hkv), position t in page
+//   table[b, t / page_tokens]; a request of length 0 gives zeros.
+// One pass with a running maximum and sum (fp32, log2 units):
+//   m' = max(m, s),  l' = l 2^(m-m') + 2^(s-m'),  o' = o 2^(m-m') + 2^(s-m') v.
+//
+// Bound by HBM: every K/V row of a request is read once, for all Hq / Hkv
+// query heads of its K/V head.  The lengths are only known on the device, so
+// the work is split there: the 64-position tiles of all (request, K/V head)
+// pairs form one list, and CTA c of G takes tiles [U c / G, U (c+1) / G), which
+// may begin and end inside a pair.  Equal bytes per SM whatever the lengths
+// (32 requests of 257 to 32768 positions or one of 700), where one CTA or one
+// fixed number of splits per pair leaves SMs idle behind the longest request.
+// A pair inside one CTA is written directly; the pieces of a pair that spans
+// CTAs go to the workspace in fp32 and a second kernel joins them in CTA order
+// (the same order every time).  The second kernel costs about 2 us; the
+// last-arriving-CTA join that would save it was slower in attn_decode.cu, and
+// its counters would tie the workspace to one stream.
+//
+// A producer warp streams K and V tiles by TMA into a ring of 32 KB stages;
+// eight consumer warps in two groups take alternate tiles, 16 positions per
+// warp: S = Q K^T by mma.sync with the pair's query heads as the rows (8, or 16
+// when Hq / Hkv > 8), the softmax above per row, O += P V with P rounded to
+// bf16 (2^-9 relative and independent per key, below the bf16 rounding of the
+// output; the sum l takes the unrounded p).
+#include <math.h>
+
+#include "common.cuh"
+
+namespace q3 {
+namespace {
+
+constexpr int kD = 128;
+constexpr int kTile = 64;                     // positions per stage
+constexpr int kHalf = kTile * 128;            // one 64-dim box of a tile (8 KB)
+constexpr int kStage = 4 * kHalf;             // K lo/hi + V lo/hi (32 KB)
+constexpr int kGroupWarps = 4;                // consumer warps that share a tile
+constexpr int kConsumers = 2 * kGroupWarps;
+constexpr int kThreads = (kConsumers + 1) * 32;
+constexpr int kMaxB = 65536;
+
+// WIDE: Hq / Hkv in 9..16 (both row halves of the MMA's A operand are used and
+// the merge buffer doubles, which leaves room for one stage less)
+template <bool WIDE>
+struct Cfg {
+  static constexpr int kRows = WIDE ? 16 : 8;
+  static constexpr int kStages = WIDE ? 5 : 6;
+  static constexpr int kOffMerge = kStages * kStage;
+  static constexpr int kMergeBytes = kConsumers * kRows * (kD + 2) * 4;
+  static constexpr int kOffBar = kOffMerge + kMergeBytes;
+  static constexpr int kSmem = kOffBar + 2 * kStages * 8 + 1024;  // + alignment slack
+};
+static_assert(Cfg<false>::kSmem <= 227 * 1024 && Cfg<true>::kSmem <= 227 * 1024, "shared memory");
+
+struct RaggedDecodeParams {
+  const __nv_bfloat16* q;
+  int64_t q_stride;
+  __nv_bfloat16* out;
+  int64_t out_stride;
+  const int32_t* table;
+  int64_t table_stride;
+  const int32_t* kv_lens;
+  float* ws_acc;   // [2 * grid][G][128] unnormalised pieces
+  float* ws_ml;    // [2 * grid][G][2]   running max (log2 units) and sum
+  int2* ws_desc;   // [grid] {pair whose first piece ends CTA c's range or -1, last CTA of it}
+  int B, Hkv, G, page_tokens, num_pages, capacity;
+  float scale_log2;
+  int* err;
+};
+
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+// Byte offset of 16-byte chunk c (0..15) of row r in a tile's K or V half pair.
+__device__ __forceinline__ uint32_t kv_at(int r, int c) {
+  return (c >> 3) * kHalf + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Length of request b, inside what its table row can hold.
+__device__ __forceinline__ int req_len(const RaggedDecodeParams& p, int b, bool* bad) {
+  const int L = p.kv_lens[b];
+  if (L < 0 || L > p.capacity) *bad = true;
+  return min(max(L, 0), p.capacity);
+}
+
+// The pieces of a CTA's range, in order: pair (b, kvh), tiles [t0, t1) of nt.
+struct Piece {
+  int b, kvh, t0, t1, nt, L;
+};
+struct Walk {
+  int b, kvh, tile, nt, L;
+  int64_t left;
+  __device__ __forceinline__ bool next(const RaggedDecodeParams& p, Piece& w) {
+    if (left <= 0) return false;
+    bool bad = false;
+    while (tile >= nt) {  // the next pair that has tiles
+      tile = 0;
+      if (nt > 0 && ++kvh < p.Hkv) break;
+      kvh = 0;
+      if (++b >= p.B) return false;
+      L = req_len(p, b, &bad);
+      nt = (L + kTile - 1) / kTile;
+    }
+    w.b = b;
+    w.kvh = kvh;
+    w.t0 = tile;
+    w.nt = nt;
+    w.L = L;
+    const int64_t n = min64(left, nt - tile);
+    w.t1 = tile + (int)n;
+    tile = w.t1;
+    left -= n;
+    return true;
+  }
+};
+
+template <bool WIDE>
+__global__ void __launch_bounds__(kThreads, 1)
+    ragged_decode_kernel(const __grid_constant__ CUtensorMap tmK,
+                         const __grid_constant__ CUtensorMap tmV, RaggedDecodeParams p) {
+  using C = Cfg<WIDE>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~uintptr_t(1023));
+  float* sm_o = reinterpret_cast<float*>(smem + C::kOffMerge);  // [warp][row][128]
+  float* sm_ml = sm_o + kConsumers * C::kRows * kD;             // [warp][row][2]
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
+  uint64_t* empty = full + C::kStages;
+  __shared__ int64_t s_warp[kThreads / 32];
+  __shared__ int s_start[4];  // b, tile inside the request's Hkv * nt, nt, L
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], kGroupWarps);
+    }
+    fence_mbar_init();
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
+    s_start[0] = p.B;
+    s_start[1] = s_start[2] = s_start[3] = 0;
+  }
+  pdl_launch();
+  pdl_wait();
+
+  // ---- this CTA's range of the tile list (every CTA scans the lengths) ----
+  const int per = (p.B + kThreads - 1) / kThreads;
+  const int b0 = min((int)threadIdx.x * per, p.B), b1 = min(b0 + per, p.B);
+  int64_t mine = 0;
+  bool bad = false;
+  for (int b = b0; b < b1; ++b) mine += (req_len(p, b, &bad) + kTile - 1) / kTile;
+  mine *= p.Hkv;
+  if (bad && blockIdx.x == 0) report_timeout(p.err, 0x921);
+  int64_t incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t y = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += y;
+  }
+  if (lane == 31) s_warp[warp] = incl;
+  __syncthreads();
+  int64_t before = incl - mine, U = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) {
+    if (w < warp) before += s_warp[w];
+    U += s_warp[w];
+  }
+  const int64_t nc = min64(gridDim.x, U);  // CTAs that get tiles
+  const int c = blockIdx.x;
+  const int64_t u0 = c < nc ? U * c / nc : U, u1 = c < nc ? U * (c + 1) / nc : U;
+  if (u0 < u1 && before <= u0 && u0 < before + mine) {
+    int64_t at = before;
+    for (int b = b0; b < b1; ++b) {
+      const int L = req_len(p, b, &bad), nt = (L + kTile - 1) / kTile;
+      const int64_t n = (int64_t)nt * p.Hkv;
+      if (u0 < at + n) {
+        s_start[0] = b;
+        s_start[1] = (int)(u0 - at);
+        s_start[2] = nt;
+        s_start[3] = L;
+        break;
+      }
+      at += n;
+    }
+  }
+  __syncthreads();
+  Walk walk;
+  walk.b = s_start[0];
+  walk.nt = s_start[2];
+  walk.L = s_start[3];
+  walk.kvh = walk.nt > 0 ? s_start[1] / walk.nt : 0;
+  walk.tile = walk.nt > 0 ? s_start[1] - walk.kvh * walk.nt : 0;
+  walk.left = u1 - u0;
+  Piece w;
+
+  if (warp == kConsumers) {
+    // ------------------------------ TMA producer ------------------------------
+    int it = 0;
+    bool ok = true;
+    while (ok && walk.next(p, w)) {
+      int pages = 0;  // this lane's entry of 32 tiles' pages
+      for (int t = w.t0; t < w.t1; ++t, ++it) {
+        const int k = (t - w.t0) & 31;
+        if (k == 0) {
+          const int tl = t + lane;
+          if (tl < w.t1) {
+            // a 64-position tile never straddles pages (page_tokens % 64 == 0)
+            pages = p.table[w.b * p.table_stride + (uint32_t)tl * kTile / (uint32_t)p.page_tokens];
+            if (pages < 0 || pages >= p.num_pages) {  // recorded, page 0 read in its place
+              report_timeout(p.err, 0x922);
+              pages = 0;
+            }
+          }
+        }
+        const int pg = __shfl_sync(0xffffffffu, pages, k);
+        const int s = it % C::kStages;
+        if (lane == 0) {
+          if (it >= C::kStages &&
+              !mbar_wait(&empty[s], ((it / C::kStages) - 1) & 1, p.err, 0x923)) {
+            ok = false;
+          } else {
+            const int y = (int)(((int64_t)pg * p.Hkv + w.kvh) * p.page_tokens +
+                                (uint32_t)t * kTile % (uint32_t)p.page_tokens);
+            uint8_t* st = smem + s * kStage;
+            mbar_arrive_expect_tx(&full[s], kStage);
+            tma_load_2d(st, &tmK, &full[s], 0, y, kCacheEvictFirst);
+            tma_load_2d(st + kHalf, &tmK, &full[s], 64, y, kCacheEvictFirst);
+            tma_load_2d(st + 2 * kHalf, &tmV, &full[s], 0, y, kCacheEvictFirst);
+            tma_load_2d(st + 3 * kHalf, &tmV, &full[s], 64, y, kCacheEvictFirst);
+          }
+        }
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+      }
+    }
+    // the copies issued land before the CTA may exit (the consumers wait for
+    // every one of them unless a wait ran out)
+    if (!ok && lane == 0)
+      for (int i = max(0, it - C::kStages); i < it; ++i)
+        mbar_wait(&full[i % C::kStages], (i / C::kStages) & 1, nullptr, 0);
+  } else {
+    // ------------------------------- consumers --------------------------------
+    const int group = warp / kGroupWarps, band = warp % kGroupWarps;
+    const int g = lane >> 2, t4 = lane & 3;
+    const uint32_t ring = smem_u32(smem);
+    bool ok = true;
+    int it = 0;
+    if (threadIdx.x == 0) p.ws_desc[c] = make_int2(-1, -1);
+    int64_t u = u0;  // first unit of the piece
+    while (walk.next(p, w)) {
+      // Q as the A operand: row g (and g + 8) = query head kvh * G + row
+      uint32_t qf[8][WIDE ? 4 : 2];
+      {
+        const __nv_bfloat16* qh =
+            p.q + w.b * p.q_stride + (int64_t)(w.kvh * p.G) * kD + 2 * t4;
+#pragma unroll
+        for (int ks = 0; ks < 8; ++ks)
+#pragma unroll
+          for (int e = 0; e < (WIDE ? 4 : 2); ++e) {
+            // registers: (row g, k lo), [row g+8, k lo], (row g, k hi), [row g+8, k hi]
+            const int row = WIDE ? g + 8 * (e & 1) : g;
+            const int col = ks * 16 + 8 * (WIDE ? (e >> 1) : e);
+            qf[ks][e] = row < p.G ? *reinterpret_cast<const uint32_t*>(qh + row * kD + col) : 0u;
+          }
+      }
+      float o[16][WIDE ? 4 : 2];
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+#pragma unroll
+        for (int e = 0; e < (WIDE ? 4 : 2); ++e) o[i][e] = 0.f;
+      float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+
+      for (int t = w.t0; t < w.t1; ++t, ++it) {
+        if ((it & 1) != group) continue;
+        const int s = it % C::kStages;
+        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&full[s], (it / C::kStages) & 1, p.err, 0x924));
+        if (!ok) continue;
+        const uint32_t sK = ring + s * kStage, sV = sK + 2 * kHalf;
+        const int pos0 = t * kTile + band * 16;
+        // ---- S = Q K^T: 16 rows x 16 positions (two n-tiles of 8) ----
+        float sc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+        for (int ks = 0; ks < 8; ++ks) {
+          uint32_t kf[4];
+          const int r = band * 16 + (lane & 7) + ((lane >> 4) << 3);
+          ldsm4(kf, sK + kv_at(r, ks * 2 + ((lane >> 3) & 1)));
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            if constexpr (WIDE)
+              mma_bf16_16816(sc[j], qf[ks][0], qf[ks][1], qf[ks][2], qf[ks][3], kf[2 * j],
+                             kf[2 * j + 1]);
+            else
+              mma_bf16_16816(sc[j], qf[ks][0], 0u, qf[ks][1], 0u, kf[2 * j], kf[2 * j + 1]);
+          }
+        }
+        const bool tail = pos0 + 16 > w.L;
+        if (tail) {
+          // V rows past the end hold whatever the page held before: 0 * V must
+          // be 0, so this warp's rows there become zeros (the ring's next copy
+          // into the stage is ordered behind the fence and the release below)
+#pragma unroll
+          for (int i = lane; i < 16 * 16; i += 32) {
+            const int r = band * 16 + (i >> 4);
+            if (t * kTile + r >= w.L)
+              asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(sV + kv_at(r, i & 15)),
+                           "r"(0u)
+                           : "memory");
+          }
+          __syncwarp();
+        }
+        // ---- running max and sum per row; P as the A operand of P V ----
+        uint32_t pa[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+        for (int hh = 0; hh < (WIDE ? 2 : 1); ++hh) {
+          float x[4];
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int pos = pos0 + j * 8 + 2 * t4 + e;
+              x[j * 2 + e] = pos < w.L ? sc[j][hh * 2 + e] * p.scale_log2 : -INFINITY;
+            }
+          float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+          const float m_new = fmaxf(m[hh], mx);
+          const float base = m_new == -INFINITY ? 0.f : m_new;
+          const float corr = ex2(m[hh] - base);
+          float rs = 0.f;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            x[e] = ex2(x[e] - base);
+            rs += x[e];
+          }
+          l[hh] = l[hh] * corr + rs;
+          m[hh] = m_new;
+#pragma unroll
+          for (int d = 0; d < 16; ++d) {
+            o[d][hh * 2] *= corr;
+            o[d][hh * 2 + 1] *= corr;
+          }
+          pa[hh] = pack_bf16x2(x[0], x[1]);
+          pa[2 + hh] = pack_bf16x2(x[2], x[3]);
+        }
+        // ---- O += P V ----
+#pragma unroll
+        for (int ip = 0; ip < 8; ++ip) {
+          uint32_t vf[4];
+          const int r = band * 16 + (lane & 7) + (((lane >> 3) & 1) << 3);
+          ldsm4t(vf, sV + kv_at(r, ip * 2 + (lane >> 4)));
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            float(&oo)[WIDE ? 4 : 2] = o[2 * ip + j];
+            if constexpr (WIDE) {
+              mma_bf16_16816(oo, pa[0], pa[1], pa[2], pa[3], vf[2 * j], vf[2 * j + 1]);
+            } else {
+              float d4[4] = {oo[0], oo[1], 0.f, 0.f};
+              mma_bf16_16816(d4, pa[0], 0u, pa[2], 0u, vf[2 * j], vf[2 * j + 1]);
+              oo[0] = d4[0];
+              oo[1] = d4[1];
+            }
+          }
+        }
+        if (tail) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[s]);
+      }
+
+      // ---- merge the eight warps; write the output or this CTA's piece ----
+#pragma unroll
+      for (int hh = 0; hh < (WIDE ? 2 : 1); ++hh) {
+        float ls = l[hh];
+        ls += __shfl_xor_sync(0xffffffffu, ls, 1);
+        ls += __shfl_xor_sync(0xffffffffu, ls, 2);
+        const int row = g + 8 * hh;
+        if (row < p.G) {
+          float* dst = sm_o + (warp * C::kRows + row) * kD;
+#pragma unroll
+          for (int d = 0; d < 16; ++d)
+            *reinterpret_cast<float2*>(dst + d * 8 + 2 * t4) =
+                make_float2(o[d][hh * 2], o[d][hh * 2 + 1]);
+          if (t4 == 0)
+            *reinterpret_cast<float2*>(sm_ml + (warp * C::kRows + row) * 2) =
+                make_float2(m[hh], ls);
+        }
+      }
+      asm volatile("bar.sync 1, %0;" ::"n"(kConsumers * 32) : "memory");
+      const bool whole = w.t0 == 0 && w.t1 == w.nt;
+      // a piece that ends this CTA's range but not its pair has the odd slot
+      // unless it also began inside the pair
+      const int slot = 2 * c + (w.t0 == 0 ? 1 : 0);
+      for (int idx = threadIdx.x; idx < p.G * kD; idx += kConsumers * 32) {
+        const int row = idx / kD, d = idx % kD;
+        float M = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kConsumers; ++i)
+          M = fmaxf(M, sm_ml[(i * C::kRows + row) * 2]);
+        float a = 0.f, ls = 0.f;
+#pragma unroll
+        for (int i = 0; i < kConsumers; ++i) {
+          const float mi = sm_ml[(i * C::kRows + row) * 2];
+          const float f = mi == -INFINITY ? 0.f : ex2(mi - M);
+          a = fmaf(f, sm_o[(i * C::kRows + row) * kD + d], a);
+          ls = fmaf(f, sm_ml[(i * C::kRows + row) * 2 + 1], ls);
+        }
+        if (whole) {
+          p.out[w.b * p.out_stride + (int64_t)(w.kvh * p.G + row) * kD + d] = f2bf(a / ls);
+        } else {
+          p.ws_acc[((int64_t)slot * p.G + row) * kD + d] = a;
+          if (d == 0) {
+            p.ws_ml[((int64_t)slot * p.G + row) * 2] = M;
+            p.ws_ml[((int64_t)slot * p.G + row) * 2 + 1] = ls;
+          }
+        }
+      }
+      if (threadIdx.x == 0 && w.t0 == 0 && !whole) {
+        // the CTA that holds the pair's last tile: the largest k with U k / nc <= it
+        const int64_t last = u + w.nt - 1;
+        p.ws_desc[c] = make_int2(w.b * p.Hkv + w.kvh, (int)(((last + 1) * nc - 1) / U));
+      }
+      u += w.t1 - w.t0;
+      asm volatile("bar.sync 1, %0;" ::"n"(kConsumers * 32) : "memory");
+    }
+    // requests with nothing cached: zeros
+    const int Hq = p.Hkv * p.G;
+    for (int b = c; b < p.B; b += gridDim.x)
+      if (p.kv_lens[b] <= 0)
+        for (int i = threadIdx.x; i < Hq * kD / 8; i += kConsumers * 32)
+          reinterpret_cast<uint4*>(p.out + b * p.out_stride)[i] = make_uint4(0, 0, 0, 0);
+  }
+}
+
+// Joins the pieces of the pair whose first piece ends CTA c's range: pieces
+// 2c+1, 2(c+1), 2(c+2), ..., 2*last.  One CTA per (c, query head of the pair).
+constexpr int kJoinWarps = 8;
+constexpr int kMaxGrid = 512;
+__global__ void __launch_bounds__(kJoinWarps * 32) ragged_decode_join(RaggedDecodeParams p) {
+  __shared__ float s_f[kMaxGrid];
+  __shared__ float s_red[kJoinWarps][2];
+  __shared__ __align__(16) float s_acc[kJoinWarps][kD];
+  pdl_launch();
+  pdl_wait();
+  const int c = blockIdx.x, row = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int2 d = p.ws_desc[c];
+  if (d.x < 0) return;
+  const int n = d.y - c + 1;  // pieces, at most the first kernel's grid (<= kMaxGrid)
+  auto piece = [&](int i) { return ((int64_t)(i == 0 ? 2 * c + 1 : 2 * (c + i)) * p.G + row); };
+  float M = -INFINITY;
+  for (int i = threadIdx.x; i < n; i += kJoinWarps * 32) {
+    const float mi = p.ws_ml[piece(i) * 2];
+    s_f[i] = mi;
+    M = fmaxf(M, mi);
+  }
+  M = warp_max(M);
+  if (lane == 0) s_red[warp][0] = M;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kJoinWarps; ++i) M = fmaxf(M, s_red[i][0]);
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+  float l = 0.f;
+#pragma unroll 4
+  for (int i = warp; i < n; i += kJoinWarps) {
+    const float f = ex2(s_f[i] - M);
+    const float4 x = *reinterpret_cast<const float4*>(p.ws_acc + piece(i) * kD + lane * 4);
+    l = fmaf(f, p.ws_ml[piece(i) * 2 + 1], l);
+    a.x = fmaf(f, x.x, a.x);
+    a.y = fmaf(f, x.y, a.y);
+    a.z = fmaf(f, x.z, a.z);
+    a.w = fmaf(f, x.w, a.w);
+  }
+  *reinterpret_cast<float4*>(&s_acc[warp][lane * 4]) = a;
+  if (lane == 0) s_red[warp][1] = l;
+  __syncthreads();
+  if (threadIdx.x < kD) {
+    float x = 0.f, ls = 0.f;
+#pragma unroll
+    for (int i = 0; i < kJoinWarps; ++i) {
+      x += s_acc[i][threadIdx.x];
+      ls += s_red[i][1];
+    }
+    const int b = d.x / p.Hkv, kvh = d.x - b * p.Hkv;
+    p.out[b * p.out_stride + (int64_t)(kvh * p.G + row) * kD + threadIdx.x] = f2bf(x / ls);
+  }
+}
+
+int decode_grid() { return (int)min64(num_sms(), kMaxGrid); }
+
+size_t decode_ws(int G, size_t* off_ml, size_t* off_desc) {
+  const size_t slots = 2 * (size_t)decode_grid();
+  size_t n = slots * G * kD * 4;
+  *off_ml = n;
+  n += slots * G * 8;
+  *off_desc = n;
+  return n + decode_grid() * sizeof(int2);
+}
+
+}  // namespace
+}  // namespace q3
+
+extern "C" size_t q3_attn_decode_ragged_workspace_bytes(int Hq, int Hkv) {
+  if (Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || Hq / Hkv > 16) return 0;
+  size_t a, b;
+  return q3::decode_ws(Hq / Hkv, &a, &b);
+}
+
+extern "C" int q3_attn_decode_ragged(const void* q, int64_t q_stride, const void* k_pages,
+                                     const void* v_pages, void* out, int64_t out_stride, int B,
+                                     int Hq, int Hkv, int head_dim, const int32_t* block_table,
+                                     int64_t table_stride, int table_width, int page_tokens,
+                                     int64_t num_pages, const int32_t* kv_lens, float scale,
+                                     void* workspace, size_t workspace_bytes,
+                                     q3_stream_t stream) {
+  using namespace q3;
+  Q3_REQUIRE(head_dim == kD, "q3_attn_decode_ragged: head_dim must be 128 (got %d)", head_dim);
+  Q3_REQUIRE(B >= 0 && B <= kMaxB && Hq > 0 && Hkv > 0 && Hkv <= 1024 && Hq % Hkv == 0,
+             "q3_attn_decode_ragged: bad shape B=%d Hq=%d Hkv=%d", B, Hq, Hkv);
+  if (Hq / Hkv > 16)
+    return fail(Q3_ERR_UNSUPPORTED, "q3_attn_decode_ragged: Hq/Hkv=%d above 16", Hq / Hkv);
+  if (B == 0) return Q3_OK;
+  Q3_REQUIRE(q && k_pages && v_pages && out && block_table && kv_lens && workspace,
+             "q3_attn_decode_ragged: null pointer");
+  Q3_REQUIRE(page_tokens > 0 && page_tokens % kTile == 0,
+             "q3_attn_decode_ragged: page_tokens=%d must be a positive multiple of %d",
+             page_tokens, kTile);
+  Q3_REQUIRE(table_width > 0 && table_stride >= table_width && num_pages > 0 &&
+                 (int64_t)table_width * page_tokens < (1ll << 31),
+             "q3_attn_decode_ragged: table width %d, stride %lld, %lld pages", table_width,
+             (long long)table_stride, (long long)num_pages);
+  Q3_REQUIRE(num_pages * Hkv * page_tokens < (1ll << 31),
+             "q3_attn_decode_ragged: the pool is too large for 32-bit TMA rows");
+  Q3_REQUIRE(q_stride >= (int64_t)Hq * kD && out_stride >= (int64_t)Hq * kD &&
+                 q_stride % 2 == 0 && out_stride % 8 == 0,
+             "q3_attn_decode_ragged: row strides");
+  Q3_REQUIRE(aligned(q, 4) && aligned(k_pages, 16) && aligned(v_pages, 16) && aligned(out, 16) &&
+                 aligned(block_table, 4) && aligned(kv_lens, 4) && aligned(workspace, 16),
+             "q3_attn_decode_ragged: misaligned pointer");
+  const int G = Hq / Hkv;
+  size_t off_ml, off_desc;
+  const size_t need = decode_ws(G, &off_ml, &off_desc);
+  Q3_REQUIRE(workspace_bytes >= need, "q3_attn_decode_ragged: workspace of %zu bytes, need %zu",
+             workspace_bytes, need);
+  CUtensorMap tk, tv;
+  const int64_t rows = num_pages * Hkv * page_tokens;
+  int rc = make_tmap_2d(&tk, k_pages, rows, kD, kTile, 64);
+  if (rc) return rc;
+  rc = make_tmap_2d(&tv, v_pages, rows, kD, kTile, 64);
+  if (rc) return rc;
+  uint8_t* ws = (uint8_t*)workspace;
+  RaggedDecodeParams p{(const __nv_bfloat16*)q, q_stride, (__nv_bfloat16*)out, out_stride,
+                       block_table, table_stride, kv_lens, (float*)ws, (float*)(ws + off_ml),
+                       (int2*)(ws + off_desc), B, Hkv, G, page_tokens, (int)num_pages,
+                       table_width * page_tokens, scale * 1.4426950408889634f,
+                       device_error_word()};
+  static bool attr_set[64] = {false};
+  int dev = 0;
+  Q3_CUDA_CHECK(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64 || !attr_set[dev]) {
+    Q3_CUDA_CHECK(cudaFuncSetAttribute(ragged_decode_kernel<false>,
+                                       cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       Cfg<false>::kSmem));
+    Q3_CUDA_CHECK(cudaFuncSetAttribute(ragged_decode_kernel<true>,
+                                       cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       Cfg<true>::kSmem));
+    if (dev >= 0 && dev < 64) attr_set[dev] = true;
+  }
+  const dim3 grid((unsigned)decode_grid());
+  rc = G > 8 ? launch_ex(ragged_decode_kernel<true>, grid, dim3(kThreads), Cfg<true>::kSmem,
+                         (cudaStream_t)stream, 1, tk, tv, p)
+             : launch_ex(ragged_decode_kernel<false>, grid, dim3(kThreads), Cfg<false>::kSmem,
+                         (cudaStream_t)stream, 1, tk, tv, p);
+  if (rc) return rc;
+  return launch_ex(ragged_decode_join, dim3(grid.x, (unsigned)G), dim3(kJoinWarps * 32), 0,
+                   (cudaStream_t)stream, 1, p);
+}

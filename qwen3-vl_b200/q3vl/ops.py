@@ -9,6 +9,7 @@ from __future__ import annotations
 import ctypes
 import math
 import os
+from typing import NamedTuple
 
 import torch
 
@@ -999,6 +1000,200 @@ def l2_prefetch(t: torch.Tensor) -> None:
     _cuda("l2_prefetch", t)
     _contig("l2_prefetch", t)
     call("q3_l2_prefetch", _p(t), t.numel() * t.element_size(), _stream())
+
+
+# ----------------------------------------------------------------------------
+# ragged serving step over paged K/V: requests of different lengths in one call
+# ----------------------------------------------------------------------------
+class RaggedPlan(NamedTuple):
+    """What a step's lengths map to (ragged_plan); all on the device."""
+    cu_q: torch.Tensor       # int32 [B + 1] first packed token of each request
+    kv_lens: torch.Tensor    # int32 [B] positions cached once the step has run
+    requests: torch.Tensor   # int32 [n_tokens] request of each packed token, -1 behind the last
+    positions: torch.Tensor  # int64 [n_tokens] rotary position, 0 behind the last
+    slots: torch.Tensor      # int64 [n_tokens] page * page_tokens + offset, -1 behind the last
+    counts: torch.Tensor     # int32 [2] packed tokens, pages taken from the free list
+
+
+def _ragged_device(name: str, *ts) -> torch.device:
+    """The one CUDA device of the tensors."""
+    dev = ts[0].device
+    for t in ts:
+        if t is not None and (not t.is_cuda or t.device != dev):
+            raise RuntimeError(f"{name}: tensors must be on one CUDA device (no CPU fallback); "
+                               f"got {dev} and {t.device}")
+    return dev
+
+
+def _ragged_call(name: str, dev: torch.device, *args) -> None:
+    """call() on the current stream of the tensors' own device."""
+    if dev.index == torch.cuda.current_device():
+        call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
+    else:
+        with torch.cuda.device(dev):
+            call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
+
+
+def _ragged_ints(name: str, dtype, **ts) -> None:
+    for k, t in ts.items():
+        if t is not None and (t.dtype != dtype or not t.is_contiguous()):
+            raise TypeError(f"{name}: {k} must be contiguous {dtype}")
+
+
+def _ragged_rows(name: str, what: str, t: torch.Tensor) -> int:
+    """Row stride of a bf16 [rows, heads, 128] tensor whose rows are dense."""
+    rows, heads, d = t.shape
+    s0, s1, s2 = t.stride()
+    if t.dtype != torch.bfloat16:
+        raise TypeError(f"{name}: {what} must be bfloat16, got {t.dtype}")
+    if d != HEAD_DIM or s2 != 1 or (s1 != HEAD_DIM and heads > 1):
+        raise ValueError(f"{name}: {what} must be [rows, heads, 128] with dense rows, got "
+                         f"{tuple(t.shape)} with strides {t.stride()}")
+    return s0 if rows > 1 else heads * HEAD_DIM
+
+
+def _ragged_pool(name: str, k_pages: torch.Tensor, v_pages: torch.Tensor):
+    if k_pages.dtype != torch.bfloat16 or v_pages.dtype != torch.bfloat16:
+        raise TypeError(f"{name}: k_pages and v_pages must be bfloat16")
+    if (k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.shape[3] != HEAD_DIM or
+            not k_pages.is_contiguous() or not v_pages.is_contiguous()):
+        raise ValueError(f"{name}: k_pages and v_pages must be contiguous "
+                         f"[num_pages, Hkv, page_tokens, 128], got {tuple(k_pages.shape)} and "
+                         f"{tuple(v_pages.shape)}")
+    return k_pages.shape[:3]
+
+
+def _ragged_table(name: str, t: torch.Tensor, B: int) -> int:
+    """Row stride of an int32 [B, width] block table."""
+    if t.dtype != torch.int32:
+        raise TypeError(f"{name}: block_table must be int32, got {t.dtype}")
+    if t.dim() != 2 or t.shape[0] != B or (t.stride(1) != 1 and t.shape[1] > 1):
+        raise ValueError(f"{name}: block_table must be [{B}, width] with dense rows, got "
+                         f"{tuple(t.shape)} with strides {t.stride()}")
+    return t.stride(0) if B > 1 else t.shape[1]
+
+
+def ragged_plan(q_lens: torch.Tensor, past_lens: torch.Tensor, block_table: torch.Tensor, *,
+                page_tokens: int, n_tokens: int, free_pages: torch.Tensor = None,
+                rope_delta: torch.Tensor = None) -> RaggedPlan:
+    """Block tables, slot map and positions of a step, from the requests' lengths.
+
+    q_lens, past_lens int32 [B] on the device: new tokens and cached positions
+    of each request.  block_table int32 [B, width] is filled in place with pages
+    of free_pages (int32 [n], in order) for the positions that need new ones;
+    without free_pages it must map every position already
+    (KVPagePool.device_table).  n_tokens is the packed buffer's size: rows behind
+    the last request get request -1, position 0 and slot -1.  rope_delta int64
+    [B] or [B, 1] (rope_index) shifts the rotary positions.  Nothing is read
+    back: counts[1] pages of the list were taken (more than its length, and
+    0x903 in the device error word, when it was short)."""
+    name = "ragged_plan"
+    dev = _ragged_device(name, q_lens, past_lens, block_table, free_pages, rope_delta)
+    _ragged_ints(name, torch.int32, q_lens=q_lens, past_lens=past_lens, free_pages=free_pages)
+    _ragged_ints(name, torch.int64, rope_delta=rope_delta)
+    B = q_lens.numel()
+    if past_lens.numel() != B or (rope_delta is not None and rope_delta.numel() != B):
+        raise ValueError(f"{name}: past_lens and rope_delta must have {B} entries")
+    stride = _ragged_table(name, block_table, B)
+    n = int(n_tokens)
+    if n < 0:
+        raise ValueError(f"{name}: n_tokens={n}")
+    i64 = torch.empty(2, n, dtype=torch.int64, device=dev)
+    i32 = torch.empty(n + 2 * B + 3, dtype=torch.int32, device=dev)
+    requests, cu_q, kv_lens, counts = i32.split((n, B + 1, B, 2))
+    at64, at32 = i64.data_ptr(), i32.data_ptr()
+    _ragged_call("q3_ragged_plan", dev, q_lens.data_ptr(), past_lens.data_ptr(), B,
+                 block_table.data_ptr(), stride, block_table.shape[1], int(page_tokens),
+                 None if free_pages is None else free_pages.data_ptr(),
+                 0 if free_pages is None else free_pages.numel(),
+                 None if rope_delta is None else rope_delta.data_ptr(), n, at32 + 4 * n,
+                 at32 + 4 * (n + B + 1), at32, at64, at64 + 8 * n, at32 + 4 * (n + 2 * B + 1))
+    return RaggedPlan(cu_q, kv_lens, requests, i64[0], i64[1], counts)
+
+
+def qkv_norm_rope_ragged(qkv: torch.Tensor, q_norm_w: torch.Tensor, k_norm_w: torch.Tensor,
+                         positions: torch.Tensor, inv_freq: torch.Tensor, slots: torch.Tensor,
+                         k_pages: torch.Tensor, v_pages: torch.Tensor, *, Hq: int, Hkv: int,
+                         mrope_section=(24, 20, 20), eps: float = 1e-6,
+                         out: torch.Tensor = None) -> torch.Tensor:
+    """Per-head QK-RMSNorm, rotary positions and the K/V write of packed tokens.
+
+    qkv bf16 [n, (Hq + 2 Hkv) * 128]; positions int64 [n] (text) or [3, n]
+    (time, height, width, interleaved by mrope_section); inv_freq f32 [64];
+    slots int64 [n] (RaggedPlan.slots; distinct, or -1 for a padding token, of
+    which nothing is read or written).  Returns q [n, Hq, 128].  Computed in
+    fp32 and rounded once, without the bf16 tables and rounding points of
+    qkv_norm_rope, so the last bit of a value may differ from it."""
+    name = "qkv_norm_rope_ragged"
+    dev = _ragged_device(name, qkv, q_norm_w, k_norm_w, positions, inv_freq, slots, k_pages,
+                         v_pages, out)
+    _bf16(name, qkv, q_norm_w, k_norm_w)
+    _ragged_ints(name, torch.int64, slots=slots)
+    num_pages, heads, page_tokens = _ragged_pool(name, k_pages, v_pages)
+    if heads != Hkv:
+        raise ValueError(f"{name}: the pool has {heads} K/V heads, Hkv is {Hkv}")
+    width = (Hq + 2 * Hkv) * HEAD_DIM
+    if qkv.dim() != 2 or qkv.shape[1] != width or qkv.stride(1) != 1:
+        raise ValueError(f"{name}: qkv must be [n, {width}] with dense rows")
+    n = qkv.shape[0]
+    if positions.dtype != torch.int64 or positions.dim() not in (1, 2) or \
+            (positions.dim() == 2 and positions.shape[0] != 3) or positions.shape[-1] != n or \
+            (positions.stride(-1) != 1 and n > 1):
+        raise ValueError(f"{name}: positions must be int64 [{n}] or [3, {n}]")
+    if slots.numel() != n:
+        raise ValueError(f"{name}: {slots.numel()} slots for {n} tokens")
+    if q_norm_w.numel() != HEAD_DIM or k_norm_w.numel() != HEAD_DIM or \
+            not q_norm_w.is_contiguous() or not k_norm_w.is_contiguous():
+        raise ValueError(f"{name}: norm weights must be contiguous [128]")
+    if inv_freq.dtype != torch.float32 or inv_freq.numel() != HEAD_DIM // 2 or \
+            not inv_freq.is_contiguous():
+        raise ValueError(f"{name}: inv_freq must be contiguous float32 [64]")
+    if out is None:
+        out = torch.empty(n, Hq, HEAD_DIM, dtype=torch.bfloat16, device=dev)
+    elif tuple(out.shape) != (n, Hq, HEAD_DIM):
+        raise ValueError(f"{name}: out must be [{n}, {Hq}, 128]")
+    _ragged_call("q3_qkv_norm_rope_ragged", dev, qkv.data_ptr(),
+                 qkv.stride(0) if n > 1 else width, q_norm_w.data_ptr(), k_norm_w.data_ptr(),
+                 positions.data_ptr(), positions.stride(0) if positions.dim() == 2 else 0,
+                 inv_freq.data_ptr(), slots.data_ptr(), out.data_ptr(),
+                 _ragged_rows(name, "out", out), k_pages.data_ptr(), v_pages.data_ptr(), n, Hq,
+                 Hkv, HEAD_DIM, page_tokens, num_pages, int(mrope_section[1]),
+                 int(mrope_section[2]), float(eps))
+    return out
+
+
+def attn_decode_ragged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                       block_table: torch.Tensor, kv_lens: torch.Tensor, scale: float = None,
+                       out: torch.Tensor = None) -> torch.Tensor:
+    """Attention of one new token per request over its own length of the pool.
+
+    q bf16 [B, Hq, 128] (any row stride); k_pages / v_pages [num_pages, Hkv,
+    page_tokens, 128]; block_table int32 [B, width]; kv_lens int32 [B] on the
+    device: request b attends to positions [0, kv_lens[b]), and a length of 0
+    gives zeros.  Hq / Hkv is any whole number up to 16."""
+    name = "attn_decode_ragged"
+    dev = _ragged_device(name, q, k_pages, v_pages, block_table, kv_lens, out)
+    _ragged_ints(name, torch.int32, kv_lens=kv_lens)
+    num_pages, Hkv, page_tokens = _ragged_pool(name, k_pages, v_pages)
+    if q.dim() != 3:
+        raise ValueError(f"{name}: q must be [B, Hq, 128]")
+    q_stride = _ragged_rows(name, "q", q)
+    B, Hq, D = q.shape
+    if kv_lens.numel() != B:
+        raise ValueError(f"{name}: {kv_lens.numel()} lengths for {B} requests")
+    table_stride = _ragged_table(name, block_table, B)
+    if out is None:
+        out = torch.empty(B, Hq, D, dtype=torch.bfloat16, device=dev)
+    elif out.shape != q.shape:
+        raise ValueError(f"{name}: out must match q")
+    nbytes = _lib.raw("q3_attn_decode_ragged_workspace_bytes")(Hq, Hkv)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    _ragged_call("q3_attn_decode_ragged", dev, q.data_ptr(), q_stride, k_pages.data_ptr(),
+                 v_pages.data_ptr(), out.data_ptr(), _ragged_rows(name, "out", out), B, Hq, Hkv, D,
+                 block_table.data_ptr(), table_stride, block_table.shape[1], page_tokens,
+                 num_pages, kv_lens.data_ptr(),
+                 1.0 / math.sqrt(D) if scale is None else float(scale), ws.data_ptr(), nbytes)
+    return out
 
 
 def device_error(clear: bool = True) -> int:

@@ -1,0 +1,297 @@
+"""Ragged serving operators on the GPU against their 64-bit forms: plan, norm +
+rotary + slots, decode attention; sizes and lengths at tile and page borders,
+padding, stale NaN rows, strides, bad entries, graphs and streams."""
+import math
+
+import pytest
+import torch
+
+from q3vl import ops
+from tests import ragged_oracle as ora
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+BF16 = torch.bfloat16
+
+
+@pytest.fixture(autouse=True)
+def clean_error_word():
+    ops.device_error(clear=True)
+    yield
+    assert ops.device_error(clear=True) == 0
+
+
+def i32(x):
+    return torch.tensor(x, dtype=torch.int32, device=DEV)
+
+
+def rnd(*shape, seed=0, std=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(*shape, generator=g) * std).to(BF16)
+
+
+# ------------------------------------------------------------------ the plan
+PLANS = [
+    ([1] * 8, [384, 1998, 116, 1596, 1772, 8, 1824, 0], 256, 0),
+    ([0], [0], 64, 3),
+    ([1], [63], 64, 0),
+    ([1], [64], 64, 0),
+    ([65, 0, 1, 128, 0, 64], [0, 5, 63, 64, 0, 1], 64, 37),
+    ([3] * 600, list(range(600)), 64, 1),               # more requests than threads
+    ([700, 1, 0, 2500], [190, 191, 192, 193], 192, 130),
+]
+
+
+@pytest.mark.parametrize("q,past,page,pad", PLANS)
+@pytest.mark.parametrize("with_free", [True, False])
+def test_plan(q, past, page, pad, with_free):
+    B = len(q)
+    W = max(1, max(-(-(a + b) // page) for a, b in zip(q, past))) + 1
+    g = torch.Generator().manual_seed(B)
+    ids = torch.randperm(B * W + 3, generator=g).tolist()
+    table = []
+    for b in range(B):
+        n = -(-past[b] // page) if with_free else -(-(past[b] + q[b]) // page)
+        table.append([ids.pop() for _ in range(n)] + [-1] * (W - n))
+    delta = torch.randint(-900, 900, (B, 1), generator=g).tolist()
+    n_tok = sum(q) + pad
+    want_table = [list(r) for r in table]
+    want = ora.plan(q, past, want_table, page, n_tok, ids if with_free else None,
+                    [d[0] for d in delta])
+    # the table as a view into a wider one, with its other columns untouched
+    wide = torch.full((B, W + 5), -7, dtype=torch.int32, device=DEV)
+    wide[:, :W] = i32(table)
+    got = ops.ragged_plan(i32(q), i32(past), wide[:, :W], page_tokens=page, n_tokens=n_tok,
+                          free_pages=i32(ids) if with_free else None,
+                          rope_delta=torch.tensor(delta, device=DEV))
+    for name, x in zip(("cu_q", "kv_lens", "requests", "positions", "slots", "counts"), want):
+        assert getattr(got, name).tolist() == x, name
+    assert wide[:, :W].tolist() == want_table
+    assert bool((wide[:, W:] == -7).all())
+
+
+def test_plan_at_the_largest_batch_and_with_no_request():
+    B = 8192
+    q = [b % 3 for b in range(B)]
+    past = [(7 * b) % 130 for b in range(B)]
+    table = [[-1] * 4 for _ in range(B)]
+    ids = list(range(B * 4, 0, -1))
+    for b in range(B):
+        for j in range(-(-past[b] // 64)):
+            table[b][j] = ids.pop()
+    want_table = [list(r) for r in table]
+    want = ora.plan(q, past, want_table, 64, sum(q), ids)
+    t = i32(table)
+    got = ops.ragged_plan(i32(q), i32(past), t, page_tokens=64, n_tokens=sum(q), free_pages=i32(ids))
+    for name, x in zip(got._fields, want):
+        assert getattr(got, name).tolist() == x, name
+    assert t.tolist() == want_table
+    none = torch.empty(0, dtype=torch.int32, device=DEV)
+    got = ops.ragged_plan(none, none, torch.empty(0, 4, dtype=torch.int32, device=DEV),
+                          page_tokens=64, n_tokens=5)
+    assert got.cu_q.tolist() == [0] and got.slots.tolist() == [-1] * 5
+    assert got.counts.tolist() == [0, 0]
+
+
+def test_plan_records_what_does_not_fit():
+    t = i32([[4, -1], [5, -1]])
+    # the free list is one page short: request 1's new page is missing
+    p = ops.ragged_plan(i32([64, 64]), i32([64, 60]), t, page_tokens=64, n_tokens=128,
+                        free_pages=i32([9]))
+    assert ops.device_error() == 0x903
+    assert p.counts.tolist() == [128, 2] and t.tolist() == [[4, 9], [5, -1]]
+    assert p.slots.tolist() == [9 * 64 + i for i in range(64)] + \
+        [5 * 64 + i for i in range(60, 64)] + [-1] * 60
+    # a table that does not map a position; a position past the table
+    p = ops.ragged_plan(i32([2]), i32([63]), i32([[3, -1]]), page_tokens=64, n_tokens=2)
+    assert ops.device_error() == 0x903 and p.slots.tolist() == [3 * 64 + 63, -1]
+    p = ops.ragged_plan(i32([3]), i32([126]), i32([[3, 8]]), page_tokens=64, n_tokens=3)
+    assert ops.device_error() == 0x902
+    assert p.slots.tolist() == [8 * 64 + 62, 8 * 64 + 63, -1] and p.kv_lens.tolist() == [128]
+    # more tokens than the packed buffer; a negative length
+    p = ops.ragged_plan(i32([3, 3]), i32([0, 0]), i32([[3], [8]]), page_tokens=64, n_tokens=4)
+    assert ops.device_error() == 0x904
+    assert p.cu_q.tolist() == [0, 3, 4] and p.kv_lens.tolist() == [3, 1]
+    p = ops.ragged_plan(i32([-5, 2]), i32([0, 1]), i32([[3], [8]]), page_tokens=64, n_tokens=2)
+    assert ops.device_error() == 0x901
+    assert p.cu_q.tolist() == [0, 0, 2] and p.slots.tolist() == [8 * 64 + 1, 8 * 64 + 2]
+
+
+# -------------------------------------------------- norm, rotary, K/V to slots
+INV = 1.0 / (5e6 ** (torch.arange(0, 128, 2, dtype=torch.float32) / 128))
+
+
+@pytest.mark.parametrize("n,Hq,Hkv,axes,page,pad", [
+    (1, 32, 8, 1, 256, 0), (8, 4, 1, 3, 64, 0), (3, 1, 1, 1, 64, 1), (129, 5, 1, 3, 192, 19),
+    (700, 32, 8, 3, 256, 3), (1037, 6, 2, 3, 64, 0), (2, 40, 8, 3, 64, 2)])
+def test_norm_rope_slots(n, Hq, Hkv, axes, page, pad):
+    width = (Hq + 2 * Hkv) * 128
+    pages = -(-n // page) + 1
+    qkv = rnd(n, width, seed=n)
+    qw, kw = 1 + rnd(128, seed=1, std=0.2), 1 + rnd(128, seed=2, std=0.2)
+    g = torch.Generator().manual_seed(3)
+    pos = torch.randint(0, 1 << 20, (axes, n), generator=g)
+    pos[:, 0] = torch.tensor([0, 1, 2 ** 31 + 5])[:axes]       # near zero, and past 32 bits
+    pos = pos[0] if axes == 1 else pos
+    slots = torch.randperm(pages * page, generator=g)[:n]
+    if pad:
+        slots[torch.randperm(n, generator=g)[:pad]] = -1
+        qkv[slots < 0] = math.nan
+    k0 = rnd(pages, Hkv, page, 128, seed=4)
+    v0 = rnd(pages, Hkv, page, 128, seed=5)
+    # qkv as columns of a wider buffer, q into one with a guard behind each row
+    wide = torch.full((n, width + 64), math.nan, dtype=BF16, device=DEV)
+    wide[:, :width] = qkv.to(DEV)
+    guard = torch.full((n, Hq + 1, 128), 77.0, dtype=BF16, device=DEV)
+    k, v = k0.to(DEV), v0.to(DEV)
+    q = ops.qkv_norm_rope_ragged(wide[:, :width], qw.to(DEV), kw.to(DEV), pos.to(DEV),
+                                 INV.to(DEV), slots.to(DEV), k, v, Hq=Hq, Hkv=Hkv,
+                                 out=guard[:, :Hq])
+    wq, wk, wv, tq, tk = ora.norm_rope(torch.nan_to_num(qkv), qw, kw, pos, INV, Hq, Hkv)
+    live = slots >= 0
+    ora.check("q", q.cpu()[live], wq[live], tq[live])
+    assert bool((guard[:, Hq] == 77).all())
+    assert bool((q.cpu()[~live] == 77).all())                   # padding rows left as they were
+    want_k, tol_k = k0.double(), torch.zeros(k0.shape, dtype=torch.float64)
+    want_v = v0.clone()
+    s = slots[live]
+    want_k[s // page, :, s % page] = wk[live]
+    tol_k[s // page, :, s % page] = tk[live]
+    want_v[s // page, :, s % page] = wv[live].to(BF16)
+    ora.check("k", k, want_k, tol_k)
+    assert torch.equal(v.cpu(), want_v)
+
+
+def test_norm_rope_equals_the_table_kernel_within_its_roundings():
+    """Against q3_qkv_norm_rope at text positions: that kernel rounds cos, sin, n
+    and both products to bf16, four half steps on values up to |a| + |b|."""
+    n, Hq, Hkv = 40, 8, 2
+    qkv = rnd(n, (Hq + 2 * Hkv) * 128, seed=8)
+    qw, kw = 1 + rnd(128, seed=1, std=0.2), 1 + rnd(128, seed=2, std=0.2)
+    t = torch.arange(n, dtype=torch.float64)[:, None] * INV.double()
+    k = torch.zeros(1, Hkv, 64, 128, dtype=BF16, device=DEV)
+    v = torch.zeros_like(k)
+    old, _, _ = ops.qkv_norm_rope(qkv.to(DEV), qw.to(DEV), kw.to(DEV), t.cos().to(BF16).to(DEV),
+                                  t.sin().to(BF16).to(DEV), B=1, S=n, Hq=Hq, Hkv=Hkv)
+    q = ops.qkv_norm_rope_ragged(qkv.to(DEV), qw.to(DEV), kw.to(DEV),
+                                 torch.arange(n, device=DEV), INV.to(DEV),
+                                 torch.arange(n, device=DEV), k, v, Hq=Hq, Hkv=Hkv)
+    _, _, _, tq, _ = ora.norm_rope(qkv, qw, kw, torch.arange(n), INV, Hq, Hkv)
+    y = old[0].transpose(0, 1).double().cpu()
+    x = qkv.double().view(n, -1, 128)[:, :Hq]
+    m = (x / (x.pow(2).mean(-1, keepdim=True) + 1e-6).sqrt() * qw.double()).abs()
+    mag = (m[..., :64] + m[..., 64:]).repeat(1, 1, 2)
+    ora.check("q", q, y, tq + 6 * ora.BF16_HALF * mag)
+
+
+def test_norm_rope_records_a_slot_outside_the_pool():
+    n, Hq, Hkv = 3, 2, 1
+    qkv = rnd(n, 4 * 128).to(DEV)
+    w = torch.ones(128, dtype=BF16, device=DEV)
+    k = torch.zeros(2, 1, 64, 128, dtype=BF16, device=DEV)
+    v = torch.zeros_like(k)
+    out = torch.full((n, Hq, 128), 5.0, dtype=BF16, device=DEV)
+    ops.qkv_norm_rope_ragged(qkv, w, w, torch.arange(n, device=DEV), INV.to(DEV),
+                             torch.tensor([128, -2, 127], device=DEV), k, v, Hq=Hq, Hkv=Hkv, out=out)
+    assert ops.device_error() == 0x911
+    assert bool((out[:2] == 5).all()) and torch.equal(v[1, 0, 63], qkv[2, 3 * 128:])
+    assert int((v != 0).any(-1).sum()) == 1
+    q = ops.qkv_norm_rope_ragged(qkv[:0], w, w, torch.arange(0, device=DEV), INV.to(DEV),
+                                 torch.arange(0, device=DEV), k, v, Hq=Hq, Hkv=Hkv)
+    assert q.shape == (0, Hq, 128)
+
+
+# ------------------------------------------------------------ decode attention
+def decode_case(lens, Hq, Hkv, page, seed=0, stale=math.nan, std=1.5, **kw):
+    k, v, table = ora.make_pool(lens, Hkv, page, seed=seed, stale=stale, **kw)
+    q = rnd(len(lens), Hq, 128, seed=seed + 9, std=std)
+    return q, k, v, table
+
+
+@pytest.mark.parametrize("lens,Hq,Hkv,page", [
+    ([1], 4, 1, 64), ([0], 4, 1, 64), ([700], 4, 1, 64), ([64], 1, 1, 64), ([65, 63], 2, 2, 64),
+    ([329, 585, 0, 2048, 580, 1, 0, 153], 32, 8, 256),
+    ([1000, 17], 3, 1, 192), ([130, 4097, 64], 10, 2, 128), ([257, 1], 16, 2, 64),
+    ([1500, 66, 0], 16, 1, 64), ([900, 31], 24, 2, 256), ([40, 2000], 9, 1, 64),
+    ([5] * 300, 8, 2, 64), ([0] * 40 + [3000] + [0] * 40 + [1], 8, 4, 64),
+    ([30000], 4, 1, 256), ([0, 0, 0], 8, 2, 64)])
+def test_decode(lens, Hq, Hkv, page):
+    q, k, v, table = decode_case(lens, Hq, Hkv, page, seed=len(lens))
+    want, tol = ora.attention(q, k, v, table, lens, [1] * len(lens))
+    got = ops.attn_decode_ragged(q.to(DEV), k.to(DEV), v.to(DEV), i32(table), i32(lens))
+    ora.check("decode", got, want, tol)
+    again = ops.attn_decode_ragged(q.to(DEV), k.to(DEV), v.to(DEV), i32(table), i32(lens))
+    assert torch.equal(got, again)                       # the same order every time
+
+
+def test_decode_matches_the_one_length_kernel():
+    L, Hq, Hkv, page = 1152, 32, 8, 256
+    q, k, v, table = decode_case([L] * 8, Hq, Hkv, page, stale=0.0)
+    args = (q.to(DEV), k.to(DEV), v.to(DEV), i32(table))
+    _, tol = ora.attention(q, k, v, table, [L] * 8, [1] * 8)
+    old = ops.attn_decode_paged(*args, kv_len=L).double().cpu()
+    ora.check("decode", ops.attn_decode_ragged(*args, i32([L] * 8)), old, 2 * tol)
+
+
+def test_decode_strides_scale_guard_and_large_scores():
+    lens, Hq, Hkv, page = [200, 0, 999], 8, 2, 64
+    q, k, v, table = decode_case(lens, Hq, Hkv, page, seed=3, std=40.0)
+    rows = torch.full((3, Hq + 2 * Hkv, 128), math.nan, dtype=BF16, device=DEV)
+    rows[:, :Hq] = q.to(DEV)
+    out = torch.full((3, Hq + 1, 128), 9.0, dtype=BF16, device=DEV)
+    wide = torch.full((3, 40), -1, dtype=torch.int32, device=DEV)
+    wide[:, :len(table[0])] = i32(table)
+    for scale in (0.25, -0.1, 0.0):
+        want, tol = ora.attention(q, k, v, table, lens, [1] * 3, scale=scale)
+        _, pos = ora.attention(q, k, v, table, lens, [1] * 3, scale=abs(scale))
+        got = ops.attn_decode_ragged(rows[:, :Hq], k.to(DEV), v.to(DEV), wide, i32(lens),
+                                     scale=scale, out=out[:, :Hq])
+        ora.check(f"scale {scale}", got, want, torch.maximum(tol, pos))
+        assert bool((out[:, Hq] == 9).all())
+
+
+def test_decode_clamps_bad_lengths_and_entries():
+    lens, Hq, Hkv, page = [128, 100], 4, 2, 64
+    q, k, v, table = decode_case(lens, Hq, Hkv, page, stale=0.0)
+    dev = (q.to(DEV), k.to(DEV), v.to(DEV))
+    got = ops.attn_decode_ragged(*dev, i32(table), i32([129, -1]))   # two pages hold 128
+    assert ops.device_error() == 0x921
+    want, tol = ora.attention(q, k, v, table, [128, 0], [1, 1])
+    ora.check("clamped", got, want, tol)
+    bad = [list(r) for r in table]
+    bad[0][1], bad[1][0] = -1, k.shape[0]
+    got = ops.attn_decode_ragged(*dev, i32(bad), i32(lens))
+    assert ops.device_error() == 0x922
+    bad[0][1] = bad[1][0] = 0
+    want, tol = ora.attention(q, k, v, bad, lens, [1, 1])
+    ora.check("page 0", got, want, tol)
+
+
+def test_decode_in_a_graph_with_new_lengths_and_on_two_streams():
+    Hq, Hkv, page = 8, 2, 64
+    sets = [[700, 64, 0], [1, 900, 333]]
+    q, k, v, table = decode_case([960] * 3, Hq, Hkv, page, stale=0.0)
+    dq, dk, dv, dt, dl = q.to(DEV), k.to(DEV), v.to(DEV), i32(table), i32(sets[0])
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        ops.attn_decode_ragged(dq, dk, dv, dt, dl)
+    torch.cuda.current_stream().wait_stream(s)
+    graphs = []
+    for _ in range(2):                                    # two graphs over the same inputs
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            o = ops.attn_decode_ragged(dq, dk, dv, dt, dl)
+        graphs.append((g, o))
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for lens in sets:
+        dl.copy_(i32(lens))
+        torch.cuda.synchronize()
+        for _ in range(5):                                # both in flight at once
+            for (g, _), st in zip(graphs, streams):
+                with torch.cuda.stream(st):
+                    g.replay()
+        torch.cuda.synchronize()
+        want, tol = ora.attention(q, k, v, table, lens, [1] * 3)
+        for _, o in graphs:
+            ora.check("replayed", o, want, tol)
