@@ -216,6 +216,28 @@ Q3_API int q3_attn_decode_ragged(const void* q, int64_t q_stride, const void* k_
                                  int64_t num_pages, const int32_t* kv_lens, float scale,
                                  void* workspace, size_t workspace_bytes, q3_stream_t stream);
 
+/* Attention of packed prompt chunks (model_fused.py:248-262 at S > 1) on
+ * tcgen05: q, out bf16 [n_tokens, Hq, 128] with row strides (multiples of 8);
+ * request b owns rows cu_q[b] .. cu_q[b+1] - 1 (int32 [B + 1] on the device,
+ * ascending, cu_q[0] need not be 0), its query i sits at position kv_lens[b] -
+ * q_len + i and, with causal != 0, sees positions up to its own; otherwise all
+ * kv_lens[b].  A query that sees nothing gives zeros; rows outside
+ * [cu_q[0], cu_q[B]) are not written.  Hq / Hkv <= 16, scale > 0.  Rows of the
+ * pools at or past kv_lens[b] may hold anything; rows before it must be finite
+ * (a masked key of the same request still meets a zero probability).  Workspace
+ * as for q3_attn_decode_ragged.  Lengths outside the table or the packed rows
+ * are clamped (0x931); a table entry outside the pool is read as page 0
+ * (0x932); 0x933-0x93d: a bounded wait ran out. */
+Q3_API size_t q3_attn_prefill_ragged_workspace_bytes(void);
+Q3_API int q3_attn_prefill_ragged(const void* q, int64_t q_stride, const void* k_pages,
+                                  const void* v_pages, void* out, int64_t out_stride,
+                                  int64_t n_tokens, int B, int Hq, int Hkv, int head_dim,
+                                  const int32_t* block_table, int64_t table_stride,
+                                  int table_width, int page_tokens, int64_t num_pages,
+                                  const int32_t* cu_q, const int32_t* kv_lens, int causal,
+                                  float scale, void* workspace, size_t workspace_bytes,
+                                  q3_stream_t stream);
+
 /* ---- vision tower (transformers 5.5.0 Qwen3VLVisionModel, which the
  * reference runs at vision.py:51-53, :74-76) --------------------------------
  * Tokens are patches in merge-block order.  The image table `imgs` is int32

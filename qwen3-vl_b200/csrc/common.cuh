@@ -65,6 +65,12 @@ int* device_error_word();
 // `rows` in a plane read as zeros.
 int make_tmap_3d_rows128(CUtensorMap* map, const void* base, int64_t rows, int64_t planes,
                          int64_t plane_stride_elems, int box_rows);
+// 3-D bf16 map over `rows` rows of `heads` x 128 elements (row stride
+// row_stride_elems), boxes of box_rows rows x box_heads heads x 64 elements with
+// the 128-byte swizzle: shared memory gets the (row, head) pairs in row-major
+// order.  Rows at or past `rows` read as zeros.
+int make_tmap_3d_heads(CUtensorMap* map, const void* base, int64_t rows, int heads,
+                       int64_t row_stride_elems, int box_rows, int box_heads);
 // 3-D view (64 elements, rows, 64-wide column blocks) of a bf16 [rows, cols]
 // matrix, boxes of box_rows rows x 64 x `depth` column blocks, laid out in
 // shared memory as depth consecutive [box_rows][64] tiles with the 128-byte
@@ -441,6 +447,38 @@ __device__ __forceinline__ float ld_shared_cluster_f32(uint32_t addr) {
   float x;
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(addr));
   return x;
+}
+
+// --------------------------- fp32 helpers ----------------------------------
+__device__ __forceinline__ float ex2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// max of three (one instruction on sm_100)
+__device__ __forceinline__ float max3f(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// Packed fp32 pairs (one instruction per pair on sm_100).
+__device__ __forceinline__ float2 ffma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 ra, rb, rc, rd;\n\t"
+      "mov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\tmov.b64 rc, {%6, %7};\n\t"
+      "fma.rn.f32x2 rd, ra, rb, rc;\n\tmov.b64 {%0, %1}, rd;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 fadd2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 ra, rb, rd;\n\t"
+      "mov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\t"
+      "add.rn.f32x2 rd, ra, rb;\n\tmov.b64 {%0, %1}, rd;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
 }
 
 // --------------------------- warp reductions -------------------------------

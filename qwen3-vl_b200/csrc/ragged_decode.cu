@@ -90,11 +90,7 @@ __device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
 __device__ __forceinline__ uint32_t kv_at(int r, int c) {
   return (c >> 3) * kHalf + r * 128 + (((c & 7) ^ (r & 7)) << 4);
 }
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
+
 
 // Length of request b, inside what its table row can hold.
 __device__ __forceinline__ int req_len(const RaggedDecodeParams& p, int b, bool* bad) {
@@ -346,11 +342,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
           const float m_new = fmaxf(m[hh], mx);
           const float base = m_new == -INFINITY ? 0.f : m_new;
-          const float corr = ex2(m[hh] - base);
+          const float corr = ex2_approx(m[hh] - base);
           float rs = 0.f;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            x[e] = ex2(x[e] - base);
+            x[e] = ex2_approx(x[e] - base);
             rs += x[e];
           }
           l[hh] = l[hh] * corr + rs;
@@ -420,7 +416,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int i = 0; i < kConsumers; ++i) {
           const float mi = sm_ml[(i * C::kRows + row) * 2];
-          const float f = mi == -INFINITY ? 0.f : ex2(mi - M);
+          const float f = mi == -INFINITY ? 0.f : ex2_approx(mi - M);
           a = fmaf(f, sm_o[(i * C::kRows + row) * kD + d], a);
           ls = fmaf(f, sm_ml[(i * C::kRows + row) * 2 + 1], ls);
         }
@@ -481,7 +477,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) ragged_decode_join(RaggedDeco
   float l = 0.f;
 #pragma unroll 4
   for (int i = warp; i < n; i += kJoinWarps) {
-    const float f = ex2(s_f[i] - M);
+    const float f = ex2_approx(s_f[i] - M);
     const float4 x = *reinterpret_cast<const float4*>(p.ws_acc + piece(i) * kD + lane * 4);
     l = fmaf(f, p.ws_ml[piece(i) * 2 + 1], l);
     a.x = fmaf(f, x.x, a.x);

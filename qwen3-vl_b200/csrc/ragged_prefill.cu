@@ -1,0 +1,785 @@
+// Ragged serving step: causal attention of packed prompt chunks over the paged
+// K/V cache, on the 5th-generation tensor cores (tcgen05 + TMEM).
+//
+// The S > 1 eager attention of forward_layer (model_fused.py:248-262) for a
+// batch whose requests bring different numbers of tokens on different cached
+// prefixes (the reference, and attn_prefill_tc.cu, take one start position and
+// one length for the batch): query i of request b (packed row cu_q[b] + i) sits
+// at position kv_lens[b] - q_len + i and sees positions up to its own,
+//   out = softmax(q K^T * scale) V,  head h over K/V head h / G, G = Hq / Hkv;
+// a query that sees nothing gives zeros.
+//
+// An item is up to 256 query rows of one K/V head: T = 128 / G tokens times its
+// G heads in each of two 128-row tiles, so one K/V tile serves all of them and
+// any G up to 16 fills the tile (rows are (token, head) pairs, laid out by one
+// 3-D TMA box).  Warp roles and the TMEM plan are those of the persistent
+// variant in attn_prefill_tc.cu: warp 0 streams K and V tiles of 128 keys, warp
+// 1 issues S(t) = Q(t) K^T and O(t) += P(t) V alternately for the two tiles, a
+// warpgroup per tile runs the softmax, P goes back to TMEM as bf16 in place of
+// S, and O is rescaled in place only when a row's maximum has grown by 2^8.
+//
+// Bound by the tensor pipe and the softmax (4 * 128 flops per visible pair).
+// The lengths are only known on the device, so the 128-key tiles of all items,
+// plus one position per item for its fixed cost, form one list that is cut into
+// equal ranges, one per SM; a cut that falls within 1/16 of a range of an item's
+// edge moves there.  An item cut in the middle leaves fp32 pieces (O, base, sum)
+// in the workspace and a second kernel joins them in CTA order: a 512-token
+// chunk on a 32k cache fills every SM (its 64 items alone would fill 64).
+#include <math.h>
+
+#include "common.cuh"
+
+namespace q3 {
+namespace {
+
+constexpr int kD = 128;
+constexpr int kM = 128;                   // rows of a query tile
+constexpr int kN = 128;                   // keys per K/V tile
+constexpr int kThreads = 320;             // TMA, MMA, 2 x 4 softmax warps
+constexpr int kQBytes = kM * kD * 2;      // 32 KB per query tile (two 64-dim halves)
+constexpr int kKVBytes = kN * kD * 2;     // 32 KB per K or V tile
+constexpr int kHalf = kKVBytes / 2;       // one 64-dim half of 128 rows
+constexpr int kBox = kHalf / 2;           // 64 rows of it: one TMA box of a page
+constexpr int kOffK = 2 * kQBytes;
+constexpr int kOffV = kOffK + 2 * kKVBytes;
+constexpr int kOffBar = kOffV + 2 * kKVBytes;
+constexpr int kSmem = kOffBar + 256 + 1024;
+constexpr uint32_t kTmemCols = 512;       // S[0] S[1] O[0] O[1], 128 columns each
+constexpr float kLazyLog2 = 8.0f;
+constexpr int kMaxB = 65536;
+constexpr int kMaxGrid = 512;
+constexpr int kPieceRows = 2 * kM;
+
+struct RaggedPrefillParams {
+  __nv_bfloat16* out;
+  int64_t out_stride;
+  const int32_t* table;
+  int64_t table_stride;
+  const int32_t* cu_q;
+  const int32_t* kv_lens;
+  float* ws_o;    // [2 * grid][32][256] float4: dims 4i..4i+3 of a row, rows contiguous
+  float* ws_ml;   // [2 * grid][2][256]  base (log2 units) and sum
+  int4* ws_desc;  // [grid] {request or -1, K/V head, item, last CTA of the item}
+  int B, Hkv, G, T, page_tokens, num_pages, capacity, n_tokens, causal;
+  float scale_log2;
+  int* err;
+};
+
+__device__ __forceinline__ bool warp_ok(uint64_t* bar, uint32_t parity, int* err, int code) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, err, code));
+}
+
+// ---------------------------------------------------------------------------
+// The work list.  Request b has n = ceil(q_len / 2T) items per K/V head; item i
+// has tiles(i) = max(1, ceil(x / 128)) key tiles, x = the positions its last
+// query sees.  Every item takes tiles(i) + 1 places in the list.
+// ---------------------------------------------------------------------------
+struct Req {
+  int q0, q_len, L, past;  // first packed row, queries, cached positions, L - q_len
+};
+__device__ __forceinline__ Req load_req(const RaggedPrefillParams& p, int b, bool* bad) {
+  Req r;
+  const int c0 = p.cu_q[b], c1 = p.cu_q[b + 1], L = p.kv_lens[b];
+  r.q0 = min(max(c0, 0), p.n_tokens);
+  r.q_len = min(max(c1, r.q0), p.n_tokens) - r.q0;
+  r.L = min(max(L, 0), p.capacity);
+  r.past = r.L - r.q_len;
+  if (r.q0 != c0 || r.q0 + r.q_len != c1 || r.L != L) *bad = true;
+  return r;
+}
+__device__ __forceinline__ int n_items(const RaggedPrefillParams& p, const Req& r) {
+  return (r.q_len + 2 * p.T - 1) / (2 * p.T);
+}
+__device__ __forceinline__ int n_tiles(const RaggedPrefillParams& p, const Req& r, int i) {
+  const int x = p.causal ? r.past + min(r.q_len, (i + 1) * 2 * p.T) : r.L;
+  return x <= kN ? 1 : (x + kN - 1) / kN;
+}
+// sum over i in [0, n) of floor((a i + b) / m), by Euclid's division steps
+__device__ __forceinline__ int64_t floor_sum(int64_t n, int64_t m, int64_t a, int64_t b) {
+  int64_t s = 0;
+  while (n > 0) {
+    s += (n - 1) * n / 2 * (a / m) + n * (b / m);
+    a %= m;
+    b %= m;
+    const int64_t y = a * n + b;
+    if (y < m) break;
+    n = y / m;
+    b = y - n * m;
+    const int64_t t = m;
+    m = a;
+    a = t;
+  }
+  return s;
+}
+// places that items [0, i) of one K/V head take
+__device__ __forceinline__ int64_t places(const RaggedPrefillParams& p, const Req& r, int i) {
+  if (!p.causal) return (int64_t)i * (n_tiles(p, r, 0) + 1);
+  const int n = n_items(p, r), S = 2 * p.T;
+  const int full = min(i, n - 1);  // items whose last query is (k + 1) * 2T
+  int64_t s = 0;
+  if (full > 0) {
+    const int one = r.past >= kN ? 0 : min(full, (kN - r.past) / S);  // those with one tile
+    s = one + floor_sum(full - one, kN, S, (int64_t)r.past + (int64_t)(one + 1) * S + kN - 1);
+  }
+  if (i > full && n > 0) s += n_tiles(p, r, n - 1);
+  return s + i;
+}
+// A cut at place `pos` of an item of nt tiles, as a tile boundary 0..nt: place 0
+// is the item's fixed cost, and a cut within `snap` tiles of an edge moves to the
+// nearer one.
+__device__ __forceinline__ int cut_tile(int64_t pos, int nt, int snap) {
+  if (pos > nt) return nt;
+  const int t = (int)max64(pos - 1, 0);
+  if (t < snap && 2 * t < nt) return 0;
+  return nt - t < snap ? nt : t;
+}
+
+struct Piece {
+  Req r;
+  int b, kvh, item, t0, t1, nt;
+  int64_t u;  // place of the item in the list
+};
+struct Walk {
+  Req r;
+  int b, kvh, item, n, nt, snap;
+  int64_t pos, u, left;  // place inside the item, of the item, places left
+  __device__ __forceinline__ bool next(const RaggedPrefillParams& p, Piece& w) {
+    while (left > 0) {
+      const int64_t end = min64(pos + left, nt + 1);
+      w.t0 = cut_tile(pos, nt, snap);
+      w.t1 = cut_tile(end, nt, snap);
+      w.r = r;
+      w.b = b;
+      w.kvh = kvh;
+      w.item = item;
+      w.nt = nt;
+      w.u = u;
+      left -= end - pos;
+      if (end == nt + 1) {
+        u += nt + 1;
+        pos = 0;
+        if (++item == n) {
+          item = 0;
+          if (++kvh == p.Hkv) {
+            kvh = 0;
+            bool bad = false;
+            do {
+              if (++b >= p.B) {
+                left = 0;
+                break;
+              }
+              r = load_req(p, b, &bad);
+              n = n_items(p, r);
+            } while (n == 0);
+          }
+        }
+        nt = n_tiles(p, r, item);
+      } else {
+        pos = end;
+      }
+      if (w.t0 < w.t1) return true;
+    }
+    return false;
+  }
+};
+
+__global__ void __launch_bounds__(kThreads, 1)
+    ragged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ,
+                          const __grid_constant__ CUtensorMap tmK,
+                          const __grid_constant__ CUtensorMap tmV, RaggedPrefillParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~uintptr_t(1023));
+  const uint32_t s_base = smem_u32(smem);
+  uint64_t* bar = reinterpret_cast<uint64_t*>(smem + kOffBar);
+  uint64_t* q_full = bar + 0;
+  uint64_t* k_full = bar + 1;    // [2]
+  uint64_t* k_empty = bar + 3;   // [2] MMA commit after S of both tiles
+  uint64_t* v_full = bar + 5;    // [2]
+  uint64_t* v_empty = bar + 7;   // [2] MMA commit after PV of both tiles
+  uint64_t* s_full = bar + 9;    // [tile] S (and the PV before it) complete
+  uint64_t* p_full = bar + 11;   // [tile] P in TMEM: one arrival per softmax warp
+  uint64_t* o_final = bar + 13;  // [tile] the piece's last PV complete
+  uint64_t* o_empty = bar + 15;  // [tile] the piece's O read out: one arrival per warp
+  uint64_t* q_empty = bar + 17;  // the piece's S MMAs complete
+  uint64_t* v_tail = bar + 18;   // copies of a V tile that reaches past the last position
+  uint64_t* mma_done = bar + 19;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar + 20);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  __shared__ int64_t s_warp[kThreads / 32];
+  __shared__ Walk s_walk;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&k_full[i], 1);
+      mbar_init(&k_empty[i], 1);
+      mbar_init(&v_full[i], 1);
+      mbar_init(&v_empty[i], 1);
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 4);
+      mbar_init(&o_final[i], 1);
+      mbar_init(&o_empty[i], 4);
+    }
+    mbar_init(v_tail, 1);
+    mbar_init(mma_done, 1);
+    *abort_flag = 0;
+    s_walk.left = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&tmQ);
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
+  }
+  // TMEM only after the wait: a kernel before this one may still have to
+  // allocate its own on this SM
+  pdl_wait();
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, kTmemCols);
+    tmem_relinquish();
+  }
+
+  // ---- this CTA's range of the list (every CTA scans the lengths) ----
+  const int per = (p.B + kThreads - 1) / kThreads;
+  const int b0 = min((int)threadIdx.x * per, p.B), b1 = min(b0 + per, p.B);
+  int64_t mine = 0;
+  bool bad = false;
+  for (int b = b0; b < b1; ++b) {
+    const Req r = load_req(p, b, &bad);
+    mine += places(p, r, n_items(p, r));
+  }
+  mine *= p.Hkv;
+  if (bad && blockIdx.x == 0) report_timeout(p.err, 0x931);
+  int64_t incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t y = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += y;
+  }
+  if (lane == 31) s_warp[warp] = incl;
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  pdl_launch();
+  const uint32_t tmem = *tmem_slot;
+  int64_t before = incl - mine, U = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) {
+    if (w < warp) before += s_warp[w];
+    U += s_warp[w];
+  }
+  const int64_t nc = min64(gridDim.x, U);  // CTAs that get places
+  const int c = blockIdx.x;
+  const int64_t u0 = c < nc ? U * c / nc : U, u1 = c < nc ? U * (c + 1) / nc : U;
+  if (u0 < u1 && before <= u0 && u0 < before + mine) {
+    int64_t at = before;
+    for (int b = b0; b < b1; ++b) {
+      const Req r = load_req(p, b, &bad);
+      const int n = n_items(p, r);
+      const int64_t per_head = places(p, r, n), all = per_head * p.Hkv;
+      if (u0 < at + all) {
+        const int kvh = (int)((u0 - at) / per_head);
+        const int64_t rem = u0 - at - kvh * per_head;
+        int lo = 0, hi = n;  // places(lo) <= rem < places(hi)
+        while (hi - lo > 1) {
+          const int mid = (lo + hi) >> 1;
+          if (places(p, r, mid) <= rem) lo = mid;
+          else hi = mid;
+        }
+        s_walk.r = r;
+        s_walk.b = b;
+        s_walk.kvh = kvh;
+        s_walk.item = lo;
+        s_walk.n = n;
+        s_walk.nt = n_tiles(p, r, lo);
+        s_walk.snap = (int)min64(U / nc / 16, 1 << 20);
+        s_walk.pos = rem - places(p, r, lo);
+        s_walk.u = u0 - s_walk.pos;
+        s_walk.left = u1 - u0;
+        break;
+      }
+      at += all;
+    }
+  }
+  __syncthreads();
+  Walk walk = s_walk;
+  Piece w;
+
+  if (warp == 0) {
+    // ------------------------------ TMA producer ------------------------------
+    int T = 0, ic = 0, nk = 0, nv = 0, tails = 0;
+    bool ok = true;
+    if (lane == 0) p.ws_desc[c] = make_int4(-1, 0, 0, 0);
+    while (ok && !*abort_flag && walk.next(p, w)) {
+      if (w.t0 == 0 && w.t1 < w.nt) {
+        // the item goes on in the next CTAs: find the last of them
+        int last = c;
+        for (int k0 = c + 1; k0 < nc; k0 += 32) {
+          const int k = k0 + lane;
+          const int64_t pos = U * k / nc - w.u;
+          const bool in = k < nc && pos <= w.nt && cut_tile(pos, w.nt, walk.snap) < w.nt;
+          const int n = __popc(__ballot_sync(0xffffffffu, in));
+          last += n;
+          if (n < 32) break;
+        }
+        if (lane == 0) p.ws_desc[c] = make_int4(w.b, w.kvh, w.item, last);
+      }
+      if (ic >= 1 && !warp_ok(q_empty, (ic - 1) & 1, p.err, 0x93b)) { ok = false; break; }
+      if (lane == 0) {
+        const int rows = p.T * p.G;  // rows of a tile that hold a (token, head) pair
+        mbar_arrive_expect_tx(q_full, 2 * 2 * rows * 128);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const int tok = w.r.q0 + (2 * w.item + t) * p.T;
+          tma_load_3d(smem + t * kQBytes, &tmQ, q_full, 0, w.kvh * p.G, tok, kCacheEvictNormal);
+          tma_load_3d(smem + t * kQBytes + kQBytes / 2, &tmQ, q_full, 64, w.kvh * p.G, tok,
+                      kCacheEvictNormal);
+        }
+      }
+      ++ic;
+      int row = 0;  // this lane's 64-key block: its first row in the pool, or -1
+      for (int j = w.t0; j < w.t1; ++j, ++T) {
+        const int s = T & 1, k = (2 * (j - w.t0)) & 31;
+        if (k == 0) {
+          // 16 tiles' pages at once (page_tokens % 64 == 0: a block never straddles)
+          const int64_t key = ((int64_t)2 * j + lane) * 64;
+          row = -1;
+          if (key < w.r.L && (2 * j + lane) < 2 * w.t1) {
+            int pg = p.table[w.b * p.table_stride + (uint32_t)key / (uint32_t)p.page_tokens];
+            if (pg < 0 || pg >= p.num_pages) {  // recorded, page 0 read in its place
+              report_timeout(p.err, 0x932);
+              pg = 0;
+            }
+            row = (int)(((int64_t)pg * p.Hkv + w.kvh) * p.page_tokens +
+                        (uint32_t)key % (uint32_t)p.page_tokens);
+          }
+        }
+        // blocks past the last position are masked: any valid rows do
+        const int ya = max(__shfl_sync(0xffffffffu, row, k), 0);
+        const int yb0 = __shfl_sync(0xffffffffu, row, k + 1);
+        const int yb = yb0 < 0 ? ya : yb0;
+        if (T >= 2 && !warp_ok(&k_empty[s], ((T >> 1) - 1) & 1, p.err, 0x933)) { ok = false; break; }
+        if (lane == 0) {
+          uint8_t* dk = smem + kOffK + s * kKVBytes;
+          mbar_arrive_expect_tx(&k_full[s], kKVBytes);
+          tma_load_2d(dk, &tmK, &k_full[s], 0, ya, kCacheEvictNormal);
+          tma_load_2d(dk + kBox, &tmK, &k_full[s], 0, yb, kCacheEvictNormal);
+          tma_load_2d(dk + kHalf, &tmK, &k_full[s], 64, ya, kCacheEvictNormal);
+          tma_load_2d(dk + kHalf + kBox, &tmK, &k_full[s], 64, yb, kCacheEvictNormal);
+        }
+        nk = T + 1;
+        if (T >= 2 && !warp_ok(&v_empty[s], ((T >> 1) - 1) & 1, p.err, 0x934)) { ok = false; break; }
+        const int valid = w.r.L - j * kN;  // keys of the tile that exist, if below 128
+        uint64_t* vb = valid < kN ? v_tail : &v_full[s];
+        uint8_t* dv = smem + kOffV + s * kKVBytes;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(vb, kKVBytes);
+          tma_load_2d(dv, &tmV, vb, 0, ya, kCacheEvictNormal);
+          tma_load_2d(dv + kBox, &tmV, vb, 0, yb, kCacheEvictNormal);
+          tma_load_2d(dv + kHalf, &tmV, vb, 64, ya, kCacheEvictNormal);
+          tma_load_2d(dv + kHalf + kBox, &tmV, vb, 64, yb, kCacheEvictNormal);
+        }
+        if (valid < kN) {
+          // V rows past the last position hold whatever the page held before
+          // (NaN included) and 0 * V must be 0: they become zeros here, before
+          // the MMA warp is told of the tile
+          ++tails;
+          if (!warp_ok(v_tail, (tails - 1) & 1, p.err, 0x935)) { ok = false; break; }
+          const int v0 = max(valid, 0);
+          for (int i = lane; i < (kN - v0) * 16; i += 32)  // 16-byte pieces of both halves
+            *reinterpret_cast<uint4*>(dv + ((i >> 3) & 1) * kHalf + (v0 + (i >> 4)) * 128 +
+                                      (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&v_full[s]);
+        } else {
+          nv = T + 1;
+        }
+      }
+    }
+    if (!ok) {
+      *abort_flag = 1;
+      // let the copies this warp issued land before the CTA exits
+      if (lane == 0) {
+        if (ic > 0) mbar_wait(q_full, (ic - 1) & 1, nullptr, 0);
+        for (int j = max(0, nk - 2); j < nk; ++j)
+          mbar_wait(&k_full[j & 1], (j >> 1) & 1, nullptr, 0);
+        for (int j = max(0, nv - 2); j < nv; ++j)
+          mbar_wait(&v_full[j & 1], (j >> 1) & 1, nullptr, 0);
+        if (tails > 0) mbar_wait(v_tail, (tails - 1) & 1, nullptr, 0);
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------ MMA issuer --------------------------------
+    if (lane == 0) {
+      constexpr uint32_t idesc_s = umma_idesc_bf16(kM, kN);
+      constexpr uint32_t idesc_o = umma_idesc_bf16_bmn(kM, kD);
+      // unrolled, every descriptor a base plus a constant (a 128 x 128 x 16 MMA
+      // takes 64 cycles; recomputing descriptors per step issues slower)
+      auto issue_s = [&](int T, int t) {
+        const uint64_t dq = umma_desc_k_sw128(s_base + t * kQBytes);
+        const uint64_t dk = umma_desc_k_sw128(s_base + kOffK + (T & 1) * kKVBytes);
+        const uint32_t ds = tmem + t * kN;
+#pragma unroll
+        for (int ks = 0; ks < kD / 16; ++ks)
+          tc_mma_bf16(ds, dq + (uint64_t)(((ks >> 2) * (kQBytes / 2)) >> 4) + 2 * (ks & 3),
+                      dk + (uint64_t)(((ks >> 2) * kHalf) >> 4) + 2 * (ks & 3), idesc_s, ks != 0);
+        tc_commit(&s_full[t]);
+      };
+      auto issue_pv = [&](int T, int t, bool first) {
+        const uint64_t dv = umma_desc_mn_sw128(s_base + kOffV + (T & 1) * kKVBytes, kHalf, 1024u);
+        const uint32_t dO = tmem + 2 * kN + t * kD, dp = tmem + t * kN;
+        tc_mma_bf16_ts(dO, dp, dv, idesc_o, first ? 0u : 1u);
+#pragma unroll
+        for (int ks = 1; ks < kN / 16; ++ks)
+          tc_mma_bf16_ts(dO, dp + ks * 8, dv + (uint64_t)((ks * 2048) >> 4), idesc_o, 1u);
+      };
+      bool ok = true;
+      int T = 0, ic = 0;
+      while (ok && !*abort_flag && walk.next(p, w)) {
+        const int n_kb = w.t1 - w.t0;
+        if (!mbar_wait(q_full, ic & 1, p.err, 0x936) ||
+            !mbar_wait(&k_full[T & 1], (T >> 1) & 1, p.err, 0x937)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        issue_s(T, 0);
+        issue_s(T, 1);
+        tc_commit(&k_empty[T & 1]);
+        if (n_kb == 1) tc_commit(q_empty);
+        for (int j = 0; ok && j < n_kb; ++j) {
+          const int Tj = T + j;
+          if (!mbar_wait(&v_full[Tj & 1], (Tj >> 1) & 1, p.err, 0x938)) { ok = false; break; }
+          for (int t = 0; t < 2 && ok; ++t) {
+            if (!mbar_wait(&p_full[t], Tj & 1, p.err, 0x939) ||
+                (j == 0 && ic >= 1 && !mbar_wait(&o_empty[t], (ic - 1) & 1, p.err, 0x93a))) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            issue_pv(Tj, t, j == 0);
+            if (t == 1) tc_commit(&v_empty[Tj & 1]);
+            if (j + 1 < n_kb) {
+              if (t == 0 && !mbar_wait(&k_full[(Tj + 1) & 1], ((Tj + 1) >> 1) & 1, p.err, 0x937)) {
+                ok = false;
+                break;
+              }
+              tc_fence_after();
+              issue_s(Tj + 1, t);
+              if (t == 1) {
+                tc_commit(&k_empty[(Tj + 1) & 1]);
+                if (j + 2 == n_kb) tc_commit(q_empty);  // the piece's last S MMAs
+              }
+            } else {
+              tc_commit(&o_final[t]);
+            }
+          }
+        }
+        T += n_kb;
+        ++ic;
+      }
+      if (!ok) *abort_flag = 1;
+      // every MMA issued above has completed before TMEM is released
+      tc_commit(mma_done);
+      mbar_wait(mma_done, 0, nullptr, 0);
+    }
+  } else {
+    // -------------------------------- softmax ---------------------------------
+    const int t = (warp - 2) >> 2;  // query tile
+    const int quarter = warp & 3;   // TMEM lane quarter of this warp
+    const int row = quarter * 32 + lane;
+    const int tok_in = row / p.G, head_in = row - tok_in * p.G;
+    const bool row_used = row < p.T * p.G;
+    const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
+    const uint32_t s_col = tmem + lane_off + t * kN;
+    const uint32_t o_col = tmem + lane_off + 2 * kN + t * kD;
+    bool ok = true;
+    int T = 0, ic = 0;
+    while (ok && walk.next(p, w)) {
+      const int n_kb = w.t1 - w.t0;
+      const int tile_tok = (2 * w.item + t) * p.T;
+      const int tok = tile_tok + tok_in;
+      const bool live = row_used && tok < w.r.q_len;
+      // the last position this row sees, and the fewest any row of the tile sees
+      const int see = !live ? -1 : p.causal ? w.r.past + tok : w.r.L - 1;
+      const int see_min = p.causal ? min(w.r.past + tile_tok, w.r.L - 1) : w.r.L - 1;
+      float m_used = -INFINITY, l = 0.f;
+      for (int j = 0; j < n_kb; ++j) {
+        const int Tj = T + j;
+        if (__any_sync(0xffffffffu, *abort_flag != 0)) { ok = false; break; }
+        if (!warp_ok(&s_full[t], Tj & 1, p.err, 0x93c)) { ok = false; break; }
+        tc_fence_after();
+        uint32_t rr[kN];  // raw scores; scaling is folded into the exponent's FMA
+#pragma unroll
+        for (int cc = 0; cc < kN / 32; ++cc) {
+          uint32_t(&r32)[32] = *reinterpret_cast<uint32_t(*)[32]>(&rr[cc * 32]);
+          tmem_ld_32cols(s_col + cc * 32, r32);
+        }
+        tc_wait_ld();
+        const int kbase = (w.t0 + j) * kN;
+        if (kbase + kN - 1 > see_min) {
+          const int lim = see - kbase;
+#pragma unroll
+          for (int i = 0; i < kN; ++i)
+            if (i > lim) rr[i] = __float_as_uint(-INFINITY);
+        }
+        float mq[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int i = 0; i < kN; i += 8)
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            mq[q] = max3f(mq[q], __uint_as_float(rr[i + 2 * q]), __uint_as_float(rr[i + 2 * q + 1]));
+        const float mx = fmaxf(fmaxf(mq[0], mq[1]), fmaxf(mq[2], mq[3]));
+        // scale > 0, so the maximum of the scaled scores is the scaled maximum
+        const float m_new = fmaxf(m_used, mx * p.scale_log2);
+        const bool move = m_new > m_used + kLazyLog2;  // -inf + 8 = -inf
+        const bool rescale = move && j > 0 && m_used != -INFINITY;
+        const float corr = rescale ? ex2_approx(m_used - m_new) : 1.f;
+        if (move) {
+          l *= ex2_approx(m_used - m_new);  // m_used = -inf: l is 0 and stays 0
+          m_used = m_new;
+        }
+        const float nbase = m_used == -INFINITY ? 0.f : -m_used;
+        const float2 sc2 = make_float2(p.scale_log2, p.scale_log2);
+        const float2 nb2 = make_float2(nbase, nbase);
+        float2 rsq[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+        for (int cc = 0; cc < kN / 32; ++cc) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float2 x = ffma2(make_float2(__uint_as_float(rr[cc * 32 + 2 * i]),
+                                               __uint_as_float(rr[cc * 32 + 2 * i + 1])),
+                                   sc2, nb2);
+            const float2 e = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+            rsq[i & 1] = fadd2(rsq[i & 1], e);
+            pk[i] = pack_bf16x2(e.x, e.y);
+          }
+          tmem_st_16cols(s_col + cc * 16, pk);  // P: 32 keys per 16 columns
+        }
+        const float rs = (rsq[0].x + rsq[1].x) + (rsq[0].y + rsq[1].y);
+        if (__any_sync(0xffffffffu, rescale)) {
+          // O holds the piece's tiles before j, complete (covered by the commit
+          // of this S): move it to the new base before this PV adds to it
+#pragma unroll 1
+          for (int cc = 0; cc < kD / 32; ++cc) {
+            uint32_t r32[32];
+            tmem_ld_32cols(o_col + cc * 32, r32);
+            tc_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) r32[i] = __float_as_uint(__uint_as_float(r32[i]) * corr);
+            tmem_st_32cols(o_col + cc * 32, r32);
+          }
+        }
+        tc_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[t]);
+        l += rs;
+      }
+      if (!ok) break;
+      if (!warp_ok(&o_final[t], ic & 1, p.err, 0x93d)) { ok = false; break; }
+      tc_fence_after();
+      if (w.t0 == 0 && w.t1 == w.nt) {
+        const float inv = l > 0.f ? 1.f / l : 0.f;
+        __nv_bfloat16* dst = p.out + (int64_t)(w.r.q0 + tok) * p.out_stride +
+                             (int64_t)(w.kvh * p.G + head_in) * kD;
+#pragma unroll
+        for (int cc = 0; cc < kD / 32; ++cc) {
+          uint32_t r32[32];
+          tmem_ld_32cols(o_col + cc * 32, r32);
+          tc_wait_ld();
+          if (live) {
+#pragma unroll
+            for (int d = 0; d < 32; d += 8) {
+              uint4 u;
+              u.x = pack_bf16x2(__uint_as_float(r32[d]) * inv, __uint_as_float(r32[d + 1]) * inv);
+              u.y = pack_bf16x2(__uint_as_float(r32[d + 2]) * inv,
+                                __uint_as_float(r32[d + 3]) * inv);
+              u.z = pack_bf16x2(__uint_as_float(r32[d + 4]) * inv,
+                                __uint_as_float(r32[d + 5]) * inv);
+              u.w = pack_bf16x2(__uint_as_float(r32[d + 6]) * inv,
+                                __uint_as_float(r32[d + 7]) * inv);
+              *reinterpret_cast<uint4*>(dst + cc * 32 + d) = u;
+            }
+          }
+        }
+      } else {
+        // a piece of an item: O relative to m_used, the base and the sum.  A
+        // piece that began inside its item has the even slot.
+        const int64_t slot = 2 * c + (w.t0 == 0 ? 1 : 0);
+        const int r256 = t * kM + row;
+        p.ws_ml[(slot * 2) * kPieceRows + r256] = m_used;
+        p.ws_ml[(slot * 2 + 1) * kPieceRows + r256] = l;
+        float4* dst = reinterpret_cast<float4*>(p.ws_o) + slot * 32 * kPieceRows + r256;
+#pragma unroll
+        for (int cc = 0; cc < kD / 32; ++cc) {
+          uint32_t r32[32];
+          tmem_ld_32cols(o_col + cc * 32, r32);
+          tc_wait_ld();
+#pragma unroll
+          for (int d = 0; d < 8; ++d)
+            dst[(cc * 8 + d) * kPieceRows] =
+                make_float4(__uint_as_float(r32[4 * d]), __uint_as_float(r32[4 * d + 1]),
+                            __uint_as_float(r32[4 * d + 2]), __uint_as_float(r32[4 * d + 3]));
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&o_empty[t]);
+      T += n_kb;
+      ++ic;
+    }
+    if (!ok) *abort_flag = 1;
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+// Joins the pieces of the item that CTA c left unfinished: slots 2c+1, 2(c+1),
+// ..., 2*last, in that order.  One thread per row of the item and 16 dims.
+constexpr int kJoinD4 = 4;  // float4 columns per CTA
+__global__ void __launch_bounds__(kPieceRows) ragged_prefill_join(RaggedPrefillParams p) {
+  pdl_launch();
+  pdl_wait();
+  const int c = blockIdx.x, d40 = blockIdx.y * kJoinD4, r256 = threadIdx.x;
+  const int4 d = p.ws_desc[c];
+  if (d.x < 0) return;
+  const int t = r256 / kM, row = r256 - t * kM;
+  const int tok_in = row / p.G, head_in = row - tok_in * p.G;
+  const int tok = (2 * d.z + t) * p.T + tok_in;
+  bool bad = false;
+  const Req r = load_req(p, d.x, &bad);
+  if (row >= p.T * p.G || tok >= r.q_len) return;
+  const int n = d.w - c + 1;
+  auto slot = [&](int i) { return (int64_t)(i == 0 ? 2 * c + 1 : 2 * (c + i)); };
+  float M = -INFINITY;
+#pragma unroll 4
+  for (int i = 0; i < n; ++i) M = fmaxf(M, p.ws_ml[slot(i) * 2 * kPieceRows + r256]);
+  float4 a[kJoinD4];
+#pragma unroll
+  for (int k = 0; k < kJoinD4; ++k) a[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+  float l = 0.f;
+#pragma unroll 2
+  for (int i = 0; i < n; ++i) {
+    const float mi = p.ws_ml[slot(i) * 2 * kPieceRows + r256];
+    const float f = mi == -INFINITY ? 0.f : ex2_approx(mi - M);
+    l = fmaf(f, p.ws_ml[(slot(i) * 2 + 1) * kPieceRows + r256], l);
+    const float4* src = reinterpret_cast<const float4*>(p.ws_o) + slot(i) * 32 * kPieceRows + r256;
+#pragma unroll
+    for (int k = 0; k < kJoinD4; ++k) {
+      const float4 x = src[(d40 + k) * kPieceRows];
+      a[k].x = fmaf(f, x.x, a[k].x);
+      a[k].y = fmaf(f, x.y, a[k].y);
+      a[k].z = fmaf(f, x.z, a[k].z);
+      a[k].w = fmaf(f, x.w, a[k].w);
+    }
+  }
+  const float inv = l > 0.f ? 1.f / l : 0.f;
+  __nv_bfloat16* dst = p.out + (int64_t)(r.q0 + tok) * p.out_stride +
+                       (int64_t)(d.y * p.G + head_in) * kD + d40 * 4;
+#pragma unroll
+  for (int k = 0; k < kJoinD4; k += 2) {
+    uint4 u;
+    u.x = pack_bf16x2(a[k].x * inv, a[k].y * inv);
+    u.y = pack_bf16x2(a[k].z * inv, a[k].w * inv);
+    u.z = pack_bf16x2(a[k + 1].x * inv, a[k + 1].y * inv);
+    u.w = pack_bf16x2(a[k + 1].z * inv, a[k + 1].w * inv);
+    *reinterpret_cast<uint4*>(dst + k * 4) = u;
+  }
+}
+
+int prefill_grid() { return (int)min64(num_sms(), kMaxGrid); }
+
+size_t prefill_ws(size_t* off_ml, size_t* off_desc) {
+  const size_t slots = 2 * (size_t)prefill_grid();
+  size_t n = slots * kPieceRows * kD * 4;
+  *off_ml = n;
+  n += slots * kPieceRows * 8;
+  *off_desc = n;
+  return n + prefill_grid() * sizeof(int4);
+}
+
+}  // namespace
+}  // namespace q3
+
+extern "C" size_t q3_attn_prefill_ragged_workspace_bytes(void) {
+  size_t a, b;
+  return q3::prefill_ws(&a, &b);
+}
+
+extern "C" int q3_attn_prefill_ragged(const void* q, int64_t q_stride, const void* k_pages,
+                                      const void* v_pages, void* out, int64_t out_stride,
+                                      int64_t n_tokens, int B, int Hq, int Hkv, int head_dim,
+                                      const int32_t* block_table, int64_t table_stride,
+                                      int table_width, int page_tokens, int64_t num_pages,
+                                      const int32_t* cu_q, const int32_t* kv_lens, int causal,
+                                      float scale, void* workspace, size_t workspace_bytes,
+                                      q3_stream_t stream) {
+  using namespace q3;
+  Q3_REQUIRE(head_dim == kD, "q3_attn_prefill_ragged: head_dim must be 128 (got %d)", head_dim);
+  Q3_REQUIRE(n_tokens >= 0 && n_tokens < (1ll << 31) - 256 && B >= 0 && B <= kMaxB && Hq > 0 &&
+                 Hkv > 0 && Hkv <= 1024 && Hq % Hkv == 0,
+             "q3_attn_prefill_ragged: bad shape n=%lld B=%d Hq=%d Hkv=%d", (long long)n_tokens, B,
+             Hq, Hkv);
+  if (Hq / Hkv > 16)
+    return fail(Q3_ERR_UNSUPPORTED, "q3_attn_prefill_ragged: Hq/Hkv=%d above 16", Hq / Hkv);
+  if (B == 0 || n_tokens == 0) return Q3_OK;
+  Q3_REQUIRE(q && k_pages && v_pages && out && block_table && cu_q && kv_lens && workspace,
+             "q3_attn_prefill_ragged: null pointer");
+  Q3_REQUIRE(page_tokens > 0 && page_tokens % 64 == 0,
+             "q3_attn_prefill_ragged: page_tokens=%d must be a positive multiple of 64",
+             page_tokens);
+  Q3_REQUIRE(table_width > 0 && table_stride >= table_width && num_pages > 0 &&
+                 (int64_t)table_width * page_tokens < (1ll << 31) - 256,
+             "q3_attn_prefill_ragged: table width %d, stride %lld, %lld pages", table_width,
+             (long long)table_stride, (long long)num_pages);
+  Q3_REQUIRE(num_pages * Hkv * page_tokens < (1ll << 31),
+             "q3_attn_prefill_ragged: the pool is too large for 32-bit TMA rows");
+  Q3_REQUIRE(q_stride >= (int64_t)Hq * kD && out_stride >= (int64_t)Hq * kD &&
+                 q_stride % 8 == 0 && out_stride % 8 == 0,
+             "q3_attn_prefill_ragged: row strides must cover a row and be multiples of 8");
+  Q3_REQUIRE(scale > 0.f && scale < INFINITY, "q3_attn_prefill_ragged: scale must be positive");
+  Q3_REQUIRE(aligned(q, 16) && aligned(k_pages, 16) && aligned(v_pages, 16) && aligned(out, 16) &&
+                 aligned(block_table, 4) && aligned(cu_q, 4) && aligned(kv_lens, 4) &&
+                 aligned(workspace, 16),
+             "q3_attn_prefill_ragged: misaligned pointer");
+  size_t off_ml, off_desc;
+  const size_t need = prefill_ws(&off_ml, &off_desc);
+  Q3_REQUIRE(workspace_bytes >= need, "q3_attn_prefill_ragged: workspace of %zu bytes, need %zu",
+             workspace_bytes, need);
+  const int G = Hq / Hkv, T = kM / G;
+  CUtensorMap tq, tk, tv;
+  int rc = make_tmap_3d_heads(&tq, q, n_tokens, Hq, q_stride, T, G);
+  if (rc) return rc;
+  const int64_t rows = num_pages * Hkv * page_tokens;
+  rc = make_tmap_2d(&tk, k_pages, rows, kD, 64, 64);
+  if (rc) return rc;
+  rc = make_tmap_2d(&tv, v_pages, rows, kD, 64, 64);
+  if (rc) return rc;
+  static bool attr_set[64] = {false};
+  int dev = 0;
+  Q3_CUDA_CHECK(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64 || !attr_set[dev]) {
+    Q3_CUDA_CHECK(cudaFuncSetAttribute(ragged_prefill_kernel,
+                                       cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+    if (dev >= 0 && dev < 64) attr_set[dev] = true;
+  }
+  uint8_t* ws = (uint8_t*)workspace;
+  RaggedPrefillParams p{(__nv_bfloat16*)out, out_stride, block_table, table_stride, cu_q, kv_lens,
+                        (float*)ws, (float*)(ws + off_ml), (int4*)(ws + off_desc), B, Hkv, G, T,
+                        page_tokens, (int)num_pages, table_width * page_tokens, (int)n_tokens,
+                        causal ? 1 : 0, scale * 1.4426950408889634f, device_error_word()};
+  const dim3 grid((unsigned)prefill_grid());
+  rc = launch_ex(ragged_prefill_kernel, grid, dim3(kThreads), kSmem, (cudaStream_t)stream, 1, tq,
+                 tk, tv, p);
+  if (rc) return rc;
+  return launch_ex(ragged_prefill_join, dim3(grid.x, kD / 4 / kJoinD4), dim3(kPieceRows), 0,
+                   (cudaStream_t)stream, 1, p);
+}

@@ -65,6 +65,25 @@ int make_tmap_3d_rows128(CUtensorMap* map, const void* base, int64_t rows, int64
   return Q3_OK;
 }
 
+int make_tmap_3d_heads(CUtensorMap* map, const void* base, int64_t rows, int heads,
+                       int64_t row_stride_elems, int box_rows, int box_heads) {
+  EncodeTiledFn enc = get_encode_fn();
+  if (!enc) return fail(Q3_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  if (rows < 1 || heads < 1 || box_rows < 1 || box_rows > 256 || box_heads < 1 || box_heads > 256)
+    return fail(Q3_ERR_INVALID, "3-D head tensor map: bad rows/heads/box");
+  if (!aligned(base, 16) || (row_stride_elems * 2) % 16 != 0)
+    return fail(Q3_ERR_INVALID, "3-D head tensor map: base/row stride must be 16-byte aligned");
+  cuuint64_t dims[3] = {128, (cuuint64_t)heads, (cuuint64_t)rows};
+  cuuint64_t strides[2] = {256, (cuuint64_t)row_stride_elems * 2};
+  cuuint32_t box[3] = {64, (cuuint32_t)box_heads, (cuuint32_t)box_rows};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims,
+                   strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(Q3_ERR_CUDA, "cuTensorMapEncodeTiled (heads) failed (%d)", (int)r);
+  return Q3_OK;
+}
+
 int make_tmap_wblocks(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int box_rows,
                       int depth) {
   EncodeTiledFn enc = get_encode_fn();

@@ -1196,6 +1196,44 @@ def attn_decode_ragged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Te
     return out
 
 
+def attn_prefill_ragged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                        block_table: torch.Tensor, cu_q: torch.Tensor, kv_lens: torch.Tensor,
+                        scale: float = None, causal: bool = True,
+                        out: torch.Tensor = None) -> torch.Tensor:
+    """Attention of packed prompt chunks over the page pool, on tcgen05.
+
+    q bf16 [n, Hq, 128] (any row stride); cu_q int32 [B + 1]: request b owns rows
+    cu_q[b] .. cu_q[b+1] - 1 of q, and its last one sits at position
+    kv_lens[b] - 1; with causal each query sees positions up to its own.  Rows of
+    out outside [cu_q[0], cu_q[B]) are not written, so a part of a batch goes
+    through slices of cu_q, kv_lens and block_table.  A query that sees nothing
+    gives zeros.  Hq / Hkv is any whole number up to 16; scale is positive."""
+    name = "attn_prefill_ragged"
+    dev = _ragged_device(name, q, k_pages, v_pages, block_table, cu_q, kv_lens, out)
+    _ragged_ints(name, torch.int32, cu_q=cu_q, kv_lens=kv_lens)
+    num_pages, Hkv, page_tokens = _ragged_pool(name, k_pages, v_pages)
+    if q.dim() != 3:
+        raise ValueError(f"{name}: q must be [n, Hq, 128]")
+    q_stride = _ragged_rows(name, "q", q)
+    n, Hq, D = q.shape
+    B = kv_lens.numel()
+    if cu_q.numel() != B + 1:
+        raise ValueError(f"{name}: cu_q must have {B + 1} entries for {B} requests")
+    table_stride = _ragged_table(name, block_table, B)
+    if out is None:
+        out = torch.empty(n, Hq, D, dtype=torch.bfloat16, device=dev)
+    elif out.shape != q.shape:
+        raise ValueError(f"{name}: out must match q")
+    nbytes = _lib.raw("q3_attn_prefill_ragged_workspace_bytes")()
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    _ragged_call("q3_attn_prefill_ragged", dev, q.data_ptr(), q_stride, k_pages.data_ptr(),
+                 v_pages.data_ptr(), out.data_ptr(), _ragged_rows(name, "out", out), n, B, Hq, Hkv,
+                 D, block_table.data_ptr(), table_stride, block_table.shape[1], page_tokens,
+                 num_pages, cu_q.data_ptr(), kv_lens.data_ptr(), 1 if causal else 0,
+                 1.0 / math.sqrt(D) if scale is None else float(scale), ws.data_ptr(), nbytes)
+    return out
+
+
 def device_error(clear: bool = True) -> int:
     """Error code recorded by a kernel whose bounded wait timed out (0 = none)."""
     return int(_lib.raw("q3_device_error")(1 if clear else 0))

@@ -295,3 +295,121 @@ def test_decode_in_a_graph_with_new_lengths_and_on_two_streams():
         want, tol = ora.attention(q, k, v, table, lens, [1] * 3)
         for _, o in graphs:
             ora.check("replayed", o, want, tol)
+
+
+# ----------------------------------------------------------- prefill attention
+def prefill_case(q_lens, pasts, Hq, Hkv, page, seed=0, stale=math.nan, std=1.5):
+    lens = [max(0, a + b) for a, b in zip(q_lens, pasts)]
+    k, v, table = ora.make_pool(lens, Hkv, page, seed=seed, stale=stale)
+    q = rnd(sum(q_lens), Hq, 128, seed=seed + 9, std=std)
+    cu = [0]
+    for x in q_lens:
+        cu.append(cu[-1] + x)
+    return q, k, v, table, cu, lens
+
+
+@pytest.mark.parametrize("q_lens,pasts,Hq,Hkv,page", [
+    ([1], [0], 4, 1, 64), ([128], [0], 1, 1, 64), ([5, 0, 70], [0, 64, 63], 4, 1, 64),
+    ([26, 46, 28, 100], [0] * 4, 4, 1, 64), ([257], [0], 2, 2, 192), ([300, 1], [5, 900], 3, 1, 64),
+    ([130], [1000], 32, 8, 256), ([64, 65], [64, 4032], 10, 2, 128), ([33], [3000], 16, 1, 64),
+    ([70, 2], [1, 0], 12, 1, 64), ([515], [0], 14, 2, 64), ([1] * 70, list(range(70)), 8, 4, 64),
+    ([700], [0], 8, 1, 64), ([9, 40], [-4, -40], 4, 2, 64)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_prefill(q_lens, pasts, Hq, Hkv, page, causal):
+    q, k, v, table, cu, lens = prefill_case(q_lens, pasts, Hq, Hkv, page, seed=len(q_lens))
+    want, tol = ora.attention(q, k, v, table, lens, q_lens, causal=causal)
+    args = (q.to(DEV), k.to(DEV), v.to(DEV), i32(table), i32(cu), i32(lens))
+    got = ops.attn_prefill_ragged(*args, causal=causal)
+    ora.check("prefill", got, want, tol)
+    assert torch.equal(got, ops.attn_prefill_ragged(*args, causal=causal))
+
+
+def test_prefill_matches_the_one_start_kernel():
+    B, S, Hq, Hkv, page, start = 2, 300, 8, 2, 128, 128
+    q, k, v, table, cu, lens = prefill_case([S] * B, [start] * B, Hq, Hkv, page, stale=0.0)
+    _, tol = ora.attention(q, k, v, table, lens, [S] * B)
+    dk, dv, dt = k.to(DEV), v.to(DEV), i32(table)
+    qd = q.to(DEV)
+    old = torch.empty(B, Hq, S, 128, dtype=BF16, device=DEV)
+    ops.attn_prefill_tc_paged(qd.view(B, S, Hq, 128).transpose(1, 2).contiguous(), dk, dv, dt,
+                              start_pos=start, causal=True, scale=1 / math.sqrt(128), out=old)
+    got = ops.attn_prefill_ragged(qd, dk, dv, dt, i32(cu), i32(lens))
+    ora.check("prefill", got, old.transpose(1, 2).reshape(B * S, Hq, 128).double().cpu(), 2 * tol)
+
+
+def test_prefill_of_a_part_of_a_batch_leaves_other_rows():
+    q_lens, pasts, Hq, Hkv, page = [1, 70, 133, 2], [600, 0, 50, 7], 8, 2, 64
+    q, k, v, table, cu, lens = prefill_case(q_lens, pasts, Hq, Hkv, page, seed=4)
+    rows = torch.full((q.shape[0] + 5, Hq + 2 * Hkv, 128), math.nan, dtype=BF16, device=DEV)
+    rows[:q.shape[0], :Hq] = q.to(DEV)
+    out = torch.full((q.shape[0] + 5, Hq + 1, 128), 9.0, dtype=BF16, device=DEV)
+    want, tol = ora.attention(q, k, v, table, lens, q_lens)
+    dc, dl, dt = i32(cu), i32(lens), i32(table)
+    got = ops.attn_prefill_ragged(rows[:, :Hq], k.to(DEV), v.to(DEV), dt[1:3], dc[1:4], dl[1:3],
+                                  out=out[:, :Hq])
+    a, b = cu[1], cu[3]
+    ora.check("part", got[a:b], want[a:b], tol[a:b])
+    assert bool((out[:a] == 9).all()) and bool((out[b:] == 9).all())
+    assert bool((out[:, Hq] == 9).all())
+
+
+def test_prefill_of_rising_scores_rescales():
+    """Keys whose scores grow along the cache move a row's base at every tile."""
+    q, k, v, table, cu, lens = prefill_case([40], [1500], 4, 1, 64, stale=0.0)
+    ramp = torch.linspace(0.0, 6.0, lens[0])
+    for i, pg in enumerate(table[0]):
+        n = min(64, lens[0] - i * 64)
+        if n > 0:
+            k[pg, 0, :n] = (ramp[i * 64:i * 64 + n, None] * torch.ones(128)).to(BF16)
+    q = q.abs()
+    want, tol = ora.attention(q, k, v, table, lens, [40], scale=1.0)
+    got = ops.attn_prefill_ragged(q.to(DEV), k.to(DEV), v.to(DEV), i32(table), i32(cu), i32(lens),
+                                  scale=1.0)
+    ora.check("rising", got, want, tol)
+
+
+def test_prefill_clamps_bad_lengths_and_entries():
+    q, k, v, table, cu, lens = prefill_case([70, 30], [0, 60], 4, 2, 64, stale=0.0)
+    dev = (q.to(DEV), k.to(DEV), v.to(DEV))
+    # request 1's rows end past the packed buffer, and its length past its table
+    got = ops.attn_prefill_ragged(*dev, i32(table), i32([0, 70, 130]), i32([70, 129]))
+    assert ops.device_error() == 0x931
+    want, tol = ora.attention(q, k, v, [table[0], table[1]], [70, 128], [70, 30])
+    ora.check("clamped", got, want, tol)
+    got = ops.attn_prefill_ragged(*dev, i32(table), i32([0, 70, 60]), i32([70, -1]))
+    assert ops.device_error() == 0x931
+    ora.check("none", got[:70], want[:70], tol[:70])
+    bad = [list(r) for r in table]
+    bad[0][1], bad[1][0] = -1, k.shape[0]
+    got = ops.attn_prefill_ragged(*dev, i32(bad), i32(cu), i32(lens))
+    assert ops.device_error() == 0x932
+    bad[0][1] = bad[1][0] = 0
+    want, tol = ora.attention(q, k, v, bad, lens, [70, 30])
+    ora.check("page 0", got, want, tol)
+
+
+def test_prefill_in_a_graph_with_new_lengths():
+    Hq, Hkv, page, n = 8, 2, 64, 200
+    sets = [([120, 80], [0, 500]), ([1, 150], [700, 3]), ([0, 0], [4, 0])]
+    q, k, v, table, _, _ = prefill_case([100, 100], [800, 800], Hq, Hkv, page, stale=0.0)
+    dq, dk, dv, dt = q.to(DEV), k.to(DEV), v.to(DEV), i32(table)
+    dc, dl = i32([0, 0, 0]), i32([0, 0])
+    out = torch.zeros_like(dq)
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        ops.attn_prefill_ragged(dq, dk, dv, dt, dc, dl, out=out)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        ops.attn_prefill_ragged(dq, dk, dv, dt, dc, dl, out=out)
+    for qs, ps in sets:
+        lens = [a + b for a, b in zip(qs, ps)]
+        dc.copy_(i32([0, qs[0], qs[0] + qs[1]]))
+        dl.copy_(i32(lens))
+        out.fill_(3.0)
+        g.replay()
+        torch.cuda.synchronize()
+        m = sum(qs)
+        want, tol = ora.attention(q[:m], k, v, table, lens, qs)
+        ora.check("replayed", out[:m], want, tol)
+        assert bool((out[m:] == 3).all())

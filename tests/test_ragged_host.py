@@ -113,3 +113,203 @@ def test_plan_form_hands_out_pages_as_the_allocator_does():
     ora.plan(q, past, table, page, sum(q), free)
     assert table == want
     pool.close()
+
+
+# ------------------------------------------------ the kernels' work division
+def decode_ranges(lens, Hkv, grid):
+    """attn_decode_ragged's division: [(cta, pair, first tile, end tile, tiles)]."""
+    tiles = [-(-x // 64) for x in lens]
+    units = [(b * Hkv + h, t, n) for b, n in enumerate(tiles) for h in range(Hkv) for t in range(n)]
+    U = len(units)
+    nc = min(grid, U)
+    out, desc = [], {}
+    for c in range(nc):
+        u = u0 = U * c // nc
+        u1 = U * (c + 1) // nc
+        while u < u1:
+            pair, t0, n = units[u]
+            t1 = min(n, t0 + u1 - u)
+            out.append((c, pair, t0, t1, n))
+            if t0 == 0 and t1 < n:
+                desc[c] = (pair, ((u + n) * nc - 1) // U)
+            u += t1 - t0
+        assert u == u1 and u0 <= u1
+    return out, desc
+
+
+def join_check(pieces, desc):
+    """Each pair or item is either one whole piece or the pieces that its
+    descriptor's slots name, in order, without a gap."""
+    split = {}
+    for c, key, t0, t1, n in pieces:
+        assert 0 <= t0 < t1 <= n
+        if (t0, t1) != (0, n):
+            slot = 2 * c + (1 if t0 == 0 else 0)
+            split.setdefault(key, []).append((slot, t0, t1, n))
+    slots = [s for v in split.values() for s, *_ in v]
+    assert len(slots) == len(set(slots))
+    named = {}
+    for c, (key, last) in desc.items():
+        named[key] = [2 * c + 1] + [2 * k for k in range(c + 1, last + 1)]
+    assert set(named) == set(split)
+    for key, parts in split.items():
+        assert [s for s, *_ in parts] == named[key]
+        assert parts[0][1] == 0 and parts[-1][2] == parts[-1][3]
+        assert all(a[2] == b[1] for a, b in zip(parts, parts[1:]))
+
+
+LENGTHS = [[1], [0], [700], [0, 0, 64, 65, 0], [329, 585, 758, 2048, 580, 1405, 0, 153],
+           [5] * 300, [30000, 1, 1, 1], [0] * 40 + [3000]]
+
+
+@pytest.mark.parametrize("lens", LENGTHS)
+@pytest.mark.parametrize("Hkv", [1, 3, 8])
+@pytest.mark.parametrize("grid", [1, 5, 148])
+def test_decode_division_covers_every_tile_once(lens, Hkv, grid):
+    pieces, desc = decode_ranges(lens, Hkv, grid)
+    seen = sorted((k, t) for _, k, t0, t1, _ in pieces for t in range(t0, t1))
+    assert seen == sorted((b * Hkv + h, t) for b, x in enumerate(lens) for h in range(Hkv)
+                          for t in range(-(-x // 64)))
+    join_check(pieces, desc)
+    per = [sum(p[3] - p[2] for p in pieces if p[0] == c) for c in range(min(grid, len(seen)))]
+    assert not per or max(per) - min(per) <= 1
+
+
+def floor_sum(n, m, a, b):
+    s = 0
+    while n > 0:
+        s += (n - 1) * n // 2 * (a // m) + n * (b // m)
+        a, b = a % m, b % m
+        y = a * n + b
+        if y < m:
+            break
+        n, b, m, a = y // m, y % m, a, m
+    return s
+
+
+def n_tiles(T, q, L, i, causal=True):
+    x = L - q + min(q, (i + 1) * 2 * T) if causal else L
+    return 1 if x <= 128 else -(-x // 128)
+
+
+def places(T, q, L, i, causal=True):
+    """Places of items [0, i), as the kernel sums them in closed form."""
+    if not causal:
+        return i * (n_tiles(T, q, L, 0, False) + 1)
+    n, S, past = -(-q // (2 * T)), 2 * T, L - q
+    full, s = min(i, n - 1), 0
+    if full > 0:
+        one = 0 if past >= 128 else min(full, (128 - past) // S)
+        s = one + floor_sum(full - one, 128, S, past + (one + 1) * S + 127)
+    if i > full and n > 0:
+        s += n_tiles(T, q, L, n - 1)
+    return s + i
+
+
+def test_places_in_closed_form():
+    import random
+    r = random.Random(2)
+    for _ in range(400):
+        T = r.choice([128, 64, 42, 32, 25, 21, 18, 16, 10, 8])
+        q, past = r.randint(0, 900), r.choice([0, 1, 63, 64, 127, 128, 129, 5000, -3, -400])
+        L = max(0, q + past)
+        n = -(-q // (2 * T))
+        for i in range(n + 1):
+            assert places(T, q, L, i) == sum(n_tiles(T, q, L, k) + 1 for k in range(i))
+
+
+def cut_tile(pos, nt, snap):
+    if pos > nt:
+        return nt
+    t = max(pos - 1, 0)
+    if t < snap and 2 * t < nt:
+        return 0
+    return nt if nt - t < snap else t
+
+
+def prefill_ranges(qs, Ls, T, Hkv, grid, causal=True):
+    """attn_prefill_ragged's division, walked as the kernel's roles walk it."""
+    items, u = [], 0
+    for b, (q, L) in enumerate(zip(qs, Ls)):
+        for h in range(Hkv):
+            for i in range(-(-q // (2 * T))):
+                nt = n_tiles(T, q, L, i, causal)
+                items.append(((b, h, i), nt, u))
+                u += nt + 1
+    U, nc = u, min(grid, u)
+    snap = U // nc // 16 if nc else 0
+    pieces, desc, at = [], {}, 0
+    for c in range(nc):
+        u0, u1 = U * c // nc, U * (c + 1) // nc
+        while items[at][2] + items[at][1] + 1 <= u0:
+            at += 1
+        k = at
+        while k < len(items) and items[k][2] < u1:
+            key, nt, base = items[k]
+            t0 = cut_tile(max(u0 - base, 0), nt, snap)
+            t1 = cut_tile(min(u1 - base, nt + 1), nt, snap)
+            if t0 < t1:
+                pieces.append((c, key, t0, t1, nt))
+                if t0 == 0 and t1 < nt:
+                    last, x = c, c + 1
+                    while x < nc:                # 32 candidates at a time, as the warp does
+                        n = 0
+                        for lane in range(32):
+                            y = x + lane
+                            pos = U * y // nc - base
+                            n += y < nc and pos <= nt and cut_tile(pos, nt, snap) < nt
+                        last += n
+                        if n < 32:
+                            break
+                        x += 32
+                    desc[c] = (key, last)
+            k += 1
+    return pieces, desc, items
+
+
+def test_prefill_division_covers_every_tile_once():
+    import random
+    r = random.Random(5)
+    cases = [([512], [32768], 32, 8), ([1], [1], 32, 1), ([0, 3, 0], [9, 3, 0], 128, 2),
+             ([4096, 1, 77], [4096, 1, 5000], 32, 8), ([16], [300000], 8, 1), ([5], [2], 25, 1),
+             ([1] * 200, list(range(1, 201)), 32, 2)]
+    for _ in range(60):
+        B = r.randint(1, 9)
+        qs = [r.choice([0, 1, 5, 64, 65, 300, 1111]) for _ in range(B)]
+        cases.append((qs, [q + r.choice([0, 0, 1, 500, 9000]) for q in qs],
+                      r.choice([128, 64, 42, 32, 18, 8]), r.choice([1, 2, 8])))
+    for qs, Ls, T, Hkv in cases:
+        for grid in (1, 7, 148):
+            for causal in (True, False):
+                pieces, desc, items = prefill_ranges(qs, Ls, T, Hkv, grid, causal)
+                seen = [(k, t) for _, k, t0, t1, _ in pieces for t in range(t0, t1)]
+                assert len(seen) == len(set(seen))
+                assert sorted(seen) == sorted((k, t) for k, nt, _ in items for t in range(nt))
+                join_check(pieces, desc)
+
+
+def prefill_args(**kw):
+    a = dict(q=ONE, qs=1024, k=ONE, v=ONE, out=ONE, os=1024, n=100, B=4, Hq=8, Hkv=2, d=128,
+             table=ONE, stride=8, width=8, page=64, pages=10, cu=ONE, lens=ONE, causal=1, scale=0.1,
+             ws=ONE, nb=1 << 30, s=None)
+    a.update(kw)
+    return list(a.values())
+
+
+@pytest.mark.parametrize("kw,text", [
+    (dict(d=64), b"head_dim"), (dict(B=-1), b"bad shape"), (dict(Hq=7), b"bad shape"),
+    (dict(n=-1), b"bad shape"), (dict(q=None), b"null"), (dict(cu=None), b"null"),
+    (dict(page=32), b"page_tokens"), (dict(width=0), b"table width"), (dict(stride=4), b"stride"),
+    (dict(pages=0), b"pages"), (dict(pages=1 << 25), b"too large"), (dict(qs=1000), b"strides"),
+    (dict(os=1028), b"strides"), (dict(q=ODD), b"misaligned"), (dict(scale=0.0), b"positive"),
+    (dict(scale=-1.0), b"positive"), (dict(scale=float("nan")), b"positive"),
+    (dict(scale=float("inf")), b"positive"), (dict(nb=100), b"workspace of 100")])
+def test_prefill_refusals(kw, text):
+    refused("q3_attn_prefill_ragged", prefill_args(**kw), text)
+
+
+def test_prefill_refuses_more_than_16_heads_a_group_and_accepts_empty_calls():
+    refused("q3_attn_prefill_ragged", prefill_args(Hq=34, qs=1 << 20, os=1 << 20), b"above 16",
+            _lib.Q3_ERR_UNSUPPORTED)
+    assert _lib.raw("q3_attn_prefill_ragged")(*prefill_args(B=0, q=None)) == 0
+    assert _lib.raw("q3_attn_prefill_ragged")(*prefill_args(n=0, q=None)) == 0
