@@ -35,7 +35,12 @@ namespace {
 constexpr int kD = 128;
 constexpr int kM = 128;                   // rows of a query tile
 constexpr int kN = 128;                   // keys per K/V tile
-constexpr int kThreads = 320;             // TMA, MMA, 2 x 4 softmax warps
+constexpr int kThreads = 384;             // TMA, MMA, 2 idle, 2 x 4 softmax warps
+// registers per thread: the launch has 168 (65536 / 384 in whole 8s), the first
+// warpgroup gives some up and the softmax warpgroups take them; 88 + 2 * 208 =
+// 3 * 168
+constexpr int kRegsIo = 88;
+constexpr int kRegsSoftmax = 208;
 constexpr int kQBytes = kM * kD * 2;      // 32 KB per query tile (two 64-dim halves)
 constexpr int kKVBytes = kN * kD * 2;     // 32 KB per K or V tile
 constexpr int kHalf = kKVBytes / 2;       // one 64-dim half of 128 rows
@@ -45,7 +50,9 @@ constexpr int kOffV = kOffK + 2 * kKVBytes;
 constexpr int kOffBar = kOffV + 2 * kKVBytes;
 constexpr int kSmem = kOffBar + 256 + 1024;
 constexpr uint32_t kTmemCols = 512;       // S[0] S[1] O[0] O[1], 128 columns each
-constexpr float kLazyLog2 = 8.0f;
+// a row's base moves when its maximum has grown by more than 2^64: P, l and O are
+// relative to the base, and bf16 and fp32 hold 2^64 times any finite V
+constexpr float kLazyLog2 = 64.0f;
 constexpr int kMaxB = 65536;
 constexpr int kMaxGrid = 512;
 constexpr int kPieceRows = 2 * kM;
@@ -67,6 +74,99 @@ struct RaggedPrefillParams {
 
 __device__ __forceinline__ bool warp_ok(uint64_t* bar, uint32_t parity, int* err, int code) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, err, code));
+}
+
+// 2^x of a pair on the FMA pipe: the MUFU pipe's 16 exponentials a cycle take as
+// long as a tile's MMAs, so every fourth pair goes here.  x = j + f with j =
+// round(x) (the 1.5 * 2^23 shifter) and f in [-0.5, 0.5]; 2^f by the degree-4
+// polynomial of smallest maximum relative error (2.6e-6, fitted by reweighted
+// least squares), 2^j added to the exponent field.  P is rounded to bf16 (2^-8)
+// after it.  x is clamped to -126, where the result is below 2^-125 and
+// vanishes against the row's sum (masked keys: x = -inf).
+constexpr float kP0 = 0.9999992847442627f, kP1 = 0.6931217908859253f, kP2 = 0.240247443318367f,
+                kP3 = 0.05591785907745361f, kP4 = 0.009570102207362652f;
+__device__ __forceinline__ float2 exp2_fma(float2 x) {
+  constexpr float kShift = 12582912.0f;
+  x.x = fmaxf(x.x, -126.f);
+  x.y = fmaxf(x.y, -126.f);
+  const float2 t = fadd2(x, make_float2(kShift, kShift));
+  const float2 j = fadd2(t, make_float2(-kShift, -kShift));
+  const float2 f = ffma2(j, make_float2(-1.f, -1.f), x);
+  float2 q = ffma2(f, make_float2(kP4, kP4), make_float2(kP3, kP3));
+  q = ffma2(q, f, make_float2(kP2, kP2));
+  q = ffma2(q, f, make_float2(kP1, kP1));
+  q = ffma2(q, f, make_float2(kP0, kP0));
+  return make_float2(__int_as_float(__float_as_int(q.x) + (__float_as_int(t.x) << 23)),
+                     __int_as_float(__float_as_int(q.y) + (__float_as_int(t.y) << 23)));
+}
+
+// The exponentials of keys 64 * HALF .. + 63 of a row against base m: their bf16
+// pairs and the sums of the unrounded values.
+template <int HALF>
+__device__ __forceinline__ void half_exps(const uint32_t (&rr)[kN], float scale_log2, float m,
+                                          float2 (&sum)[2], uint32_t (&pk)[32]) {
+  const float nbase = m == -INFINITY ? 0.f : -m;
+  const float2 sc2 = make_float2(scale_log2, scale_log2);
+  const float2 nb2 = make_float2(nbase, nbase);
+#pragma unroll
+  for (int i = 0; i < 32; ++i) {
+    const float2 x = ffma2(make_float2(__uint_as_float(rr[HALF * 64 + 2 * i]),
+                                       __uint_as_float(rr[HALF * 64 + 2 * i + 1])),
+                           sc2, nb2);
+    const float2 e = (i & 3) == 3 ? exp2_fma(x) : make_float2(ex2_approx(x.x), ex2_approx(x.y));
+    sum[i & 1] = fadd2(sum[i & 1], e);
+    pk[i] = pack_bf16x2(e.x, e.y);
+  }
+}
+
+// tc_mma_bf16, tc_mma_bf16_ts and tc_commit for one lane of a converged warp
+// (`leader` != 0 in that lane), with descriptors as (low, high) words: the high
+// word is the same for every operand here (stride 1024 bytes, version 1, 128-byte
+// swizzle), the low word is the address and the leading offset.
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t is;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(is));
+  return is;
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t hi,
+                                       uint32_t idesc, uint32_t accumulate, uint32_t leader) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 da, db;\n\t"
+      "mov.b64 da, {%1, %3};\n\tmov.b64 db, {%2, %3};\n\t"
+      "setp.ne.b32 p, %5, 0;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, p;\n\t}" ::"r"(d),
+      "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate), "r"(leader)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a_tmem, uint32_t b_lo, uint32_t hi,
+                                       uint32_t idesc, uint32_t accumulate, uint32_t leader) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 db;\n\t"
+      "mov.b64 db, {%2, %3};\n\t"
+      "setp.ne.b32 p, %5, 0;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p;\n\t}" ::"r"(d),
+      "r"(a_tmem), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate), "r"(leader)
+      : "memory");
+}
+__device__ __forceinline__ void commit_if(uint64_t* bar, uint32_t leader) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(
+          smem_u32(bar)),
+      "r"(leader)
+      : "memory");
+}
+
+template <int N>
+__device__ __forceinline__ void regs_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void regs_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
 }
 
 // ---------------------------------------------------------------------------
@@ -198,13 +298,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* v_full = bar + 5;    // [2]
   uint64_t* v_empty = bar + 7;   // [2] MMA commit after PV of both tiles
   uint64_t* s_full = bar + 9;    // [tile] S (and the PV before it) complete
-  uint64_t* p_full = bar + 11;   // [tile] P in TMEM: one arrival per softmax warp
-  uint64_t* o_final = bar + 13;  // [tile] the piece's last PV complete
-  uint64_t* o_empty = bar + 15;  // [tile] the piece's O read out: one arrival per warp
-  uint64_t* q_empty = bar + 17;  // the piece's S MMAs complete
-  uint64_t* v_tail = bar + 18;   // copies of a V tile that reaches past the last position
-  uint64_t* mma_done = bar + 19;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar + 20);
+  uint64_t* p_full = bar + 11;   // [tile][half] P of 64 keys in TMEM: one arrival per warp
+  uint64_t* o_final = bar + 15;  // [tile] the piece's last PV complete
+  uint64_t* o_empty = bar + 17;  // [tile] the piece's O read out: one arrival per warp
+  uint64_t* q_empty = bar + 19;  // the piece's S MMAs complete
+  uint64_t* v_tail = bar + 20;   // copies of a V tile that reaches past the last position
+  uint64_t* mma_done = bar + 21;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar + 23);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   __shared__ int64_t s_warp[kThreads / 32];
   __shared__ Walk s_walk;
@@ -219,7 +319,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&v_full[i], 1);
       mbar_init(&v_empty[i], 1);
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 4);
+      mbar_init(&p_full[2 * i], 4);
+      mbar_init(&p_full[2 * i + 1], 4);
       mbar_init(&o_final[i], 1);
       mbar_init(&o_empty[i], 4);
     }
@@ -303,191 +404,208 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   }
   __syncthreads();
-  Walk walk = s_walk;
   Piece w;
 
-  if (warp == 0) {
-    // ------------------------------ TMA producer ------------------------------
-    int T = 0, ic = 0, nk = 0, nv = 0, tails = 0;
-    bool ok = true;
-    if (lane == 0) p.ws_desc[c] = make_int4(-1, 0, 0, 0);
-    while (ok && !*abort_flag && walk.next(p, w)) {
-      if (w.t0 == 0 && w.t1 < w.nt) {
-        // the item goes on in the next CTAs: find the last of them
-        int last = c;
-        for (int k0 = c + 1; k0 < nc; k0 += 32) {
-          const int k = k0 + lane;
-          const int64_t pos = U * k / nc - w.u;
-          const bool in = k < nc && pos <= w.nt && cut_tile(pos, w.nt, walk.snap) < w.nt;
-          const int n = __popc(__ballot_sync(0xffffffffu, in));
-          last += n;
-          if (n < 32) break;
+  if (warp < 4) {
+    regs_dec<kRegsIo>();
+    if (warp == 0) {
+      Walk walk = s_walk;
+      // ------------------------------ TMA producer ------------------------------
+      int T = 0, ic = 0, nk = 0, nv = 0, tails = 0;
+      bool ok = true;
+      if (lane == 0) p.ws_desc[c] = make_int4(-1, 0, 0, 0);
+      while (ok && !*abort_flag && walk.next(p, w)) {
+        if (w.t0 == 0 && w.t1 < w.nt) {
+          // the item goes on in the next CTAs: find the last of them
+          int last = c;
+          for (int k0 = c + 1; k0 < nc; k0 += 32) {
+            const int k = k0 + lane;
+            const int64_t pos = U * k / nc - w.u;
+            const bool in = k < nc && pos <= w.nt && cut_tile(pos, w.nt, walk.snap) < w.nt;
+            const int n = __popc(__ballot_sync(0xffffffffu, in));
+            last += n;
+            if (n < 32) break;
+          }
+          if (lane == 0) p.ws_desc[c] = make_int4(w.b, w.kvh, w.item, last);
         }
-        if (lane == 0) p.ws_desc[c] = make_int4(w.b, w.kvh, w.item, last);
-      }
-      if (ic >= 1 && !warp_ok(q_empty, (ic - 1) & 1, p.err, 0x93b)) { ok = false; break; }
-      if (lane == 0) {
-        const int rows = p.T * p.G;  // rows of a tile that hold a (token, head) pair
-        mbar_arrive_expect_tx(q_full, 2 * 2 * rows * 128);
+        if (ic >= 1 && !warp_ok(q_empty, (ic - 1) & 1, p.err, 0x93b)) { ok = false; break; }
+        if (lane == 0) {
+          const int rows = p.T * p.G;  // rows of a tile that hold a (token, head) pair
+          mbar_arrive_expect_tx(q_full, 2 * 2 * rows * 128);
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const int tok = w.r.q0 + (2 * w.item + t) * p.T;
-          tma_load_3d(smem + t * kQBytes, &tmQ, q_full, 0, w.kvh * p.G, tok, kCacheEvictNormal);
-          tma_load_3d(smem + t * kQBytes + kQBytes / 2, &tmQ, q_full, 64, w.kvh * p.G, tok,
-                      kCacheEvictNormal);
-        }
-      }
-      ++ic;
-      int row = 0;  // this lane's 64-key block: its first row in the pool, or -1
-      for (int j = w.t0; j < w.t1; ++j, ++T) {
-        const int s = T & 1, k = (2 * (j - w.t0)) & 31;
-        if (k == 0) {
-          // 16 tiles' pages at once (page_tokens % 64 == 0: a block never straddles)
-          const int64_t key = ((int64_t)2 * j + lane) * 64;
-          row = -1;
-          if (key < w.r.L && (2 * j + lane) < 2 * w.t1) {
-            int pg = p.table[w.b * p.table_stride + (uint32_t)key / (uint32_t)p.page_tokens];
-            if (pg < 0 || pg >= p.num_pages) {  // recorded, page 0 read in its place
-              report_timeout(p.err, 0x932);
-              pg = 0;
-            }
-            row = (int)(((int64_t)pg * p.Hkv + w.kvh) * p.page_tokens +
-                        (uint32_t)key % (uint32_t)p.page_tokens);
+          for (int t = 0; t < 2; ++t) {
+            const int tok = w.r.q0 + (2 * w.item + t) * p.T;
+            tma_load_3d(smem + t * kQBytes, &tmQ, q_full, 0, w.kvh * p.G, tok, kCacheEvictNormal);
+            tma_load_3d(smem + t * kQBytes + kQBytes / 2, &tmQ, q_full, 64, w.kvh * p.G, tok,
+                        kCacheEvictNormal);
           }
         }
-        // blocks past the last position are masked: any valid rows do
-        const int ya = max(__shfl_sync(0xffffffffu, row, k), 0);
-        const int yb0 = __shfl_sync(0xffffffffu, row, k + 1);
-        const int yb = yb0 < 0 ? ya : yb0;
-        if (T >= 2 && !warp_ok(&k_empty[s], ((T >> 1) - 1) & 1, p.err, 0x933)) { ok = false; break; }
-        if (lane == 0) {
-          uint8_t* dk = smem + kOffK + s * kKVBytes;
-          mbar_arrive_expect_tx(&k_full[s], kKVBytes);
-          tma_load_2d(dk, &tmK, &k_full[s], 0, ya, kCacheEvictNormal);
-          tma_load_2d(dk + kBox, &tmK, &k_full[s], 0, yb, kCacheEvictNormal);
-          tma_load_2d(dk + kHalf, &tmK, &k_full[s], 64, ya, kCacheEvictNormal);
-          tma_load_2d(dk + kHalf + kBox, &tmK, &k_full[s], 64, yb, kCacheEvictNormal);
-        }
-        nk = T + 1;
-        if (T >= 2 && !warp_ok(&v_empty[s], ((T >> 1) - 1) & 1, p.err, 0x934)) { ok = false; break; }
-        const int valid = w.r.L - j * kN;  // keys of the tile that exist, if below 128
-        uint64_t* vb = valid < kN ? v_tail : &v_full[s];
-        uint8_t* dv = smem + kOffV + s * kKVBytes;
-        if (lane == 0) {
-          mbar_arrive_expect_tx(vb, kKVBytes);
-          tma_load_2d(dv, &tmV, vb, 0, ya, kCacheEvictNormal);
-          tma_load_2d(dv + kBox, &tmV, vb, 0, yb, kCacheEvictNormal);
-          tma_load_2d(dv + kHalf, &tmV, vb, 64, ya, kCacheEvictNormal);
-          tma_load_2d(dv + kHalf + kBox, &tmV, vb, 64, yb, kCacheEvictNormal);
-        }
-        if (valid < kN) {
-          // V rows past the last position hold whatever the page held before
-          // (NaN included) and 0 * V must be 0: they become zeros here, before
-          // the MMA warp is told of the tile
-          ++tails;
-          if (!warp_ok(v_tail, (tails - 1) & 1, p.err, 0x935)) { ok = false; break; }
-          const int v0 = max(valid, 0);
-          for (int i = lane; i < (kN - v0) * 16; i += 32)  // 16-byte pieces of both halves
-            *reinterpret_cast<uint4*>(dv + ((i >> 3) & 1) * kHalf + (v0 + (i >> 4)) * 128 +
-                                      (i & 7) * 16) = make_uint4(0, 0, 0, 0);
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&v_full[s]);
-        } else {
-          nv = T + 1;
+        ++ic;
+        int row = 0;  // this lane's 64-key block: its first row in the pool, or -1
+        for (int j = w.t0; j < w.t1; ++j, ++T) {
+          const int s = T & 1, k = (2 * (j - w.t0)) & 31;
+          if (k == 0) {
+            // 16 tiles' pages at once (page_tokens % 64 == 0: a block never straddles)
+            const int64_t key = ((int64_t)2 * j + lane) * 64;
+            row = -1;
+            if (key < w.r.L && (2 * j + lane) < 2 * w.t1) {
+              int pg = p.table[w.b * p.table_stride + (uint32_t)key / (uint32_t)p.page_tokens];
+              if (pg < 0 || pg >= p.num_pages) {  // recorded, page 0 read in its place
+                report_timeout(p.err, 0x932);
+                pg = 0;
+              }
+              row = (int)(((int64_t)pg * p.Hkv + w.kvh) * p.page_tokens +
+                          (uint32_t)key % (uint32_t)p.page_tokens);
+            }
+          }
+          // blocks past the last position are masked: any valid rows do
+          const int ya = max(__shfl_sync(0xffffffffu, row, k), 0);
+          const int yb0 = __shfl_sync(0xffffffffu, row, k + 1);
+          const int yb = yb0 < 0 ? ya : yb0;
+          if (T >= 2 && !warp_ok(&k_empty[s], ((T >> 1) - 1) & 1, p.err, 0x933)) { ok = false; break; }
+          if (lane == 0) {
+            uint8_t* dk = smem + kOffK + s * kKVBytes;
+            mbar_arrive_expect_tx(&k_full[s], kKVBytes);
+            tma_load_2d(dk, &tmK, &k_full[s], 0, ya, kCacheEvictNormal);
+            tma_load_2d(dk + kBox, &tmK, &k_full[s], 0, yb, kCacheEvictNormal);
+            tma_load_2d(dk + kHalf, &tmK, &k_full[s], 64, ya, kCacheEvictNormal);
+            tma_load_2d(dk + kHalf + kBox, &tmK, &k_full[s], 64, yb, kCacheEvictNormal);
+          }
+          nk = T + 1;
+          if (T >= 2 && !warp_ok(&v_empty[s], ((T >> 1) - 1) & 1, p.err, 0x934)) { ok = false; break; }
+          const int valid = w.r.L - j * kN;  // keys of the tile that exist, if below 128
+          uint64_t* vb = valid < kN ? v_tail : &v_full[s];
+          uint8_t* dv = smem + kOffV + s * kKVBytes;
+          if (lane == 0) {
+            mbar_arrive_expect_tx(vb, kKVBytes);
+            tma_load_2d(dv, &tmV, vb, 0, ya, kCacheEvictNormal);
+            tma_load_2d(dv + kBox, &tmV, vb, 0, yb, kCacheEvictNormal);
+            tma_load_2d(dv + kHalf, &tmV, vb, 64, ya, kCacheEvictNormal);
+            tma_load_2d(dv + kHalf + kBox, &tmV, vb, 64, yb, kCacheEvictNormal);
+          }
+          if (valid < kN) {
+            // V rows past the last position hold whatever the page held before
+            // (NaN included) and 0 * V must be 0: they become zeros here, before
+            // the MMA warp is told of the tile
+            ++tails;
+            if (!warp_ok(v_tail, (tails - 1) & 1, p.err, 0x935)) { ok = false; break; }
+            const int v0 = max(valid, 0);
+            for (int i = lane; i < (kN - v0) * 16; i += 32)  // 16-byte pieces of both halves
+              *reinterpret_cast<uint4*>(dv + ((i >> 3) & 1) * kHalf + (v0 + (i >> 4)) * 128 +
+                                        (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&v_full[s]);
+          } else {
+            nv = T + 1;
+          }
         }
       }
-    }
-    if (!ok) {
-      *abort_flag = 1;
-      // let the copies this warp issued land before the CTA exits
-      if (lane == 0) {
-        if (ic > 0) mbar_wait(q_full, (ic - 1) & 1, nullptr, 0);
-        for (int j = max(0, nk - 2); j < nk; ++j)
-          mbar_wait(&k_full[j & 1], (j >> 1) & 1, nullptr, 0);
-        for (int j = max(0, nv - 2); j < nv; ++j)
-          mbar_wait(&v_full[j & 1], (j >> 1) & 1, nullptr, 0);
-        if (tails > 0) mbar_wait(v_tail, (tails - 1) & 1, nullptr, 0);
+      if (!ok) {
+        *abort_flag = 1;
+        // let the copies this warp issued land before the CTA exits
+        if (lane == 0) {
+          if (ic > 0) mbar_wait(q_full, (ic - 1) & 1, nullptr, 0);
+          for (int j = max(0, nk - 2); j < nk; ++j)
+            mbar_wait(&k_full[j & 1], (j >> 1) & 1, nullptr, 0);
+          for (int j = max(0, nv - 2); j < nv; ++j)
+            mbar_wait(&v_full[j & 1], (j >> 1) & 1, nullptr, 0);
+          if (tails > 0) mbar_wait(v_tail, (tails - 1) & 1, nullptr, 0);
+        }
       }
-    }
-  } else if (warp == 1) {
-    // ------------------------------ MMA issuer --------------------------------
-    if (lane == 0) {
+    } else if (warp == 1) {
+      // ------------------------------ MMA issuer --------------------------------
+      // One thread for both tiles, in turn: S(t) of the next keys goes out behind
+      // P V(t), so the tiles stay half a period apart and one tile's softmax runs
+      // under the other's MMAs.  (A thread per tile let them fall into step, both
+      // in softmax and then both waiting for the tensor pipe: 5500 cycles per
+      // K/V tile.)
+      // The whole warp runs the loop and every MMA is predicated on one elected
+      // lane: control flow and descriptors stay warp-uniform, so the descriptor
+      // words live in uniform registers (a lane-0 branch issued an MMA every 96
+      // cycles; one takes 64).
+      Walk walk = s_walk;
       constexpr uint32_t idesc_s = umma_idesc_bf16(kM, kN);
       constexpr uint32_t idesc_o = umma_idesc_bf16_bmn(kM, kD);
-      // unrolled, every descriptor a base plus a constant (a 128 x 128 x 16 MMA
-      // takes 64 cycles; recomputing descriptors per step issues slower)
-      auto issue_s = [&](int T, int t) {
-        const uint64_t dq = umma_desc_k_sw128(s_base + t * kQBytes);
-        const uint64_t dk = umma_desc_k_sw128(s_base + kOffK + (T & 1) * kKVBytes);
-        const uint32_t ds = tmem + t * kN;
+      const uint32_t leader = elect_one();
+      const uint32_t base = __shfl_sync(0xffffffffu, s_base, 0);
+      const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+      const uint32_t lo_q = (uint32_t)umma_desc_k_sw128(base);
+      const uint32_t lo_k = (uint32_t)umma_desc_k_sw128(base + kOffK);
+      const uint32_t lo_v = (uint32_t)umma_desc_mn_sw128(base + kOffV, kHalf, 1024u);
+      auto issue_s = [&](uint32_t stage, int t) {
+        const uint32_t dq = lo_q + t * (kQBytes >> 4), dk = lo_k + stage * (kKVBytes >> 4);
+        const uint32_t tS = tm + t * kN;
 #pragma unroll
         for (int ks = 0; ks < kD / 16; ++ks)
-          tc_mma_bf16(ds, dq + (uint64_t)(((ks >> 2) * (kQBytes / 2)) >> 4) + 2 * (ks & 3),
-                      dk + (uint64_t)(((ks >> 2) * kHalf) >> 4) + 2 * (ks & 3), idesc_s, ks != 0);
-        tc_commit(&s_full[t]);
+          mma_ss(tS, dq + ((ks >> 2) * (kQBytes / 2) >> 4) + 2 * (ks & 3),
+                 dk + ((ks >> 2) * kHalf >> 4) + 2 * (ks & 3), kDescHi, idesc_s, ks != 0, leader);
+        commit_if(&s_full[t], leader);
       };
-      auto issue_pv = [&](int T, int t, bool first) {
-        const uint64_t dv = umma_desc_mn_sw128(s_base + kOffV + (T & 1) * kKVBytes, kHalf, 1024u);
-        const uint32_t dO = tmem + 2 * kN + t * kD, dp = tmem + t * kN;
-        tc_mma_bf16_ts(dO, dp, dv, idesc_o, first ? 0u : 1u);
+      // keys 64 * half .. + 63 of a tile
+      auto issue_pv = [&](uint32_t stage, int t, int half, uint32_t accumulate) {
+        const uint32_t dv = lo_v + stage * (kKVBytes >> 4) + half * (4 * 2048 >> 4);
+        const uint32_t dp = tm + t * kN + half * 32, tO = tm + 2 * kN + t * kD;
+        mma_ts(tO, dp, dv, kDescHi, idesc_o, accumulate, leader);
 #pragma unroll
-        for (int ks = 1; ks < kN / 16; ++ks)
-          tc_mma_bf16_ts(dO, dp + ks * 8, dv + (uint64_t)((ks * 2048) >> 4), idesc_o, 1u);
+        for (int ks = 1; ks < 4; ++ks)
+          mma_ts(tO, dp + ks * 8, dv + (ks * 2048 >> 4), kDescHi, idesc_o, 1u, leader);
       };
       bool ok = true;
-      int T = 0, ic = 0;
-      while (ok && !*abort_flag && walk.next(p, w)) {
-        const int n_kb = w.t1 - w.t0;
-        if (!mbar_wait(q_full, ic & 1, p.err, 0x936) ||
-            !mbar_wait(&k_full[T & 1], (T >> 1) & 1, p.err, 0x937)) {
-          ok = false;
-          break;
-        }
+      uint32_t T = 0, ic = 0;
+      while (ok && walk.next(p, w)) {
+        const int n_kb = __shfl_sync(0xffffffffu, w.t1 - w.t0, 0);
+        ok = !__any_sync(0xffffffffu, *abort_flag != 0) &&
+             warp_ok(q_full, ic & 1, p.err, 0x936) &&
+             warp_ok(&k_full[T & 1], (T >> 1) & 1, p.err, 0x937);
+        if (!ok) break;
         tc_fence_after();
-        issue_s(T, 0);
-        issue_s(T, 1);
-        tc_commit(&k_empty[T & 1]);
-        if (n_kb == 1) tc_commit(q_empty);
-        for (int j = 0; ok && j < n_kb; ++j) {
-          const int Tj = T + j;
-          if (!mbar_wait(&v_full[Tj & 1], (Tj >> 1) & 1, p.err, 0x938)) { ok = false; break; }
-          for (int t = 0; t < 2 && ok; ++t) {
-            if (!mbar_wait(&p_full[t], Tj & 1, p.err, 0x939) ||
-                (j == 0 && ic >= 1 && !mbar_wait(&o_empty[t], (ic - 1) & 1, p.err, 0x93a))) {
-              ok = false;
-              break;
-            }
+        issue_s(T & 1, 0);
+        issue_s(T & 1, 1);
+        commit_if(&k_empty[T & 1], leader);
+        if (n_kb == 1) commit_if(q_empty, leader);
+        for (int j = 0; ok && j < n_kb; ++j, ++T) {
+          ok = warp_ok(&v_full[T & 1], (T >> 1) & 1, p.err, 0x938);
+          if (!ok) break;
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            ok = ok &&
+                 (j > 0 || ic == 0 || warp_ok(&o_empty[t], (ic - 1) & 1, p.err, 0x93a)) &&
+                 warp_ok(&p_full[2 * t], T & 1, p.err, 0x939);
+            if (!ok) break;
             tc_fence_after();
-            issue_pv(Tj, t, j == 0);
-            if (t == 1) tc_commit(&v_empty[Tj & 1]);
+            issue_pv(T & 1, t, 0, j > 0 ? 1u : 0u);
+            ok = warp_ok(&p_full[2 * t + 1], T & 1, p.err, 0x939);
+            if (!ok) break;
+            tc_fence_after();
+            issue_pv(T & 1, t, 1, 1u);
+            if (t == 1) commit_if(&v_empty[T & 1], leader);
             if (j + 1 < n_kb) {
-              if (t == 0 && !mbar_wait(&k_full[(Tj + 1) & 1], ((Tj + 1) >> 1) & 1, p.err, 0x937)) {
-                ok = false;
-                break;
-              }
+              if (t == 0) ok = warp_ok(&k_full[(T + 1) & 1], ((T + 1) >> 1) & 1, p.err, 0x937);
+              if (!ok) break;
               tc_fence_after();
-              issue_s(Tj + 1, t);
+              issue_s((T + 1) & 1, t);
               if (t == 1) {
-                tc_commit(&k_empty[(Tj + 1) & 1]);
-                if (j + 2 == n_kb) tc_commit(q_empty);  // the piece's last S MMAs
+                commit_if(&k_empty[(T + 1) & 1], leader);
+                if (j + 2 == n_kb) commit_if(q_empty, leader);  // the piece's last S MMAs
               }
             } else {
-              tc_commit(&o_final[t]);
+              commit_if(&o_final[t], leader);
             }
           }
         }
-        T += n_kb;
         ++ic;
       }
       if (!ok) *abort_flag = 1;
       // every MMA issued above has completed before TMEM is released
-      tc_commit(mma_done);
-      mbar_wait(mma_done, 0, nullptr, 0);
+      commit_if(mma_done, leader);
+      warp_ok(mma_done, 0, nullptr, 0);
     }
   } else {
     // -------------------------------- softmax ---------------------------------
-    const int t = (warp - 2) >> 2;  // query tile
+    regs_inc<kRegsSoftmax>();
+    Walk walk = s_walk;
+    const int t = (warp >> 2) - 1;  // query tile
     const int quarter = warp & 3;   // TMEM lane quarter of this warp
     const int row = quarter * 32 + lane;
     const int tok_in = row / p.G, head_in = row - tok_in * p.G;
@@ -496,7 +614,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t s_col = tmem + lane_off + t * kN;
     const uint32_t o_col = tmem + lane_off + 2 * kN + t * kD;
     bool ok = true;
-    int T = 0, ic = 0;
+    uint32_t T = 0, ic = 0;
     while (ok && walk.next(p, w)) {
       const int n_kb = w.t1 - w.t0;
       const int tile_tok = (2 * w.item + t) * p.T;
@@ -506,17 +624,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int see = !live ? -1 : p.causal ? w.r.past + tok : w.r.L - 1;
       const int see_min = p.causal ? min(w.r.past + tile_tok, w.r.L - 1) : w.r.L - 1;
       float m_used = -INFINITY, l = 0.f;
-      for (int j = 0; j < n_kb; ++j) {
-        const int Tj = T + j;
-        if (__any_sync(0xffffffffu, *abort_flag != 0)) { ok = false; break; }
-        if (!warp_ok(&s_full[t], Tj & 1, p.err, 0x93c)) { ok = false; break; }
+      for (int j = 0; j < n_kb; ++j, ++T) {
+        ok = !__any_sync(0xffffffffu, *abort_flag != 0) && warp_ok(&s_full[t], T & 1, p.err, 0x93c);
+        if (!ok) break;
         tc_fence_after();
         uint32_t rr[kN];  // raw scores; scaling is folded into the exponent's FMA
 #pragma unroll
-        for (int cc = 0; cc < kN / 32; ++cc) {
-          uint32_t(&r32)[32] = *reinterpret_cast<uint32_t(*)[32]>(&rr[cc * 32]);
-          tmem_ld_32cols(s_col + cc * 32, r32);
-        }
+        for (int cc = 0; cc < kN / 32; ++cc)
+          tmem_ld_32cols(s_col + cc * 32, *reinterpret_cast<uint32_t(*)[32]>(&rr[cc * 32]));
         tc_wait_ld();
         const int kbase = (w.t0 + j) * kN;
         if (kbase + kN - 1 > see_min) {
@@ -525,6 +640,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int i = 0; i < kN; ++i)
             if (i > lim) rr[i] = __float_as_uint(-INFINITY);
         }
+        // P = 2^(S scale - base).  The first 64 keys' exponentials are taken
+        // against the old base while the tile's maximum is still being found, and
+        // taken again in a tile that moves the base (an item's first, and after
+        // that one where the maximum has grown by 2^64).
+        float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        uint32_t pk[32];
+        half_exps<0>(rr, p.scale_log2, m_used, sum, pk);
         float mq[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (int i = 0; i < kN; i += 8)
@@ -534,53 +656,46 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float mx = fmaxf(fmaxf(mq[0], mq[1]), fmaxf(mq[2], mq[3]));
         // scale > 0, so the maximum of the scaled scores is the scaled maximum
         const float m_new = fmaxf(m_used, mx * p.scale_log2);
-        const bool move = m_new > m_used + kLazyLog2;  // -inf + 8 = -inf
-        const bool rescale = move && j > 0 && m_used != -INFINITY;
-        const float corr = rescale ? ex2_approx(m_used - m_new) : 1.f;
-        if (move) {
-          l *= ex2_approx(m_used - m_new);  // m_used = -inf: l is 0 and stays 0
-          m_used = m_new;
-        }
-        const float nbase = m_used == -INFINITY ? 0.f : -m_used;
-        const float2 sc2 = make_float2(p.scale_log2, p.scale_log2);
-        const float2 nb2 = make_float2(nbase, nbase);
-        float2 rsq[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll
-        for (int cc = 0; cc < kN / 32; ++cc) {
-          uint32_t pk[16];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float2 x = ffma2(make_float2(__uint_as_float(rr[cc * 32 + 2 * i]),
-                                               __uint_as_float(rr[cc * 32 + 2 * i + 1])),
-                                   sc2, nb2);
-            const float2 e = make_float2(ex2_approx(x.x), ex2_approx(x.y));
-            rsq[i & 1] = fadd2(rsq[i & 1], e);
-            pk[i] = pack_bf16x2(e.x, e.y);
+        const bool move = m_new > m_used + kLazyLog2;  // -inf + 64 = -inf
+        if (__any_sync(0xffffffffu, move)) {
+          const bool rescale = move && j > 0 && m_used != -INFINITY;
+          const float corr = rescale ? ex2_approx(m_used - m_new) : 1.f;
+          if (move) {
+            l *= ex2_approx(m_used - m_new);  // m_used = -inf: l is 0 and stays 0
+            m_used = m_new;
           }
-          tmem_st_16cols(s_col + cc * 16, pk);  // P: 32 keys per 16 columns
-        }
-        const float rs = (rsq[0].x + rsq[1].x) + (rsq[0].y + rsq[1].y);
-        if (__any_sync(0xffffffffu, rescale)) {
-          // O holds the piece's tiles before j, complete (covered by the commit
-          // of this S): move it to the new base before this PV adds to it
+          sum[0] = sum[1] = make_float2(0.f, 0.f);
+          half_exps<0>(rr, p.scale_log2, m_used, sum, pk);
+          if (__any_sync(0xffffffffu, rescale)) {
+            // O holds the piece's tiles before j, complete (covered by the commit
+            // of this S): move it to the new base before this PV adds to it
 #pragma unroll 1
-          for (int cc = 0; cc < kD / 32; ++cc) {
-            uint32_t r32[32];
-            tmem_ld_32cols(o_col + cc * 32, r32);
-            tc_wait_ld();
+            for (int cc = 0; cc < kD / 16; ++cc) {
+              uint32_t r16[16];
+              tmem_ld_16cols(o_col + cc * 16, r16);
+              tc_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) r32[i] = __float_as_uint(__uint_as_float(r32[i]) * corr);
-            tmem_st_32cols(o_col + cc * 32, r32);
+              for (int i = 0; i < 16; ++i)
+                r16[i] = __float_as_uint(__uint_as_float(r16[i]) * corr);
+              tmem_st_16cols(o_col + cc * 16, r16);
+            }
           }
         }
+        tmem_st_32cols(s_col, pk);  // P in place of S: 64 keys in 32 columns
         tc_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[t]);
-        l += rs;
+        if (lane == 0) mbar_arrive(&p_full[2 * t]);
+        half_exps<1>(rr, p.scale_log2, m_used, sum, pk);
+        tmem_st_32cols(s_col + 32, pk);
+        tc_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[2 * t + 1]);
+        l += (sum[0].x + sum[1].x) + (sum[0].y + sum[1].y);
       }
+      ok = ok && warp_ok(&o_final[t], ic & 1, p.err, 0x93d);
       if (!ok) break;
-      if (!warp_ok(&o_final[t], ic & 1, p.err, 0x93d)) { ok = false; break; }
       tc_fence_after();
       if (w.t0 == 0 && w.t1 == w.nt) {
         const float inv = l > 0.f ? 1.f / l : 0.f;
@@ -629,11 +744,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&o_empty[t]);
-      T += n_kb;
       ++ic;
     }
     if (!ok) *abort_flag = 1;
   }
+  __syncwarp();
   tc_fence_before();
   __syncthreads();
   if (warp == 1) {
