@@ -21,8 +21,9 @@
 // Bound by the tensor pipe and the softmax (4 * 128 flops per visible pair).
 // The lengths are only known on the device, so the 128-key tiles of all items,
 // plus one position per item for its fixed cost, form one list that is cut into
-// equal ranges, one per SM; a cut that falls within 1/16 of a range of an item's
-// edge moves there.  An item cut in the middle leaves fp32 pieces (O, base, sum)
+// equal ranges, one per SM; a cut within 2 tiles of an item's edge moves there (a
+// split costs about as much as a tile; with cuts moved by up to 1/16 of a range
+// the six-prompt case had 12 % more tiles on one SM than on average).  An item cut in the middle leaves fp32 pieces (O, base, sum)
 // in the workspace and a second kernel joins them in CTA order: a 512-token
 // chunk on a 32k cache fills every SM (its 64 items alone would fill 64).
 #include <math.h>
@@ -47,8 +48,10 @@ constexpr int kHalf = kKVBytes / 2;       // one 64-dim half of 128 rows
 constexpr int kBox = kHalf / 2;           // 64 rows of it: one TMA box of a page
 constexpr int kOffK = 2 * kQBytes;
 constexpr int kOffV = kOffK + 2 * kKVBytes;
-constexpr int kOffBar = kOffV + 2 * kKVBytes;
+constexpr int kOffOut = kOffV + 2 * kKVBytes;  // 4 KB per softmax warp: 32 rows x 64 dims
+constexpr int kOffBar = kOffOut + 8 * 4096;
 constexpr int kSmem = kOffBar + 256 + 1024;
+static_assert(kSmem + 1024 <= 227 * 1024, "shared memory (1 KB for the static part)");
 constexpr uint32_t kTmemCols = 512;       // S[0] S[1] O[0] O[1], 128 columns each
 // a row's base moves when its maximum has grown by more than 2^64: P, l and O are
 // relative to the base, and bf16 and fp32 hold 2^64 times any finite V
@@ -76,32 +79,10 @@ __device__ __forceinline__ bool warp_ok(uint64_t* bar, uint32_t parity, int* err
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, err, code));
 }
 
-// 2^x of a pair on the FMA pipe: the MUFU pipe's 16 exponentials a cycle take as
-// long as a tile's MMAs, so every fourth pair goes here.  x = j + f with j =
-// round(x) (the 1.5 * 2^23 shifter) and f in [-0.5, 0.5]; 2^f by the degree-4
-// polynomial of smallest maximum relative error (2.6e-6, fitted by reweighted
-// least squares), 2^j added to the exponent field.  P is rounded to bf16 (2^-8)
-// after it.  x is clamped to -126, where the result is below 2^-125 and
-// vanishes against the row's sum (masked keys: x = -inf).
-constexpr float kP0 = 0.9999992847442627f, kP1 = 0.6931217908859253f, kP2 = 0.240247443318367f,
-                kP3 = 0.05591785907745361f, kP4 = 0.009570102207362652f;
-__device__ __forceinline__ float2 exp2_fma(float2 x) {
-  constexpr float kShift = 12582912.0f;
-  x.x = fmaxf(x.x, -126.f);
-  x.y = fmaxf(x.y, -126.f);
-  const float2 t = fadd2(x, make_float2(kShift, kShift));
-  const float2 j = fadd2(t, make_float2(-kShift, -kShift));
-  const float2 f = ffma2(j, make_float2(-1.f, -1.f), x);
-  float2 q = ffma2(f, make_float2(kP4, kP4), make_float2(kP3, kP3));
-  q = ffma2(q, f, make_float2(kP2, kP2));
-  q = ffma2(q, f, make_float2(kP1, kP1));
-  q = ffma2(q, f, make_float2(kP0, kP0));
-  return make_float2(__int_as_float(__float_as_int(q.x) + (__float_as_int(t.x) << 23)),
-                     __int_as_float(__float_as_int(q.y) + (__float_as_int(t.y) << 23)));
-}
-
 // The exponentials of keys 64 * HALF .. + 63 of a row against base m: their bf16
-// pairs and the sums of the unrounded values.
+// pairs and the sums of the unrounded values.  All on the MUFU pipe: with a
+// quarter of them as polynomials on the FMA pipe the six-prompt case took 561 us
+// against 520 (a thread's chain of instructions is what is long, not one pipe).
 template <int HALF>
 __device__ __forceinline__ void half_exps(const uint32_t (&rr)[kN], float scale_log2, float m,
                                           float2 (&sum)[2], uint32_t (&pk)[32]) {
@@ -113,7 +94,7 @@ __device__ __forceinline__ void half_exps(const uint32_t (&rr)[kN], float scale_
     const float2 x = ffma2(make_float2(__uint_as_float(rr[HALF * 64 + 2 * i]),
                                        __uint_as_float(rr[HALF * 64 + 2 * i + 1])),
                            sc2, nb2);
-    const float2 e = (i & 3) == 3 ? exp2_fma(x) : make_float2(ex2_approx(x.x), ex2_approx(x.y));
+    const float2 e = make_float2(ex2_approx(x.x), ex2_approx(x.y));
     sum[i & 1] = fadd2(sum[i & 1], e);
     pk[i] = pack_bf16x2(e.x, e.y);
   }
@@ -308,6 +289,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   __shared__ int64_t s_warp[kThreads / 32];
   __shared__ Walk s_walk;
+  __shared__ int s_row[kM];  // token (low 16 bits) and head of a tile's row
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -339,6 +321,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == 1) {
     tmem_alloc(tmem_slot, kTmemCols);
     tmem_relinquish();
+  }
+  if (threadIdx.x < kM) {
+    const int tk = threadIdx.x / p.G;
+    // rows past the last (token, head) pair: a token past any request's end
+    s_row[threadIdx.x] = (int)threadIdx.x < p.T * p.G ? tk | (threadIdx.x - tk * p.G) << 16 : 0x7fff;
   }
 
   // ---- this CTA's range of the list (every CTA scans the lengths) ----
@@ -394,7 +381,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         s_walk.item = lo;
         s_walk.n = n;
         s_walk.nt = n_tiles(p, r, lo);
-        s_walk.snap = (int)min64(U / nc / 16, 1 << 20);
+        s_walk.snap = (int)min64(U / nc / 8, 2);
         s_walk.pos = rem - places(p, r, lo);
         s_walk.u = u0 - s_walk.pos;
         s_walk.left = u1 - u0;
@@ -608,7 +595,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int t = (warp >> 2) - 1;  // query tile
     const int quarter = warp & 3;   // TMEM lane quarter of this warp
     const int row = quarter * 32 + lane;
-    const int tok_in = row / p.G, head_in = row - tok_in * p.G;
+    const int tok_in = row / p.G;
     const bool row_used = row < p.T * p.G;
     const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
     const uint32_t s_col = tmem + lane_off + t * kN;
@@ -635,15 +622,21 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_wait_ld();
         const int kbase = (w.t0 + j) * kN;
         if (kbase + kN - 1 > see_min) {
-          const int lim = see - kbase;
+          const int lim = see - kbase;  // the last key this row sees
 #pragma unroll
-          for (int i = 0; i < kN; ++i)
-            if (i > lim) rr[i] = __float_as_uint(-INFINITY);
+          for (int cc = 0; cc < kN / 32; ++cc) {
+            const int n = lim - cc * 32;
+            const uint32_t seen = n >= 31 ? 0xffffffffu : n < 0 ? 0u : (2u << n) - 1u;
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (!((seen >> i) & 1)) rr[cc * 32 + i] = __float_as_uint(-INFINITY);
+          }
         }
         // P = 2^(S scale - base).  The first 64 keys' exponentials are taken
         // against the old base while the tile's maximum is still being found, and
-        // taken again in a tile that moves the base (an item's first, and after
-        // that one where the maximum has grown by 2^64).
+        // taken again in a tile that moves the base: an item's first, and one
+        // where the maximum has grown by 2^64.  (No branch around them: the
+        // compiler overlaps them with the maximum.)
         float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
         uint32_t pk[32];
         half_exps<0>(rr, p.scale_log2, m_used, sum, pk);
@@ -699,27 +692,45 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_after();
       if (w.t0 == 0 && w.t1 == w.nt) {
         const float inv = l > 0.f ? 1.f / l : 0.f;
-        __nv_bfloat16* dst = p.out + (int64_t)(w.r.q0 + tok) * p.out_stride +
-                             (int64_t)(w.kvh * p.G + head_in) * kD;
+        // 64 dims of the warp's 32 rows at a time through shared memory, so that
+        // eight lanes write 128 bytes of a row (a thread writing its own row
+        // touched 32 lines per store: 5000 cycles per item)
+        uint8_t* stage = smem + kOffOut + (warp - 4) * 4096;
+        const int r4 = lane >> 3, u8 = lane & 7;
+        const int n_tok = min(w.r.q_len - tile_tok, p.T);  // tokens of the tile
+        __nv_bfloat16* dst =
+            p.out + (int64_t)(w.r.q0 + tile_tok) * p.out_stride + (int64_t)w.kvh * p.G * kD;
 #pragma unroll
-        for (int cc = 0; cc < kD / 32; ++cc) {
-          uint32_t r32[32];
-          tmem_ld_32cols(o_col + cc * 32, r32);
-          tc_wait_ld();
-          if (live) {
+        for (int hd = 0; hd < 2; ++hd) {
 #pragma unroll
-            for (int d = 0; d < 32; d += 8) {
+          for (int cc = 0; cc < 2; ++cc) {
+            uint32_t r32[32];
+            tmem_ld_32cols(o_col + hd * 64 + cc * 32, r32);
+            tc_wait_ld();
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {
               uint4 u;
-              u.x = pack_bf16x2(__uint_as_float(r32[d]) * inv, __uint_as_float(r32[d + 1]) * inv);
-              u.y = pack_bf16x2(__uint_as_float(r32[d + 2]) * inv,
-                                __uint_as_float(r32[d + 3]) * inv);
-              u.z = pack_bf16x2(__uint_as_float(r32[d + 4]) * inv,
-                                __uint_as_float(r32[d + 5]) * inv);
-              u.w = pack_bf16x2(__uint_as_float(r32[d + 6]) * inv,
-                                __uint_as_float(r32[d + 7]) * inv);
-              *reinterpret_cast<uint4*>(dst + cc * 32 + d) = u;
+              u.x = pack_bf16x2(__uint_as_float(r32[8 * d]) * inv, __uint_as_float(r32[8 * d + 1]) * inv);
+              u.y = pack_bf16x2(__uint_as_float(r32[8 * d + 2]) * inv,
+                                __uint_as_float(r32[8 * d + 3]) * inv);
+              u.z = pack_bf16x2(__uint_as_float(r32[8 * d + 4]) * inv,
+                                __uint_as_float(r32[8 * d + 5]) * inv);
+              u.w = pack_bf16x2(__uint_as_float(r32[8 * d + 6]) * inv,
+                                __uint_as_float(r32[8 * d + 7]) * inv);
+              *reinterpret_cast<uint4*>(stage + lane * 128 + (((cc * 4 + d) ^ (lane & 7)) << 4)) = u;
             }
           }
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int r = i * 4 + r4, rt = quarter * 32 + r;  // row of the warp, of the tile
+            const uint4 u =
+                *reinterpret_cast<const uint4*>(stage + r * 128 + ((u8 ^ (r & 7)) << 4));
+            const int tk = s_row[rt] & 0xffff, hh = s_row[rt] >> 16;
+            if (tk < n_tok)
+              *reinterpret_cast<uint4*>(dst + tk * p.out_stride + hh * kD + hd * 64 + u8 * 8) = u;
+          }
+          __syncwarp();
         }
       } else {
         // a piece of an item: O relative to m_used, the base and the sum.  A

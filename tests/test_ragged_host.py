@@ -237,7 +237,7 @@ def prefill_ranges(qs, Ls, T, Hkv, grid, causal=True):
                 items.append(((b, h, i), nt, u))
                 u += nt + 1
     U, nc = u, min(grid, u)
-    snap = U // nc // 16 if nc else 0
+    snap = min(U // nc // 8, 2) if nc else 0
     pieces, desc, at = [], {}, 0
     for c in range(nc):
         u0, u1 = U * c // nc, U * (c + 1) // nc
