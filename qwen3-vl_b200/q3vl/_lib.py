@@ -171,12 +171,14 @@ def exported_symbols() -> list[str]:
     return list(SIGNATURES)
 
 
-def call(name: str, *args) -> None:
-    lib = load()
-    rc = getattr(lib, name)(*args)
+def check(rc: int, name: str) -> None:
+    """Raise Q3Error with the library's message for a non-zero status."""
     if rc != Q3_OK:
-        msg = lib.q3_last_error().decode(errors="replace")
-        raise Q3Error(rc, name, msg)
+        raise Q3Error(rc, name, load().q3_last_error().decode(errors="replace"))
+
+
+def call(name: str, *args) -> None:
+    check(getattr(load(), name)(*args), name)
 
 
 def raw(name: str):

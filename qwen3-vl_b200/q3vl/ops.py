@@ -1015,62 +1015,85 @@ class RaggedPlan(NamedTuple):
     counts: torch.Tensor     # int32 [2] packed tokens, pages taken from the free list
 
 
-def _ragged_device(name: str, *ts) -> torch.device:
-    """The one CUDA device of the tensors."""
-    dev = ts[0].device
+# These calls are made for every layer of every step, often for a few rows, so
+# the host's part is kept small: one pass over the arguments, no ctypes objects,
+# the raw stream handle, few allocations.
+def _ragged_device(name: str, *ts) -> int:
+    """Index of the one CUDA device of the tensors."""
+    dev = ts[0].get_device()
     for t in ts:
-        if t is not None and (not t.is_cuda or t.device != dev):
+        if t is not None and t.get_device() != dev or dev < 0:
             raise RuntimeError(f"{name}: tensors must be on one CUDA device (no CPU fallback); "
-                               f"got {dev} and {t.device}")
+                               f"got {[str(t.device) for t in ts if t is not None]}")
     return dev
 
 
-def _ragged_call(name: str, dev: torch.device, *args) -> None:
+def _ragged_call(name: str, dev: int, *args) -> None:
     """call() on the current stream of the tensors' own device."""
-    if dev.index == torch.cuda.current_device():
-        call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
+    if dev == torch.cuda.current_device():
+        rc = _lib.raw(name)(*args, torch._C._cuda_getCurrentRawStream(dev))
     else:
         with torch.cuda.device(dev):
-            call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
-
-
-def _ragged_ints(name: str, dtype, **ts) -> None:
-    for k, t in ts.items():
-        if t is not None and (t.dtype != dtype or not t.is_contiguous()):
-            raise TypeError(f"{name}: {k} must be contiguous {dtype}")
+            rc = _lib.raw(name)(*args, torch._C._cuda_getCurrentRawStream(dev))
+    if rc:
+        _lib.check(rc, name)
 
 
 def _ragged_rows(name: str, what: str, t: torch.Tensor) -> int:
     """Row stride of a bf16 [rows, heads, 128] tensor whose rows are dense."""
     rows, heads, d = t.shape
-    s0, s1, s2 = t.stride()
     if t.dtype != torch.bfloat16:
         raise TypeError(f"{name}: {what} must be bfloat16, got {t.dtype}")
+    if d == HEAD_DIM and t.is_contiguous():
+        return heads * HEAD_DIM
+    s0, s1, s2 = t.stride()
     if d != HEAD_DIM or s2 != 1 or (s1 != HEAD_DIM and heads > 1):
         raise ValueError(f"{name}: {what} must be [rows, heads, 128] with dense rows, got "
                          f"{tuple(t.shape)} with strides {t.stride()}")
     return s0 if rows > 1 else heads * HEAD_DIM
 
 
+def _ragged_out(name: str, out, q: torch.Tensor, q_stride: int):
+    """The output tensor, new or the caller's, and its row stride."""
+    if out is None:
+        if q.is_contiguous():
+            return torch.empty_like(q), q_stride
+        return q.new_empty(q.shape), q.shape[1] * HEAD_DIM
+    if out.shape != q.shape:
+        raise ValueError(f"{name}: out must be {tuple(q.shape)}, got {tuple(out.shape)}")
+    return out, _ragged_rows(name, "out", out)
+
+
 def _ragged_pool(name: str, k_pages: torch.Tensor, v_pages: torch.Tensor):
+    shape = k_pages.shape
     if k_pages.dtype != torch.bfloat16 or v_pages.dtype != torch.bfloat16:
         raise TypeError(f"{name}: k_pages and v_pages must be bfloat16")
-    if (k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.shape[3] != HEAD_DIM or
+    if (len(shape) != 4 or shape != v_pages.shape or shape[3] != HEAD_DIM or
             not k_pages.is_contiguous() or not v_pages.is_contiguous()):
         raise ValueError(f"{name}: k_pages and v_pages must be contiguous "
                          f"[num_pages, Hkv, page_tokens, 128], got {tuple(k_pages.shape)} and "
                          f"{tuple(v_pages.shape)}")
-    return k_pages.shape[:3]
+    return shape
 
 
-def _ragged_table(name: str, t: torch.Tensor, B: int) -> int:
-    """Row stride of an int32 [B, width] block table."""
+def _ragged_table(name: str, t: torch.Tensor, B: int):
+    """Row stride and width of an int32 [B, width] block table."""
     if t.dtype != torch.int32:
         raise TypeError(f"{name}: block_table must be int32, got {t.dtype}")
     if t.dim() != 2 or t.shape[0] != B or (t.stride(1) != 1 and t.shape[1] > 1):
         raise ValueError(f"{name}: block_table must be [{B}, width] with dense rows, got "
                          f"{tuple(t.shape)} with strides {t.stride()}")
-    return t.stride(0) if B > 1 else t.shape[1]
+    width = t.shape[1]
+    return (t.stride(0) if B > 1 else width), width
+
+
+def _ragged_ints(name: str, what: str, t: torch.Tensor, dtype, n: int) -> int:
+    """Address of a contiguous integer tensor of n entries."""
+    if t.dtype != dtype or not t.is_contiguous():
+        raise TypeError(f"{name}: {what} must be contiguous {dtype}")
+    if t.numel() != n:
+        raise ValueError(f"{name}: {what} must have {n} entries, got {t.numel()}")
+    return t.data_ptr()
 
 
 def ragged_plan(q_lens: torch.Tensor, past_lens: torch.Tensor, block_table: torch.Tensor, *,
@@ -1089,26 +1112,27 @@ def ragged_plan(q_lens: torch.Tensor, past_lens: torch.Tensor, block_table: torc
     0x903 in the device error word, when it was short)."""
     name = "ragged_plan"
     dev = _ragged_device(name, q_lens, past_lens, block_table, free_pages, rope_delta)
-    _ragged_ints(name, torch.int32, q_lens=q_lens, past_lens=past_lens, free_pages=free_pages)
-    _ragged_ints(name, torch.int64, rope_delta=rope_delta)
-    B = q_lens.numel()
-    if past_lens.numel() != B or (rope_delta is not None and rope_delta.numel() != B):
-        raise ValueError(f"{name}: past_lens and rope_delta must have {B} entries")
-    stride = _ragged_table(name, block_table, B)
-    n = int(n_tokens)
+    B, n = q_lens.numel(), int(n_tokens)
     if n < 0:
         raise ValueError(f"{name}: n_tokens={n}")
-    i64 = torch.empty(2, n, dtype=torch.int64, device=dev)
-    i32 = torch.empty(n + 2 * B + 3, dtype=torch.int32, device=dev)
-    requests, cu_q, kv_lens, counts = i32.split((n, B + 1, B, 2))
-    at64, at32 = i64.data_ptr(), i32.data_ptr()
-    _ragged_call("q3_ragged_plan", dev, q_lens.data_ptr(), past_lens.data_ptr(), B,
-                 block_table.data_ptr(), stride, block_table.shape[1], int(page_tokens),
-                 None if free_pages is None else free_pages.data_ptr(),
-                 0 if free_pages is None else free_pages.numel(),
-                 None if rope_delta is None else rope_delta.data_ptr(), n, at32 + 4 * n,
-                 at32 + 4 * (n + B + 1), at32, at64, at64 + 8 * n, at32 + 4 * (n + 2 * B + 1))
-    return RaggedPlan(cu_q, kv_lens, requests, i64[0], i64[1], counts)
+    stride, width = _ragged_table(name, block_table, B)
+    n_free = 0 if free_pages is None else free_pages.numel()
+    # one allocation for the six results (the 64-bit ones first, for alignment)
+    buf = q_lens.new_empty(5 * n + 2 * B + 3)
+    positions, slots, requests, cu_q, kv_lens, counts = buf.split_with_sizes(
+        (2 * n, 2 * n, n, B + 1, B, 2))
+    at = buf.data_ptr()
+    at_cu = at + 20 * n
+    _ragged_call("q3_ragged_plan", dev, _ragged_ints(name, "q_lens", q_lens, torch.int32, B),
+                 _ragged_ints(name, "past_lens", past_lens, torch.int32, B), B,
+                 block_table.data_ptr(), stride, width, page_tokens,
+                 None if free_pages is None else
+                 _ragged_ints(name, "free_pages", free_pages, torch.int32, n_free), n_free,
+                 None if rope_delta is None else
+                 _ragged_ints(name, "rope_delta", rope_delta, torch.int64, B), n, at_cu,
+                 at_cu + 4 * (B + 1), at + 16 * n, at, at + 8 * n, at_cu + 4 * (2 * B + 1))
+    return RaggedPlan(cu_q, kv_lens, requests, positions.view(torch.int64),
+                      slots.view(torch.int64), counts)
 
 
 def qkv_norm_rope_ragged(qkv: torch.Tensor, q_norm_w: torch.Tensor, k_norm_w: torch.Tensor,
@@ -1127,38 +1151,38 @@ def qkv_norm_rope_ragged(qkv: torch.Tensor, q_norm_w: torch.Tensor, k_norm_w: to
     name = "qkv_norm_rope_ragged"
     dev = _ragged_device(name, qkv, q_norm_w, k_norm_w, positions, inv_freq, slots, k_pages,
                          v_pages, out)
-    _bf16(name, qkv, q_norm_w, k_norm_w)
-    _ragged_ints(name, torch.int64, slots=slots)
-    num_pages, heads, page_tokens = _ragged_pool(name, k_pages, v_pages)
+    num_pages, heads, page_tokens, _ = _ragged_pool(name, k_pages, v_pages)
     if heads != Hkv:
         raise ValueError(f"{name}: the pool has {heads} K/V heads, Hkv is {Hkv}")
     width = (Hq + 2 * Hkv) * HEAD_DIM
+    _bf16(name, qkv, q_norm_w, k_norm_w)
     if qkv.dim() != 2 or qkv.shape[1] != width or qkv.stride(1) != 1:
-        raise ValueError(f"{name}: qkv must be [n, {width}] with dense rows")
+        raise ValueError(f"{name}: qkv must be [n, {width}] with dense rows, got "
+                         f"{tuple(qkv.shape)}")
     n = qkv.shape[0]
-    if positions.dtype != torch.int64 or positions.dim() not in (1, 2) or \
-            (positions.dim() == 2 and positions.shape[0] != 3) or positions.shape[-1] != n or \
-            (positions.stride(-1) != 1 and n > 1):
-        raise ValueError(f"{name}: positions must be int64 [{n}] or [3, {n}]")
-    if slots.numel() != n:
-        raise ValueError(f"{name}: {slots.numel()} slots for {n} tokens")
-    if q_norm_w.numel() != HEAD_DIM or k_norm_w.numel() != HEAD_DIM or \
-            not q_norm_w.is_contiguous() or not k_norm_w.is_contiguous():
+    pos_shape = positions.shape
+    if (positions.dtype != torch.int64 or pos_shape not in ((n,), (3, n)) or
+            (positions.stride(-1) != 1 and n > 1)):
+        raise ValueError(f"{name}: positions must be int64 [{n}] or [3, {n}], got "
+                         f"{positions.dtype} {tuple(pos_shape)}")
+    if (q_norm_w.numel() != HEAD_DIM or k_norm_w.numel() != HEAD_DIM or
+            not q_norm_w.is_contiguous() or not k_norm_w.is_contiguous()):
         raise ValueError(f"{name}: norm weights must be contiguous [128]")
-    if inv_freq.dtype != torch.float32 or inv_freq.numel() != HEAD_DIM // 2 or \
-            not inv_freq.is_contiguous():
+    if (inv_freq.dtype != torch.float32 or inv_freq.numel() != HEAD_DIM // 2 or
+            not inv_freq.is_contiguous()):
         raise ValueError(f"{name}: inv_freq must be contiguous float32 [64]")
     if out is None:
-        out = torch.empty(n, Hq, HEAD_DIM, dtype=torch.bfloat16, device=dev)
-    elif tuple(out.shape) != (n, Hq, HEAD_DIM):
-        raise ValueError(f"{name}: out must be [{n}, {Hq}, 128]")
+        out, out_stride = qkv.new_empty((n, Hq, HEAD_DIM)), Hq * HEAD_DIM
+    elif out.shape != (n, Hq, HEAD_DIM):
+        raise ValueError(f"{name}: out must be [{n}, {Hq}, 128], got {tuple(out.shape)}")
+    else:
+        out_stride = _ragged_rows(name, "out", out)
     _ragged_call("q3_qkv_norm_rope_ragged", dev, qkv.data_ptr(),
                  qkv.stride(0) if n > 1 else width, q_norm_w.data_ptr(), k_norm_w.data_ptr(),
-                 positions.data_ptr(), positions.stride(0) if positions.dim() == 2 else 0,
-                 inv_freq.data_ptr(), slots.data_ptr(), out.data_ptr(),
-                 _ragged_rows(name, "out", out), k_pages.data_ptr(), v_pages.data_ptr(), n, Hq,
-                 Hkv, HEAD_DIM, page_tokens, num_pages, int(mrope_section[1]),
-                 int(mrope_section[2]), float(eps))
+                 positions.data_ptr(), positions.stride(0) if len(pos_shape) == 2 else 0,
+                 inv_freq.data_ptr(), _ragged_ints(name, "slots", slots, torch.int64, n),
+                 out.data_ptr(), out_stride, k_pages.data_ptr(), v_pages.data_ptr(), n, Hq, Hkv,
+                 HEAD_DIM, page_tokens, num_pages, mrope_section[1], mrope_section[2], eps)
     return out
 
 
@@ -1173,26 +1197,20 @@ def attn_decode_ragged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Te
     gives zeros.  Hq / Hkv is any whole number up to 16."""
     name = "attn_decode_ragged"
     dev = _ragged_device(name, q, k_pages, v_pages, block_table, kv_lens, out)
-    _ragged_ints(name, torch.int32, kv_lens=kv_lens)
-    num_pages, Hkv, page_tokens = _ragged_pool(name, k_pages, v_pages)
+    num_pages, Hkv, page_tokens, _ = _ragged_pool(name, k_pages, v_pages)
     if q.dim() != 3:
-        raise ValueError(f"{name}: q must be [B, Hq, 128]")
-    q_stride = _ragged_rows(name, "q", q)
+        raise ValueError(f"{name}: q must be [B, Hq, 128], got {tuple(q.shape)}")
     B, Hq, D = q.shape
-    if kv_lens.numel() != B:
-        raise ValueError(f"{name}: {kv_lens.numel()} lengths for {B} requests")
-    table_stride = _ragged_table(name, block_table, B)
-    if out is None:
-        out = torch.empty(B, Hq, D, dtype=torch.bfloat16, device=dev)
-    elif out.shape != q.shape:
-        raise ValueError(f"{name}: out must match q")
+    q_stride = _ragged_rows(name, "q", q)
+    table_stride, width = _ragged_table(name, block_table, B)
+    out, out_stride = _ragged_out(name, out, q, q_stride)
     nbytes = _lib.raw("q3_attn_decode_ragged_workspace_bytes")(Hq, Hkv)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    ws = q.new_empty(nbytes, dtype=torch.uint8)
     _ragged_call("q3_attn_decode_ragged", dev, q.data_ptr(), q_stride, k_pages.data_ptr(),
-                 v_pages.data_ptr(), out.data_ptr(), _ragged_rows(name, "out", out), B, Hq, Hkv, D,
-                 block_table.data_ptr(), table_stride, block_table.shape[1], page_tokens,
-                 num_pages, kv_lens.data_ptr(),
-                 1.0 / math.sqrt(D) if scale is None else float(scale), ws.data_ptr(), nbytes)
+                 v_pages.data_ptr(), out.data_ptr(), out_stride, B, Hq, Hkv, D,
+                 block_table.data_ptr(), table_stride, width, page_tokens, num_pages,
+                 _ragged_ints(name, "kv_lens", kv_lens, torch.int32, B),
+                 HEAD_DIM ** -0.5 if scale is None else scale, ws.data_ptr(), nbytes)
     return out
 
 
@@ -1210,27 +1228,22 @@ def attn_prefill_ragged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.T
     gives zeros.  Hq / Hkv is any whole number up to 16; scale is positive."""
     name = "attn_prefill_ragged"
     dev = _ragged_device(name, q, k_pages, v_pages, block_table, cu_q, kv_lens, out)
-    _ragged_ints(name, torch.int32, cu_q=cu_q, kv_lens=kv_lens)
-    num_pages, Hkv, page_tokens = _ragged_pool(name, k_pages, v_pages)
+    num_pages, Hkv, page_tokens, _ = _ragged_pool(name, k_pages, v_pages)
     if q.dim() != 3:
-        raise ValueError(f"{name}: q must be [n, Hq, 128]")
-    q_stride = _ragged_rows(name, "q", q)
+        raise ValueError(f"{name}: q must be [n, Hq, 128], got {tuple(q.shape)}")
     n, Hq, D = q.shape
     B = kv_lens.numel()
-    if cu_q.numel() != B + 1:
-        raise ValueError(f"{name}: cu_q must have {B + 1} entries for {B} requests")
-    table_stride = _ragged_table(name, block_table, B)
-    if out is None:
-        out = torch.empty(n, Hq, D, dtype=torch.bfloat16, device=dev)
-    elif out.shape != q.shape:
-        raise ValueError(f"{name}: out must match q")
+    q_stride = _ragged_rows(name, "q", q)
+    table_stride, width = _ragged_table(name, block_table, B)
+    out, out_stride = _ragged_out(name, out, q, q_stride)
     nbytes = _lib.raw("q3_attn_prefill_ragged_workspace_bytes")()
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    ws = q.new_empty(nbytes, dtype=torch.uint8)
     _ragged_call("q3_attn_prefill_ragged", dev, q.data_ptr(), q_stride, k_pages.data_ptr(),
-                 v_pages.data_ptr(), out.data_ptr(), _ragged_rows(name, "out", out), n, B, Hq, Hkv,
-                 D, block_table.data_ptr(), table_stride, block_table.shape[1], page_tokens,
-                 num_pages, cu_q.data_ptr(), kv_lens.data_ptr(), 1 if causal else 0,
-                 1.0 / math.sqrt(D) if scale is None else float(scale), ws.data_ptr(), nbytes)
+                 v_pages.data_ptr(), out.data_ptr(), out_stride, n, B, Hq, Hkv, D,
+                 block_table.data_ptr(), table_stride, width, page_tokens, num_pages,
+                 _ragged_ints(name, "cu_q", cu_q, torch.int32, B + 1),
+                 _ragged_ints(name, "kv_lens", kv_lens, torch.int32, B), 1 if causal else 0,
+                 HEAD_DIM ** -0.5 if scale is None else scale, ws.data_ptr(), nbytes)
     return out
 
 
