@@ -188,8 +188,8 @@ Q3_API int q3_ragged_plan(const int32_t* q_lens, const int32_t* past_lens, int B
  * q_out [n_tokens, Hq, 128], row stride q_stride; the K and V rows of token i
  * go to position slots[i] % page_tokens of page slots[i] / page_tokens.  fp32
  * throughout with one rounding at the end (angles reduced in fp64).  A token
- * whose slot is -1 is padding: nothing of it is read or written.  A slot
- * outside the pool is recorded (0x911) and its token skipped. */
+ * whose slot is -1 is padding: nothing of it is written.  A slot outside the
+ * pool is recorded (0x911) and its token skipped. */
 Q3_API int q3_qkv_norm_rope_ragged(const void* qkv, int64_t qkv_stride, const void* q_norm_w,
                                    const void* k_norm_w, const int64_t* positions,
                                    int64_t pos_axis_stride, const float* inv_freq,

@@ -17,11 +17,13 @@
 // before the fp32 sine and cosine: an fp32 product is off by 4e-3 rad at
 // position 10^5.
 //
-// Bound by HBM: each qkv row is read once, each q, k, v row written once.
-// Eight lanes own one head row; lane l holds dims 8l..8l+7 and their rotation
-// partners 64+8l..64+8l+7 (two 16-byte loads), so the rotation needs no
-// shuffle and a pair shares one cosine and sine.  A CTA takes a few tokens: 64
-// threads per token compute the angles once for all heads.
+// Bound by HBM: each qkv row is read once, each q, k, v row written once.  A warp
+// takes one token (or, when there are few tokens, a part of its heads) and waits
+// for no other warp: each lane computes two of the 64 angles and the warp shares
+// them.  Eight lanes own one head row; lane l holds dims 8l..8l+7 and their
+// rotation partners 64+8l..64+8l+7, so the rotation needs no shuffle, and the
+// factors w_j cos a_j, w_{j+64} sin a_j, w_{j+64} cos a_j, w_j sin a_j of its dims
+// stay in registers for all heads.
 #include <math.h>
 
 #include "common.cuh"
@@ -30,8 +32,13 @@ namespace q3 {
 namespace {
 
 constexpr int kRD = 128;
-constexpr int kRThreads = 256;
-constexpr int kRRows = kRThreads / 8;  // head rows per CTA pass
+constexpr int kRWarps = 2;   // per CTA
+// Quads of rows whose loads are in flight together.  16384 tokens of 32 + 2 x 8
+// heads, 403 MB: 70.6 us (5.7 TB/s, 0.88 of a copy) with 4 quads, 75 with 8
+// (fewer warps fit), 80 with 3, 90 with 1; 8 warps per CTA 73; a CTA of 256
+// threads sharing the angles of 4 tokens 83, the same fed by bulk copies into a
+// shared-memory ring 95 (a barrier per stage)
+constexpr int kRUnroll = 4;
 
 struct RaggedRopeParams {
   const __nv_bfloat16* qkv;
@@ -47,123 +54,166 @@ struct RaggedRopeParams {
   __nv_bfloat16* k_pages;
   __nv_bfloat16* v_pages;
   int64_t n_slots;
-  int n, Hq, Hkv, page_tokens, sec_h, sec_w;
+  int n, parts, Hq, Hkv, page_tokens, sec_h, sec_w;
   float eps;
   int* err;
 };
 
-__device__ __forceinline__ void unpack8(const uint4& u, float (&v)[8]) {
-  const float2 a = unpack_bf16x2(u.x), b = unpack_bf16x2(u.y), c = unpack_bf16x2(u.z),
-               d = unpack_bf16x2(u.w);
-  v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
-  v[4] = c.x; v[5] = c.y; v[6] = d.x; v[7] = d.y;
+// Eight bf16 values as four fp32 pairs, and back.
+__device__ __forceinline__ void unpack8(const uint4& u, float2 (&v)[4]) {
+  v[0] = unpack_bf16x2(u.x);
+  v[1] = unpack_bf16x2(u.y);
+  v[2] = unpack_bf16x2(u.z);
+  v[3] = unpack_bf16x2(u.w);
 }
-__device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
-  return make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
-                    pack_bf16x2(v[6], v[7]));
+__device__ __forceinline__ uint4 pack8(const float2 (&v)[4]) {
+  return make_uint4(pack_bf16x2(v[0].x, v[0].y), pack_bf16x2(v[1].x, v[1].y),
+                    pack_bf16x2(v[2].x, v[2].y), pack_bf16x2(v[3].x, v[3].y));
+}
+__device__ __forceinline__ float2 fmul2(float2 a, float2 b) {
+  return ffma2(a, b, make_float2(-0.f, -0.f));
 }
 
-template <int TPC>
-__global__ void __launch_bounds__(kRThreads) qkv_norm_rope_ragged_kernel(RaggedRopeParams p) {
-  __shared__ __align__(16) float s_cos[TPC][64];
-  __shared__ __align__(16) float s_sin[TPC][64];
-  __shared__ int64_t s_kv[TPC];  // element offset of (slot, KV head 0); -1: skip the token
-  pdl_launch();
+// A lane's factors: a' = rs (a ac + b bs), b' = rs (b bc + a as).
+struct Factors {
+  float2 ac[4], bs[4], bc[4], as[4];
+};
+__device__ __forceinline__ void make_factors(const __nv_bfloat16* w, int l, const float2 (&cs)[4],
+                                             const float2 (&sn)[4], Factors& f) {
+  float2 wa[4], wb[4];
+  unpack8(reinterpret_cast<const uint4*>(w)[l], wa);
+  unpack8(reinterpret_cast<const uint4*>(w)[8 + l], wb);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f.ac[i] = fmul2(wa[i], cs[i]);
+    f.bc[i] = fmul2(wb[i], cs[i]);
+    f.as[i] = fmul2(wa[i], sn[i]);
+    f.bs[i] = fmul2(wb[i], make_float2(-sn[i].x, -sn[i].y));
+  }
+}
+// Norm and rotation of the row that this lane's group of eight holds.
+__device__ __forceinline__ void norm_rotate(uint4& lo, uint4& hi, const Factors& f, float eps) {
+  float2 a[4], b[4];
+  unpack8(lo, a);
+  unpack8(hi, b);
+  float2 q = ffma2(b[0], b[0], fmul2(a[0], a[0]));
+#pragma unroll
+  for (int i = 1; i < 4; ++i) q = ffma2(a[i], a[i], ffma2(b[i], b[i], q));
+  float ss = q.x + q.y;
+  ss += __shfl_xor_sync(0xffffffffu, ss, 1);
+  ss += __shfl_xor_sync(0xffffffffu, ss, 2);
+  ss += __shfl_xor_sync(0xffffffffu, ss, 4);
+  const float rs = rsqrtf(ss * (1.0f / kRD) + eps);
+  const float2 rs2 = make_float2(rs, rs);
+  float2 oa[4], ob[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    oa[i] = fmul2(rs2, ffma2(a[i], f.ac[i], fmul2(b[i], f.bs[i])));
+    ob[i] = fmul2(rs2, ffma2(b[i], f.bc[i], fmul2(a[i], f.as[i])));
+  }
+  lo = pack8(oa);
+  hi = pack8(ob);
+}
+
+__global__ void __launch_bounds__(kRWarps * 32) qkv_norm_rope_ragged_kernel(RaggedRopeParams p) {
+  // No early launch of the next kernel: one that reads cache rows before its own
+  // wait (attn_decode_paged streams old rows) must not start before these are
+  // written.
   pdl_wait();
-  const int t0 = blockIdx.x * TPC;
-  const int H = p.Hq + 2 * p.Hkv;
-  if (threadIdx.x < TPC) {
-    const int t = t0 + threadIdx.x;
-    int64_t off = -1;
-    if (t < p.n) {
-      const int64_t slot = p.slots[t];
-      if (slot >= 0 && slot < p.n_slots) {
-        const uint32_t pg = (uint32_t)slot / (uint32_t)p.page_tokens;
-        off = ((int64_t)pg * p.Hkv * p.page_tokens +
-               ((uint32_t)slot - pg * (uint32_t)p.page_tokens)) * kRD;
-      } else if (slot != -1) {
-        report_timeout(p.err, 0x911);
+  const int lane = threadIdx.x & 31, l = lane & 7, grp = lane >> 3;
+  const int64_t unit = (int64_t)blockIdx.x * kRWarps + (threadIdx.x >> 5);
+  if (unit >= (int64_t)p.n * p.parts) return;
+  const int t = (int)(unit / p.parts), part = (int)(unit - (int64_t)t * p.parts);
+  const int64_t slot = p.slots[t];
+  if (slot < 0 || slot >= p.n_slots) {  // the whole warp
+    if (slot != -1 && lane == 0) report_timeout(p.err, 0x911);
+    return;
+  }
+  // this part's heads, in quads: of q, and of k and v together
+  const int nq = (p.Hq + 3) / 4, nkv = (2 * p.Hkv + 3) / 4;
+  const int q0 = nq * part / p.parts * 4, q1 = min(nq * (part + 1) / p.parts * 4, p.Hq);
+  const int k0 = nkv * part / p.parts * 4, k1 = min(nkv * (part + 1) / p.parts * 4, 2 * p.Hkv);
+  const uint4* src = reinterpret_cast<const uint4*>(p.qkv + (int64_t)t * p.qkv_stride) + l;
+
+  uint4 lo[kRUnroll], hi[kRUnroll];
+  auto load_q = [&](int base) {
+#pragma unroll
+    for (int u = 0; u < kRUnroll; ++u) {
+      const int h = min(base + 4 * u + grp, p.Hq - 1);
+      lo[u] = __ldcs(src + h * 16);
+      hi[u] = __ldcs(src + h * 16 + 8);
+    }
+  };
+  if (q0 < q1) load_q(q0);
+  // angles j = lane and lane + 32, as half turns (a / pi) reduced to [-1, 1]
+  float cv[2], sv[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int j = lane + 32 * i;
+    const int axis = (j % 3 == 1 && j < 3 * p.sec_h) ? 1 : (j % 3 == 2 && j < 3 * p.sec_w) ? 2 : 0;
+    double h = (double)p.pos[axis * p.pos_stride + t] * (double)p.inv_freq[j] *
+               0.31830988618379067154;
+    h -= 2.0 * rint(0.5 * h);
+    sincospif((float)h, &sv[i], &cv[i]);
+  }
+  // angles 8l .. 8l+7: lanes 8 (l & 3) .. + 7, the first or the second of theirs
+  float2 cs[4], sn[4];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int from = (8 * l + i) & 31;
+    const float c0 = __shfl_sync(0xffffffffu, cv[0], from), c1 = __shfl_sync(0xffffffffu, cv[1], from);
+    const float s0 = __shfl_sync(0xffffffffu, sv[0], from), s1 = __shfl_sync(0xffffffffu, sv[1], from);
+    (i & 1 ? cs[i >> 1].y : cs[i >> 1].x) = l < 4 ? c0 : c1;
+    (i & 1 ? sn[i >> 1].y : sn[i >> 1].x) = l < 4 ? s0 : s1;
+  }
+
+  Factors f;
+  make_factors(p.qw, l, cs, sn, f);
+  uint4* dst = reinterpret_cast<uint4*>(p.q_out + (int64_t)t * p.q_stride) + l;
+  for (int base = q0; base < q1; base += 4 * kRUnroll) {
+    if (base > q0) load_q(base);
+#pragma unroll
+    for (int u = 0; u < kRUnroll; ++u) {
+      const int h = base + 4 * u + grp;
+      if (base + 4 * u >= q1) break;
+      norm_rotate(lo[u], hi[u], f, p.eps);
+      if (h < q1) {
+        dst[h * 16] = lo[u];
+        dst[h * 16 + 8] = hi[u];
       }
     }
-    s_kv[threadIdx.x] = off;
   }
-  for (int i = threadIdx.x; i < TPC * 64; i += kRThreads) {
-    const int tt = i >> 6, j = i & 63, t = t0 + tt;
-    if (t < p.n) {
-      const int axis = (j % 3 == 1 && j < 3 * p.sec_h) ? 1 : (j % 3 == 2 && j < 3 * p.sec_w) ? 2 : 0;
-      // half turns: an angle a is a / pi of them, reduced to [-1, 1]
-      double h = (double)p.pos[axis * p.pos_stride + t] * (double)p.inv_freq[j] *
-                 0.31830988618379067154;
-      h -= 2.0 * rint(0.5 * h);
-      float sn, cs;
-      sincospif((float)h, &sn, &cs);
-      s_cos[tt][j] = cs;
-      s_sin[tt][j] = sn;
+  make_factors(p.kw, l, cs, sn, f);
+  const uint32_t pg = (uint32_t)slot / (uint32_t)p.page_tokens;
+  const int64_t kv = ((int64_t)pg * p.Hkv * p.page_tokens +
+                      ((uint32_t)slot - pg * (uint32_t)p.page_tokens)) * kRD;
+  for (int base = k0; base < k1; base += 4 * kRUnroll) {
+#pragma unroll
+    for (int u = 0; u < kRUnroll; ++u) {
+      const int h = p.Hq + min(base + 4 * u + grp, 2 * p.Hkv - 1);
+      lo[u] = __ldcs(src + h * 16);
+      hi[u] = __ldcs(src + h * 16 + 8);
     }
-  }
-  __syncthreads();
-
-  const int l = threadIdx.x & 7, row0 = threadIdx.x >> 3;
-  const uint4 qw0 = reinterpret_cast<const uint4*>(p.qw)[l];
-  const uint4 qw1 = reinterpret_cast<const uint4*>(p.qw)[8 + l];
-  const uint4 kw0 = reinterpret_cast<const uint4*>(p.kw)[l];
-  const uint4 kw1 = reinterpret_cast<const uint4*>(p.kw)[8 + l];
-  const int rows = TPC * H;
-  // the loop runs by whole warps (4 rows each): the shuffles stay converged
-  for (int base = 0; base < rows; base += kRRows) {
-    const int r = base + row0;
-    const int tt = r / H, h = r - tt * H;
-    const int64_t kv = r < rows ? s_kv[min(tt, TPC - 1)] : -1;
-    const bool live = kv >= 0;
-    uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
-    if (live) {
-      const uint4* src = reinterpret_cast<const uint4*>(p.qkv + (int64_t)(t0 + tt) * p.qkv_stride +
-                                                        (int64_t)h * kRD);
-      lo = src[l];
-      hi = src[8 + l];
-    }
-    const bool is_v = h >= p.Hq + p.Hkv;
-    float a[8], b[8];
-    unpack8(lo, a);
-    unpack8(hi, b);
-    float ss = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) ss = fmaf(a[i], a[i], fmaf(b[i], b[i], ss));
-    ss += __shfl_xor_sync(0xffffffffu, ss, 1);
-    ss += __shfl_xor_sync(0xffffffffu, ss, 2);
-    ss += __shfl_xor_sync(0xffffffffu, ss, 4);
-    if (!live) continue;
-    if (!is_v) {
-      const bool is_q = h < p.Hq;
-      const float rs = 1.0f / sqrtf(ss * (1.0f / kRD) + p.eps);
-      float wa[8], wb[8];
-      unpack8(is_q ? qw0 : kw0, wa);
-      unpack8(is_q ? qw1 : kw1, wb);
-      float oa[8], ob[8];
-#pragma unroll
-      for (int i = 0; i < 8; i += 4) {
-        const float4 c = *reinterpret_cast<const float4*>(&s_cos[tt][l * 8 + i]);
-        const float4 s = *reinterpret_cast<const float4*>(&s_sin[tt][l * 8 + i]);
-        const float cc[4] = {c.x, c.y, c.z, c.w}, sn[4] = {s.x, s.y, s.z, s.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float na = a[i + e] * rs * wa[i + e], nb = b[i + e] * rs * wb[i + e];
-          oa[i + e] = fmaf(na, cc[e], -nb * sn[e]);
-          ob[i + e] = fmaf(nb, cc[e], na * sn[e]);
+    for (int u = 0; u < kRUnroll; ++u) {
+      const int h = base + 4 * u + grp;
+      if (base + 4 * u >= k1) break;
+      if (base + 4 * u < p.Hkv) {  // a key row among the four
+        uint4 a = lo[u], b = hi[u];
+        norm_rotate(a, b, f, p.eps);
+        if (h < p.Hkv) {
+          lo[u] = a;
+          hi[u] = b;
         }
       }
-      lo = pack8(oa);
-      hi = pack8(ob);
+      if (h < k1) {
+        const bool is_v = h >= p.Hkv;
+        uint4* row = reinterpret_cast<uint4*>((is_v ? p.v_pages : p.k_pages) + kv +
+                                              (int64_t)(is_v ? h - p.Hkv : h) * p.page_tokens * kRD);
+        row[l] = lo[u];
+        row[8 + l] = hi[u];
+      }
     }
-    __nv_bfloat16* dst;
-    if (h < p.Hq)
-      dst = p.q_out + (int64_t)(t0 + tt) * p.q_stride + (int64_t)h * kRD;
-    else if (!is_v)
-      dst = p.k_pages + kv + (int64_t)(h - p.Hq) * p.page_tokens * kRD;
-    else
-      dst = p.v_pages + kv + (int64_t)(h - p.Hq - p.Hkv) * p.page_tokens * kRD;
-    reinterpret_cast<uint4*>(dst)[l] = lo;
-    reinterpret_cast<uint4*>(dst)[8 + l] = hi;
   }
 }
 
@@ -199,15 +249,15 @@ extern "C" int q3_qkv_norm_rope_ragged(const void* qkv, int64_t qkv_stride, cons
                  aligned(positions, 8) && aligned(inv_freq, 4) && aligned(slots, 8) &&
                  aligned(q_out, 16) && aligned(k_pages, 16) && aligned(v_pages, 16),
              "q3_qkv_norm_rope_ragged: misaligned pointer");
+  // heads of a token split over warps while that still fills idle SMs
+  int parts = 1;
+  while (parts < 8 && n_tokens * parts < (int64_t)num_sms() * kRWarps && parts * 4 < Hq) parts *= 2;
   RaggedRopeParams p{(const __nv_bfloat16*)qkv, qkv_stride, (const __nv_bfloat16*)q_norm_w,
                      (const __nv_bfloat16*)k_norm_w, positions, pos_axis_stride, inv_freq, slots,
                      (__nv_bfloat16*)q_out, q_stride, (__nv_bfloat16*)k_pages,
-                     (__nv_bfloat16*)v_pages, num_pages * page_tokens, (int)n_tokens, Hq, Hkv,
-                     page_tokens, sec_h, sec_w, eps, device_error_word()};
-  cudaStream_t st = (cudaStream_t)stream;
-  if (n_tokens <= 4 * (int64_t)num_sms())
-    return launch_ex(qkv_norm_rope_ragged_kernel<1>, dim3((unsigned)n_tokens), dim3(kRThreads), 0,
-                     st, 1, p);
-  return launch_ex(qkv_norm_rope_ragged_kernel<4>, dim3((unsigned)((n_tokens + 3) / 4)),
-                   dim3(kRThreads), 0, st, 1, p);
+                     (__nv_bfloat16*)v_pages, num_pages * page_tokens, (int)n_tokens, parts, Hq,
+                     Hkv, page_tokens, sec_h, sec_w, eps, device_error_word()};
+  const int64_t ctas = (n_tokens * parts + kRWarps - 1) / kRWarps;
+  return launch_ex(qkv_norm_rope_ragged_kernel, dim3((unsigned)ctas), dim3(kRWarps * 32), 0,
+                   (cudaStream_t)stream, 1, p);
 }

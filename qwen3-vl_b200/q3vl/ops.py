@@ -1145,7 +1145,7 @@ def qkv_norm_rope_ragged(qkv: torch.Tensor, q_norm_w: torch.Tensor, k_norm_w: to
     qkv bf16 [n, (Hq + 2 Hkv) * 128]; positions int64 [n] (text) or [3, n]
     (time, height, width, interleaved by mrope_section); inv_freq f32 [64];
     slots int64 [n] (RaggedPlan.slots; distinct, or -1 for a padding token, of
-    which nothing is read or written).  Returns q [n, Hq, 128].  Computed in
+    which nothing is written).  Returns q [n, Hq, 128].  Computed in
     fp32 and rounded once, without the bf16 tables and rounding points of
     qkv_norm_rope, so the last bit of a value may differ from it."""
     name = "qkv_norm_rope_ragged"

@@ -123,7 +123,8 @@ INV = 1.0 / (5e6 ** (torch.arange(0, 128, 2, dtype=torch.float32) / 128))
 
 @pytest.mark.parametrize("n,Hq,Hkv,axes,page,pad", [
     (1, 32, 8, 1, 256, 0), (8, 4, 1, 3, 64, 0), (3, 1, 1, 1, 64, 1), (129, 5, 1, 3, 192, 19),
-    (700, 32, 8, 3, 256, 3), (1037, 6, 2, 3, 64, 0), (2, 40, 8, 3, 64, 2)])
+    (700, 32, 8, 3, 256, 3), (1037, 6, 2, 3, 64, 0), (2, 40, 8, 3, 64, 2),
+    (5, 128, 64, 1, 64, 0), (3000, 2, 1, 3, 64, 7)])
 def test_norm_rope_slots(n, Hq, Hkv, axes, page, pad):
     width = (Hq + 2 * Hkv) * 128
     pages = -(-n // page) + 1
