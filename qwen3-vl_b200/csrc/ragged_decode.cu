@@ -23,9 +23,8 @@
 // last-arriving-CTA join that would save it was slower in attn_decode.cu, and
 // its counters would tie the workspace to one stream.
 //
-// A producer warp streams K and V tiles by TMA into a ring of 32 KB stages;
-// eight consumer warps in two groups take alternate tiles, 16 positions per
-// warp: S = Q K^T by mma.sync with the pair's query heads as the rows (8, or 16
+// A producer warp streams K and V tiles by TMA into a ring of 32 KB stages; four
+// consumer warps take 16 positions of each: S = Q K^T by mma.sync with the pair's query heads as the rows (8, or 16
 // when Hq / Hkv > 8), the softmax above per row, O += P V with P rounded to
 // bf16 (2^-9 relative and independent per key, below the bf16 rounding of the
 // output; the sum l takes the unrounded p).
@@ -40,17 +39,15 @@ constexpr int kD = 128;
 constexpr int kTile = 64;                     // positions per stage
 constexpr int kHalf = kTile * 128;            // one 64-dim box of a tile (8 KB)
 constexpr int kStage = 4 * kHalf;             // K lo/hi + V lo/hi (32 KB)
-constexpr int kGroupWarps = 4;                // consumer warps that share a tile
-constexpr int kConsumers = 2 * kGroupWarps;
+constexpr int kConsumers = 4;                 // consumer warps, 16 positions of a tile each
 constexpr int kThreads = (kConsumers + 1) * 32;
 constexpr int kMaxB = 65536;
 
-// WIDE: Hq / Hkv in 9..16 (both row halves of the MMA's A operand are used and
-// the merge buffer doubles, which leaves room for one stage less)
+// WIDE: Hq / Hkv in 9..16 (both row halves of the MMA's A operand are used)
 template <bool WIDE>
 struct Cfg {
   static constexpr int kRows = WIDE ? 16 : 8;
-  static constexpr int kStages = WIDE ? 5 : 6;
+  static constexpr int kStages = 6;
   static constexpr int kOffMerge = kStages * kStage;
   static constexpr int kMergeBytes = kConsumers * kRows * (kD + 2) * 4;
   static constexpr int kOffBar = kOffMerge + kMergeBytes;
@@ -149,71 +146,118 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::kStages; ++s) {
       mbar_init(&full[s], 1);
-      mbar_init(&empty[s], kGroupWarps);
+      mbar_init(&empty[s], kConsumers);
     }
     fence_mbar_init();
     tma_prefetch_desc(&tmK);
     tma_prefetch_desc(&tmV);
-    s_start[0] = p.B;
-    s_start[1] = s_start[2] = s_start[3] = 0;
   }
   pdl_launch();
   pdl_wait();
 
   // ---- this CTA's range of the tile list (every CTA scans the lengths) ----
-  const int per = (p.B + kThreads - 1) / kThreads;
-  const int b0 = min((int)threadIdx.x * per, p.B), b1 = min(b0 + per, p.B);
-  int64_t mine = 0;
-  bool bad = false;
-  for (int b = b0; b < b1; ++b) mine += (req_len(p, b, &bad) + kTile - 1) / kTile;
-  mine *= p.Hkv;
-  if (bad && blockIdx.x == 0) report_timeout(p.err, 0x921);
-  int64_t incl = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int64_t y = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += y;
-  }
-  if (lane == 31) s_warp[warp] = incl;
-  __syncthreads();
-  int64_t before = incl - mine, U = 0;
-#pragma unroll
-  for (int w = 0; w < kThreads / 32; ++w) {
-    if (w < warp) before += s_warp[w];
-    U += s_warp[w];
-  }
-  const int64_t nc = min64(gridDim.x, U);  // CTAs that get tiles
   const int c = blockIdx.x;
-  const int64_t u0 = c < nc ? U * c / nc : U, u1 = c < nc ? U * (c + 1) / nc : U;
-  if (u0 < u1 && before <= u0 && u0 < before + mine) {
-    int64_t at = before;
-    for (int b = b0; b < b1; ++b) {
-      const int L = req_len(p, b, &bad), nt = (L + kTile - 1) / kTile;
-      const int64_t n = (int64_t)nt * p.Hkv;
-      if (u0 < at + n) {
-        s_start[0] = b;
-        s_start[1] = (int)(u0 - at);
-        s_start[2] = nt;
-        s_start[3] = L;
-        break;
+  uint32_t nc;  // CTAs that get tiles
+  int64_t share;
+  uint32_t rest;
+  // CTA k's range [U k / nc, U (k + 1) / nc) by one division of U (in 32 bits
+  // where it fits) and remainders below 2^18
+  auto divide = [&](int64_t U) {
+    nc = (uint32_t)min64(gridDim.x, U);
+    share = nc == 0 ? 0 : U >> 32 ? U / nc : (int64_t)((uint32_t)U / nc);
+    rest = (uint32_t)(U - share * nc);
+  };
+  auto cut = [&](uint32_t k) { return share * k + (rest * k) / nc; };
+  Walk walk;
+  int64_t u0 = 0, off = 0;
+  bool bad = false;
+  walk.b = p.B;
+  walk.nt = walk.L = walk.kvh = walk.tile = 0;
+  walk.left = 0;
+  if (p.B <= 32) {
+    // one request per lane: every warp scans for itself
+    walk.L = lane < p.B ? req_len(p, lane, &bad) : 0;
+    walk.nt = (walk.L + kTile - 1) / kTile;
+    const int64_t mine = (int64_t)walk.nt * p.Hkv;
+    int64_t incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += y;
+    }
+    const int64_t U = __shfl_sync(0xffffffffu, incl, 31);
+    divide(U);
+    __syncthreads();  // barriers are initialised
+    if (c < (int)nc) {
+      u0 = cut(c);
+      walk.left = cut(c + 1) - u0;
+      const int src = __ffs(__ballot_sync(0xffffffffu, u0 < incl)) - 1;
+      off = u0 - __shfl_sync(0xffffffffu, incl - mine, src);
+      walk.L = __shfl_sync(0xffffffffu, walk.L, src);
+      walk.nt = __shfl_sync(0xffffffffu, walk.nt, src);
+      walk.b = src;
+    }
+  } else {
+    const int per = (p.B + kThreads - 1) / kThreads;
+    const int b0 = min((int)threadIdx.x * per, p.B), b1 = min(b0 + per, p.B);
+    int64_t mine = 0;
+    for (int b = b0; b < b1; ++b) mine += (req_len(p, b, &bad) + kTile - 1) / kTile;
+    mine *= p.Hkv;
+    int64_t incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += y;
+    }
+    if (lane == 31) s_warp[warp] = incl;
+    __syncthreads();
+    int64_t before = incl - mine, U = 0;
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; ++w) {
+      if (w < warp) before += s_warp[w];
+      U += s_warp[w];
+    }
+    divide(U);
+    if (c < (int)nc) {
+      u0 = cut(c);
+      walk.left = cut(c + 1) - u0;
+      if (before <= u0 && u0 < before + mine) {  // one thread's requests
+        int64_t at = before;
+        for (int b = b0; b < b1; ++b) {
+          const int L = req_len(p, b, &bad), nt = (L + kTile - 1) / kTile;
+          const int64_t n = (int64_t)nt * p.Hkv;
+          if (u0 < at + n) {
+            s_start[0] = b;
+            s_start[1] = (int)(u0 - at);
+            s_start[2] = nt;
+            s_start[3] = L;
+            break;
+          }
+          at += n;
+        }
       }
-      at += n;
+    }
+    __syncthreads();
+    if (c < (int)nc) {
+      walk.b = s_start[0];
+      off = s_start[1];
+      walk.nt = s_start[2];
+      walk.L = s_start[3];
     }
   }
-  __syncthreads();
-  Walk walk;
-  walk.b = s_start[0];
-  walk.nt = s_start[2];
-  walk.L = s_start[3];
-  walk.kvh = walk.nt > 0 ? s_start[1] / walk.nt : 0;
-  walk.tile = walk.nt > 0 ? s_start[1] - walk.kvh * walk.nt : 0;
-  walk.left = u1 - u0;
+  if (bad && c == 0) report_timeout(p.err, 0x921);
+  if (walk.left > 0) {
+    walk.kvh = (int)((uint32_t)off / (uint32_t)walk.nt);
+    walk.tile = (int)off - walk.kvh * walk.nt;
+  }
   Piece w;
 
   if (warp == kConsumers) {
     // ------------------------------ TMA producer ------------------------------
     int it = 0;
     bool ok = true;
+    int64_t u = u0;  // first tile of the piece in the list
+    if (lane == 0) p.ws_desc[c] = make_int2(-1, -1);
     while (ok && walk.next(p, w)) {
       int pages = 0;  // this lane's entry of 32 tiles' pages
       for (int t = w.t0; t < w.t1; ++t, ++it) {
@@ -249,6 +293,19 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
       }
+      if (w.t0 == 0 && w.t1 < w.nt) {
+        // the pair goes on in the next CTAs: the last is the one with its last
+        // tile, the largest k with cut(k) <= that tile
+        int last = c;
+        for (uint32_t k0 = c + 1; k0 < nc; k0 += 32) {
+          const uint32_t k = k0 + lane;
+          const int n = __popc(__ballot_sync(0xffffffffu, k < nc && cut(k) <= u + w.nt - 1));
+          last += n;
+          if (n < 32) break;
+        }
+        if (lane == 0) p.ws_desc[c] = make_int2(w.b * p.Hkv + w.kvh, last);
+      }
+      u += w.t1 - w.t0;
     }
     // the copies issued land before the CTA may exit (the consumers wait for
     // every one of them unless a wait ran out)
@@ -257,13 +314,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_wait(&full[i % C::kStages], (i / C::kStages) & 1, nullptr, 0);
   } else {
     // ------------------------------- consumers --------------------------------
-    const int group = warp / kGroupWarps, band = warp % kGroupWarps;
+    const int band = warp;
     const int g = lane >> 2, t4 = lane & 3;
     const uint32_t ring = smem_u32(smem);
     bool ok = true;
     int it = 0;
-    if (threadIdx.x == 0) p.ws_desc[c] = make_int2(-1, -1);
-    int64_t u = u0;  // first unit of the piece
     while (walk.next(p, w)) {
       // Q as the A operand: row g (and g + 8) = query head kvh * G + row
       uint32_t qf[8][WIDE ? 4 : 2];
@@ -288,7 +343,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 
       for (int t = w.t0; t < w.t1; ++t, ++it) {
-        if ((it & 1) != group) continue;
         const int s = it % C::kStages;
         if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&full[s], (it / C::kStages) & 1, p.err, 0x924));
         if (!ok) continue;
@@ -383,7 +437,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) mbar_arrive(&empty[s]);
       }
 
-      // ---- merge the eight warps; write the output or this CTA's piece ----
+      // ---- merge the warps; write the output or this CTA's piece ----
 #pragma unroll
       for (int hh = 0; hh < (WIDE ? 2 : 1); ++hh) {
         float ls = l[hh];
@@ -406,36 +460,41 @@ __global__ void __launch_bounds__(kThreads, 1)
       // a piece that ends this CTA's range but not its pair has the odd slot
       // unless it also began inside the pair
       const int slot = 2 * c + (w.t0 == 0 ? 1 : 0);
-      for (int idx = threadIdx.x; idx < p.G * kD; idx += kConsumers * 32) {
-        const int row = idx / kD, d = idx % kD;
-        float M = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < kConsumers; ++i)
-          M = fmaxf(M, sm_ml[(i * C::kRows + row) * 2]);
-        float a = 0.f, ls = 0.f;
+      for (int idx = threadIdx.x; idx < p.G * (kD / 4); idx += kConsumers * 32) {
+        const int row = idx / (kD / 4), d = idx % (kD / 4) * 4;
+        float2 ml[kConsumers];
+        float4 x[kConsumers];
 #pragma unroll
         for (int i = 0; i < kConsumers; ++i) {
-          const float mi = sm_ml[(i * C::kRows + row) * 2];
-          const float f = mi == -INFINITY ? 0.f : ex2_approx(mi - M);
-          a = fmaf(f, sm_o[(i * C::kRows + row) * kD + d], a);
-          ls = fmaf(f, sm_ml[(i * C::kRows + row) * 2 + 1], ls);
+          ml[i] = *reinterpret_cast<const float2*>(sm_ml + (i * C::kRows + row) * 2);
+          x[i] = *reinterpret_cast<const float4*>(sm_o + (i * C::kRows + row) * kD + d);
+        }
+        float M = ml[0].x;
+#pragma unroll
+        for (int i = 1; i < kConsumers; ++i) M = fmaxf(M, ml[i].x);
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+        float ls = 0.f;
+#pragma unroll
+        for (int i = 0; i < kConsumers; ++i) {
+          const float f = ml[i].x == -INFINITY ? 0.f : ex2_approx(ml[i].x - M);
+          a.x = fmaf(f, x[i].x, a.x);
+          a.y = fmaf(f, x[i].y, a.y);
+          a.z = fmaf(f, x[i].z, a.z);
+          a.w = fmaf(f, x[i].w, a.w);
+          ls = fmaf(f, ml[i].y, ls);
         }
         if (whole) {
-          p.out[w.b * p.out_stride + (int64_t)(w.kvh * p.G + row) * kD + d] = f2bf(a / ls);
+          const float inv = 1.0f / ls;
+          *reinterpret_cast<uint2*>(p.out + w.b * p.out_stride +
+                                    (int64_t)(w.kvh * p.G + row) * kD + d) =
+              make_uint2(pack_bf16x2(a.x * inv, a.y * inv), pack_bf16x2(a.z * inv, a.w * inv));
         } else {
-          p.ws_acc[((int64_t)slot * p.G + row) * kD + d] = a;
-          if (d == 0) {
-            p.ws_ml[((int64_t)slot * p.G + row) * 2] = M;
-            p.ws_ml[((int64_t)slot * p.G + row) * 2 + 1] = ls;
-          }
+          *reinterpret_cast<float4*>(p.ws_acc + ((int64_t)slot * p.G + row) * kD + d) = a;
+          if (d == 0)
+            *reinterpret_cast<float2*>(p.ws_ml + ((int64_t)slot * p.G + row) * 2) =
+                make_float2(M, ls);
         }
       }
-      if (threadIdx.x == 0 && w.t0 == 0 && !whole) {
-        // the CTA that holds the pair's last tile: the largest k with U k / nc <= it
-        const int64_t last = u + w.nt - 1;
-        p.ws_desc[c] = make_int2(w.b * p.Hkv + w.kvh, (int)(((last + 1) * nc - 1) / U));
-      }
-      u += w.t1 - w.t0;
       asm volatile("bar.sync 1, %0;" ::"n"(kConsumers * 32) : "memory");
     }
     // requests with nothing cached: zeros
@@ -452,48 +511,44 @@ __global__ void __launch_bounds__(kThreads, 1)
 constexpr int kJoinWarps = 8;
 constexpr int kMaxGrid = 512;
 __global__ void __launch_bounds__(kJoinWarps * 32) ragged_decode_join(RaggedDecodeParams p) {
-  __shared__ float s_f[kMaxGrid];
-  __shared__ float s_red[kJoinWarps][2];
+  __shared__ float2 s_ml[kJoinWarps];
   __shared__ __align__(16) float s_acc[kJoinWarps][kD];
   pdl_launch();
   pdl_wait();
   const int c = blockIdx.x, row = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int2 d = p.ws_desc[c];
   if (d.x < 0) return;
-  const int n = d.y - c + 1;  // pieces, at most the first kernel's grid (<= kMaxGrid)
-  auto piece = [&](int i) { return ((int64_t)(i == 0 ? 2 * c + 1 : 2 * (c + i)) * p.G + row); };
-  float M = -INFINITY;
-  for (int i = threadIdx.x; i < n; i += kJoinWarps * 32) {
-    const float mi = p.ws_ml[piece(i) * 2];
-    s_f[i] = mi;
-    M = fmaxf(M, mi);
-  }
-  M = warp_max(M);
-  if (lane == 0) s_red[warp][0] = M;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < kJoinWarps; ++i) M = fmaxf(M, s_red[i][0]);
+  const int n = d.y - c + 1;  // pieces, at most the first kernel's grid
+  // a warp's pieces against a running maximum, then the warps'
+  float M = -INFINITY, l = 0.f;
   float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-  float l = 0.f;
 #pragma unroll 4
   for (int i = warp; i < n; i += kJoinWarps) {
-    const float f = ex2_approx(s_f[i] - M);
-    const float4 x = *reinterpret_cast<const float4*>(p.ws_acc + piece(i) * kD + lane * 4);
-    l = fmaf(f, p.ws_ml[piece(i) * 2 + 1], l);
-    a.x = fmaf(f, x.x, a.x);
-    a.y = fmaf(f, x.y, a.y);
-    a.z = fmaf(f, x.z, a.z);
-    a.w = fmaf(f, x.w, a.w);
+    const int64_t piece = (int64_t)(i == 0 ? 2 * c + 1 : 2 * (c + i)) * p.G + row;
+    const float2 ml = *reinterpret_cast<const float2*>(p.ws_ml + piece * 2);
+    const float4 x = *reinterpret_cast<const float4*>(p.ws_acc + piece * kD + lane * 4);
+    const float m_new = fmaxf(M, ml.x);  // a piece has at least one position: finite
+    const float f0 = ex2_approx(M - m_new), f1 = ex2_approx(ml.x - m_new);
+    M = m_new;
+    l = fmaf(f1, ml.y, l * f0);
+    a.x = fmaf(f1, x.x, a.x * f0);
+    a.y = fmaf(f1, x.y, a.y * f0);
+    a.z = fmaf(f1, x.z, a.z * f0);
+    a.w = fmaf(f1, x.w, a.w * f0);
   }
   *reinterpret_cast<float4*>(&s_acc[warp][lane * 4]) = a;
-  if (lane == 0) s_red[warp][1] = l;
+  if (lane == 0) s_ml[warp] = make_float2(M, l);
   __syncthreads();
   if (threadIdx.x < kD) {
+    float Ma = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < kJoinWarps; ++i) Ma = fmaxf(Ma, s_ml[i].x);
     float x = 0.f, ls = 0.f;
 #pragma unroll
     for (int i = 0; i < kJoinWarps; ++i) {
-      x += s_acc[i][threadIdx.x];
-      ls += s_red[i][1];
+      const float f = s_ml[i].x == -INFINITY ? 0.f : ex2_approx(s_ml[i].x - Ma);
+      x = fmaf(f, s_acc[i][threadIdx.x], x);
+      ls = fmaf(f, s_ml[i].y, ls);
     }
     const int b = d.x / p.Hkv, kvh = d.x - b * p.Hkv;
     p.out[b * p.out_stride + (int64_t)(kvh * p.G + row) * kD + threadIdx.x] = f2bf(x / ls);
