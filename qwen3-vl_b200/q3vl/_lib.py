@@ -181,5 +181,12 @@ def call(name: str, *args) -> None:
     check(getattr(load(), name)(*args), name)
 
 
+_bound: dict = {}
+
+
 def raw(name: str):
-    return getattr(load(), name)
+    """The bound entry point itself (returns its status)."""
+    fn = _bound.get(name)
+    if fn is None:
+        fn = _bound[name] = getattr(load(), name)
+    return fn

@@ -1078,6 +1078,9 @@ def _ragged_pool(name: str, k_pages: torch.Tensor, v_pages: torch.Tensor):
 
 def _ragged_table(name: str, t: torch.Tensor, B: int):
     """Row stride and width of an int32 [B, width] block table."""
+    shape = t.shape
+    if t.dtype == torch.int32 and len(shape) == 2 and shape[0] == B and t.is_contiguous():
+        return shape[1], shape[1]
     if t.dtype != torch.int32:
         raise TypeError(f"{name}: block_table must be int32, got {t.dtype}")
     if t.dim() != 2 or t.shape[0] != B or (t.stride(1) != 1 and t.shape[1] > 1):
