@@ -20,7 +20,7 @@
 //
 // Bound by the tensor pipe and the softmax (4 * 128 flops per visible pair).
 // The lengths are only known on the device, so the 128-key tiles of all items,
-// plus one position per item for its fixed cost, form one list that is cut into
+// plus two places per item for its fixed cost, form one list that is cut into
 // equal ranges, one per SM; a cut within 2 tiles of an item's edge moves there (a
 // split costs about as much as a tile; with cuts moved by up to 1/16 of a range
 // the six-prompt case had 12 % more tiles on one SM than on average).  An item cut in the middle leaves fp32 pieces (O, base, sum)
@@ -59,6 +59,7 @@ constexpr float kLazyLog2 = 64.0f;
 constexpr int kMaxB = 65536;
 constexpr int kMaxGrid = 512;
 constexpr int kPieceRows = 2 * kM;
+constexpr int kItemCost = 2;              // places of the work list an item takes besides its tiles
 
 struct RaggedPrefillParams {
   __nv_bfloat16* out;
@@ -153,7 +154,9 @@ __device__ __forceinline__ void regs_inc() {
 // ---------------------------------------------------------------------------
 // The work list.  Request b has n = ceil(q_len / 2T) items per K/V head; item i
 // has tiles(i) = max(1, ceil(x / 128)) key tiles, x = the positions its last
-// query sees.  Every item takes tiles(i) + 1 places in the list.
+// query sees.  Every item takes tiles(i) + kItemCost places in the list (loading
+// its queries, an epilogue and a first tile that moves the base cost about 5000
+// cycles; a tile takes about 3200).
 // ---------------------------------------------------------------------------
 struct Req {
   int q0, q_len, L, past;  // first packed row, queries, cached positions, L - q_len
@@ -194,7 +197,7 @@ __device__ __forceinline__ int64_t floor_sum(int64_t n, int64_t m, int64_t a, in
 }
 // places that items [0, i) of one K/V head take
 __device__ __forceinline__ int64_t places(const RaggedPrefillParams& p, const Req& r, int i) {
-  if (!p.causal) return (int64_t)i * (n_tiles(p, r, 0) + 1);
+  if (!p.causal) return (int64_t)i * (n_tiles(p, r, 0) + kItemCost);
   const int n = n_items(p, r), S = 2 * p.T;
   const int full = min(i, n - 1);  // items whose last query is (k + 1) * 2T
   int64_t s = 0;
@@ -203,14 +206,14 @@ __device__ __forceinline__ int64_t places(const RaggedPrefillParams& p, const Re
     s = one + floor_sum(full - one, kN, S, (int64_t)r.past + (int64_t)(one + 1) * S + kN - 1);
   }
   if (i > full && n > 0) s += n_tiles(p, r, n - 1);
-  return s + i;
+  return s + (int64_t)i * kItemCost;
 }
-// A cut at place `pos` of an item of nt tiles, as a tile boundary 0..nt: place 0
-// is the item's fixed cost, and a cut within `snap` tiles of an edge moves to the
+// A cut at place `pos` of an item of nt tiles, as a tile boundary 0..nt: the first
+// places are the item's fixed cost, and a cut within `snap` tiles of an edge moves to the
 // nearer one.
 __device__ __forceinline__ int cut_tile(int64_t pos, int nt, int snap) {
-  if (pos > nt) return nt;
-  const int t = (int)max64(pos - 1, 0);
+  if (pos >= nt + kItemCost) return nt;
+  const int t = (int)max64(pos - kItemCost, 0);
   if (t < snap && 2 * t < nt) return 0;
   return nt - t < snap ? nt : t;
 }
@@ -226,7 +229,7 @@ struct Walk {
   int64_t pos, u, left;  // place inside the item, of the item, places left
   __device__ __forceinline__ bool next(const RaggedPrefillParams& p, Piece& w) {
     while (left > 0) {
-      const int64_t end = min64(pos + left, nt + 1);
+      const int64_t end = min64(pos + left, nt + kItemCost);
       w.t0 = cut_tile(pos, nt, snap);
       w.t1 = cut_tile(end, nt, snap);
       w.r = r;
@@ -236,8 +239,8 @@ struct Walk {
       w.nt = nt;
       w.u = u;
       left -= end - pos;
-      if (end == nt + 1) {
-        u += nt + 1;
+      if (end == nt + kItemCost) {
+        u += nt + kItemCost;
         pos = 0;
         if (++item == n) {
           item = 0;
@@ -408,7 +411,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int k0 = c + 1; k0 < nc; k0 += 32) {
             const int k = k0 + lane;
             const int64_t pos = U * k / nc - w.u;
-            const bool in = k < nc && pos <= w.nt && cut_tile(pos, w.nt, walk.snap) < w.nt;
+            const bool in = k < nc && cut_tile(pos, w.nt, walk.snap) < w.nt;
             const int n = __popc(__ballot_sync(0xffffffffu, in));
             last += n;
             if (n < 32) break;

@@ -187,6 +187,9 @@ def floor_sum(n, m, a, b):
     return s
 
 
+ITEM_COST = 2          # places of the list an item takes besides its tiles
+
+
 def n_tiles(T, q, L, i, causal=True):
     x = L - q + min(q, (i + 1) * 2 * T) if causal else L
     return 1 if x <= 128 else -(-x // 128)
@@ -195,7 +198,7 @@ def n_tiles(T, q, L, i, causal=True):
 def places(T, q, L, i, causal=True):
     """Places of items [0, i), as the kernel sums them in closed form."""
     if not causal:
-        return i * (n_tiles(T, q, L, 0, False) + 1)
+        return i * (n_tiles(T, q, L, 0, False) + ITEM_COST)
     n, S, past = -(-q // (2 * T)), 2 * T, L - q
     full, s = min(i, n - 1), 0
     if full > 0:
@@ -203,7 +206,7 @@ def places(T, q, L, i, causal=True):
         s = one + floor_sum(full - one, 128, S, past + (one + 1) * S + 127)
     if i > full and n > 0:
         s += n_tiles(T, q, L, n - 1)
-    return s + i
+    return s + i * ITEM_COST
 
 
 def test_places_in_closed_form():
@@ -215,13 +218,13 @@ def test_places_in_closed_form():
         L = max(0, q + past)
         n = -(-q // (2 * T))
         for i in range(n + 1):
-            assert places(T, q, L, i) == sum(n_tiles(T, q, L, k) + 1 for k in range(i))
+            assert places(T, q, L, i) == sum(n_tiles(T, q, L, k) + ITEM_COST for k in range(i))
 
 
 def cut_tile(pos, nt, snap):
-    if pos > nt:
+    if pos >= nt + ITEM_COST:
         return nt
-    t = max(pos - 1, 0)
+    t = max(pos - ITEM_COST, 0)
     if t < snap and 2 * t < nt:
         return 0
     return nt if nt - t < snap else t
@@ -235,19 +238,19 @@ def prefill_ranges(qs, Ls, T, Hkv, grid, causal=True):
             for i in range(-(-q // (2 * T))):
                 nt = n_tiles(T, q, L, i, causal)
                 items.append(((b, h, i), nt, u))
-                u += nt + 1
+                u += nt + ITEM_COST
     U, nc = u, min(grid, u)
     snap = min(U // nc // 8, 2) if nc else 0
     pieces, desc, at = [], {}, 0
     for c in range(nc):
         u0, u1 = U * c // nc, U * (c + 1) // nc
-        while items[at][2] + items[at][1] + 1 <= u0:
+        while items[at][2] + items[at][1] + ITEM_COST <= u0:
             at += 1
         k = at
         while k < len(items) and items[k][2] < u1:
             key, nt, base = items[k]
             t0 = cut_tile(max(u0 - base, 0), nt, snap)
-            t1 = cut_tile(min(u1 - base, nt + 1), nt, snap)
+            t1 = cut_tile(min(u1 - base, nt + ITEM_COST), nt, snap)
             if t0 < t1:
                 pieces.append((c, key, t0, t1, nt))
                 if t0 == 0 and t1 < nt:
@@ -257,7 +260,7 @@ def prefill_ranges(qs, Ls, T, Hkv, grid, causal=True):
                         for lane in range(32):
                             y = x + lane
                             pos = U * y // nc - base
-                            n += y < nc and pos <= nt and cut_tile(pos, nt, snap) < nt
+                            n += y < nc and cut_tile(pos, nt, snap) < nt
                         last += n
                         if n < 32:
                             break
