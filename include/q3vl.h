@@ -162,7 +162,9 @@ Q3_API int q3_attn_decode_paged(const void* q, const void* k_pages, const void* 
  * ceil((past + q) / page_tokens) - ceil(past / page_tokens) pages from the list,
  * in request order, written to its row of block_table behind the pages of its
  * past positions (entries there are taken as empty); with NULL the table
- * already maps every position.  Outputs: cu_q int32 [B + 1] first packed token
+ * already maps every position.  free_start (int32 [1] on the device, or NULL: 0)
+ * is the list's first entry that no earlier call has taken; it is only read (a
+ * step adds counts[1] to it).  Outputs: cu_q int32 [B + 1] first packed token
  * of each request; kv_lens int32 [B] = past + q; counts int32 [2] = {packed
  * tokens, pages taken}; for each of n_tokens packed rows requests int32,
  * positions int64 (cache position + rope_delta[b], rope_delta int64 [B] or
@@ -175,7 +177,7 @@ Q3_API int q3_attn_decode_paged(const void* q, const void* k_pages, const void* 
 Q3_API int q3_ragged_plan(const int32_t* q_lens, const int32_t* past_lens, int B,
                           int32_t* block_table, int64_t table_stride, int table_width,
                           int page_tokens, const int32_t* free_pages, int n_free,
-                          const int64_t* rope_delta, int64_t n_tokens, int32_t* cu_q,
+                          const int32_t* free_start, const int64_t* rope_delta, int64_t n_tokens, int32_t* cu_q,
                           int32_t* kv_lens, int32_t* requests, int64_t* positions, int64_t* slots,
                           int32_t* counts, q3_stream_t stream);
 

@@ -595,6 +595,7 @@ extern "C" int q3_attn_decode_ragged(const void* q, int64_t q_stride, const void
              "q3_attn_decode_ragged: page_tokens=%d must be a positive multiple of %d",
              page_tokens, kTile);
   Q3_REQUIRE(table_width > 0 && table_stride >= table_width && num_pages > 0 &&
+                 num_pages < (1ll << 31) &&
                  (int64_t)table_width * page_tokens < (1ll << 31),
              "q3_attn_decode_ragged: table width %d, stride %lld, %lld pages", table_width,
              (long long)table_stride, (long long)num_pages);

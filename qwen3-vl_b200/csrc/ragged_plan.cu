@@ -31,6 +31,7 @@ struct PlanParams {
   int32_t* table;
   int64_t table_stride;
   const int32_t* free_pages;
+  const int32_t* free_start;
   const int64_t* delta;
   int32_t* cu_q;
   int32_t* kv_lens;
@@ -83,7 +84,8 @@ __global__ void __launch_bounds__(kPlanThreads) ragged_plan_kernel(PlanParams p)
   extern __shared__ int32_t sm[];
   int32_t* cu = sm;                // [B + 1]
   int32_t* first = sm + p.B + 1;   // [B + 1] pages taken before request b
-  pdl_launch();
+  // No early launch of the next kernel: attn_decode_paged reads its table before
+  // its own wait, and must not start before this one has written it.
   pdl_wait();
   const int tid = threadIdx.x;
   const int per = (p.B + kPlanThreads - 1) / kPlanThreads;
@@ -129,6 +131,10 @@ __global__ void __launch_bounds__(kPlanThreads) ragged_plan_kernel(PlanParams p)
   const int32_t n_new = (int32_t)min64(taken, INT32_MAX);
   if (tid == 0) first[p.B] = n_new;
   __syncthreads();
+  // the list's entries not taken by earlier calls
+  const int start = p.free_start ? min(max(*p.free_start, 0), p.n_free) : 0;
+  const int32_t* fresh = p.free_pages + start;
+  const int n_free = p.n_free - start;
 
   const int gtid = blockIdx.x * kPlanThreads + tid, gsize = gridDim.x * kPlanThreads;
   for (int b = gtid; b <= p.B; b += gsize) {
@@ -140,12 +146,12 @@ __global__ void __launch_bounds__(kPlanThreads) ragged_plan_kernel(PlanParams p)
   if (gtid == 0) {
     p.counts[0] = cu[p.B];
     p.counts[1] = n_new;
-    if (n_new > p.n_free) report_timeout(p.err, 0x903);
+    if (n_new > n_free) report_timeout(p.err, 0x903);
   }
   for (int i = gtid; i < n_new; i += gsize) {
     const int b = find_last(first, p.B, i);
     const int j = pages(max(p.past[b], 0)) + i - first[b];
-    p.table[b * p.table_stride + j] = i < p.n_free ? p.free_pages[i] : -1;
+    p.table[b * p.table_stride + j] = i < n_free ? fresh[i] : -1;
   }
   const int32_t n_live = cu[p.B];
   for (int64_t t = gtid; t < p.n_tokens; t += gsize) {
@@ -163,7 +169,7 @@ __global__ void __launch_bounds__(kPlanThreads) ragged_plan_kernel(PlanParams p)
           pg = p.table[req * p.table_stride + j];
         } else {
           const int64_t i = (int64_t)first[req] + j - have;
-          if (i < p.n_free) pg = p.free_pages[i];
+          if (i < n_free) pg = fresh[i];
         }
         if (pg >= 0) slot = (int64_t)pg * P + (pos - (int64_t)j * P);
         else report_timeout(p.err, 0x903);
@@ -184,7 +190,7 @@ __global__ void __launch_bounds__(kPlanThreads) ragged_plan_kernel(PlanParams p)
 extern "C" int q3_ragged_plan(const int32_t* q_lens, const int32_t* past_lens, int B,
                               int32_t* block_table, int64_t table_stride, int table_width,
                               int page_tokens, const int32_t* free_pages, int n_free,
-                              const int64_t* rope_delta, int64_t n_tokens, int32_t* cu_q,
+                              const int32_t* free_start, const int64_t* rope_delta, int64_t n_tokens, int32_t* cu_q,
                               int32_t* kv_lens, int32_t* requests, int64_t* positions,
                               int64_t* slots, int32_t* counts, q3_stream_t stream) {
   using namespace q3;
@@ -202,9 +208,10 @@ extern "C" int q3_ragged_plan(const int32_t* q_lens, const int32_t* past_lens, i
   Q3_REQUIRE((int64_t)table_width * page_tokens < (1ll << 31),
              "q3_ragged_plan: %d pages of %d positions pass 32-bit lengths", table_width,
              page_tokens);
-  Q3_REQUIRE(n_free >= 0 && (free_pages || n_free == 0), "q3_ragged_plan: free list");
+  Q3_REQUIRE(n_free >= 0 && (free_pages || (n_free == 0 && !free_start)),
+             "q3_ragged_plan: free list");
   Q3_REQUIRE(aligned(q_lens, 4) && aligned(past_lens, 4) && aligned(block_table, 4) &&
-                 aligned(free_pages, 4) && aligned(rope_delta, 8) && aligned(cu_q, 4) &&
+                 aligned(free_pages, 4) && aligned(free_start, 4) && aligned(rope_delta, 8) && aligned(cu_q, 4) &&
                  aligned(kv_lens, 4) && aligned(requests, 4) && aligned(positions, 8) &&
                  aligned(slots, 8) && aligned(counts, 4),
              "q3_ragged_plan: misaligned pointer");
@@ -214,7 +221,8 @@ extern "C" int q3_ragged_plan(const int32_t* q_lens, const int32_t* past_lens, i
                                        cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        2 * (kPlanMaxB + 1) * (int)sizeof(int32_t)));
   const int64_t want = (max64(n_tokens, B + 1) + kPlanThreads - 1) / kPlanThreads;
-  PlanParams p{q_lens, past_lens, block_table, table_stride, free_pages, rope_delta, cu_q,
+  PlanParams p{q_lens, past_lens, block_table, table_stride, free_pages, free_start, rope_delta,
+               cu_q,
                kv_lens, requests, positions, slots, counts, n_tokens, B, table_width,
                page_tokens, n_free, device_error_word()};
   return launch_ex(ragged_plan_kernel, dim3((unsigned)min64(want, num_sms())),

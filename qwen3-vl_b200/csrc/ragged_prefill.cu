@@ -53,9 +53,9 @@ constexpr int kOffBar = kOffOut + 8 * 4096;
 constexpr int kSmem = kOffBar + 256 + 1024;
 static_assert(kSmem + 1024 <= 227 * 1024, "shared memory (1 KB for the static part)");
 constexpr uint32_t kTmemCols = 512;       // S[0] S[1] O[0] O[1], 128 columns each
-// a row's base moves when its maximum has grown by more than 2^64: P, l and O are
-// relative to the base, and bf16 and fp32 hold 2^64 times any finite V
-constexpr float kLazyLog2 = 64.0f;
+// a row's base moves when its maximum has grown by more than 2^16: P, l and O are
+// relative to the base, and fp32 holds 2^16 times V for any |V| below 2^112
+constexpr float kLazyLog2 = 16.0f;
 constexpr int kMaxB = 65536;
 constexpr int kMaxGrid = 512;
 constexpr int kPieceRows = 2 * kM;
@@ -325,6 +325,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     tmem_alloc(tmem_slot, kTmemCols);
     tmem_relinquish();
   }
+  // rows of the query tiles past the last (token, head) pair, which no copy
+  // fills: zeros, so that they never move a base
+  for (int i = p.T * p.G * 16 + threadIdx.x; i < kM * 16; i += kThreads)
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+      *reinterpret_cast<uint4*>(smem + t * kQBytes + (i & 1) * (kQBytes / 2) + (i >> 4) * 128 +
+                                ((i >> 1) & 7) * 16) = make_uint4(0, 0, 0, 0);
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   if (threadIdx.x < kM) {
     const int tk = threadIdx.x / p.G;
     // rows past the last (token, head) pair: a token past any request's end
@@ -638,7 +646,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // P = 2^(S scale - base).  The first 64 keys' exponentials are taken
         // against the old base while the tile's maximum is still being found, and
         // taken again in a tile that moves the base: an item's first, and one
-        // where the maximum has grown by 2^64.  (No branch around them: the
+        // where the maximum has grown by 2^16.  (No branch around them: the
         // compiler overlaps them with the maximum.)
         float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
         uint32_t pk[32];
@@ -652,7 +660,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float mx = fmaxf(fmaxf(mq[0], mq[1]), fmaxf(mq[2], mq[3]));
         // scale > 0, so the maximum of the scaled scores is the scaled maximum
         const float m_new = fmaxf(m_used, mx * p.scale_log2);
-        const bool move = m_new > m_used + kLazyLog2;  // -inf + 64 = -inf
+        const bool move = m_new > m_used + kLazyLog2;  // -inf + 16 = -inf
         if (__any_sync(0xffffffffu, move)) {
           const bool rescale = move && j > 0 && m_used != -INFINITY;
           const float corr = rescale ? ex2_approx(m_used - m_new) : 1.f;
@@ -866,6 +874,7 @@ extern "C" int q3_attn_prefill_ragged(const void* q, int64_t q_stride, const voi
              "q3_attn_prefill_ragged: page_tokens=%d must be a positive multiple of 64",
              page_tokens);
   Q3_REQUIRE(table_width > 0 && table_stride >= table_width && num_pages > 0 &&
+                 num_pages < (1ll << 31) &&
                  (int64_t)table_width * page_tokens < (1ll << 31) - 256,
              "q3_attn_prefill_ragged: table width %d, stride %lld, %lld pages", table_width,
              (long long)table_stride, (long long)num_pages);

@@ -230,7 +230,7 @@ extern "C" int q3_qkv_norm_rope_ragged(const void* qkv, int64_t qkv_stride, cons
   using namespace q3;
   Q3_REQUIRE(head_dim == kRD, "q3_qkv_norm_rope_ragged: head_dim must be 128 (got %d)", head_dim);
   Q3_REQUIRE(n_tokens >= 0 && n_tokens < (1ll << 31) && Hq > 0 && Hkv > 0 && Hq <= 1024 &&
-                 Hkv <= 1024 && page_tokens > 0 && num_pages > 0,
+                 Hkv <= 1024 && page_tokens > 0 && num_pages > 0 && num_pages < (1ll << 31),
              "q3_qkv_norm_rope_ragged: bad shape n=%lld Hq=%d Hkv=%d", (long long)n_tokens, Hq,
              Hkv);
   Q3_REQUIRE(num_pages * page_tokens < (1ll << 31),

@@ -73,7 +73,7 @@ SIGNATURES: dict[str, tuple] = {
     "q3_kv_pages_write": (I32, [P, P, P, P, I32, I32, I32, I32, P, I64, I32, I32, I64, P, P]),
     "q3_attn_decode_paged": (I32, [P, P, P, P, I32, I32, I32, I32, I64, P, P, I64, I32, I32, F32,
                                    P, SZ, P]),
-    "q3_ragged_plan": (I32, [P, P, I32, P, I64, I32, I32, P, I32, P, I64, P, P, P, P, P, P, P]),
+    "q3_ragged_plan": (I32, [P, P, I32, P, I64, I32, I32, P, I32, P, P, I64, P, P, P, P, P, P, P]),
     "q3_qkv_norm_rope_ragged": (I32, [P, I64, P, P, P, I64, P, P, P, I64, P, P, I64, I32, I32, I32,
                                       I32, I64, I32, I32, F32, P]),
     "q3_attn_decode_ragged_workspace_bytes": (SZ, [I32, I32]),

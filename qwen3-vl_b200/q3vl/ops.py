@@ -1101,20 +1101,21 @@ def _ragged_ints(name: str, what: str, t: torch.Tensor, dtype, n: int) -> int:
 
 def ragged_plan(q_lens: torch.Tensor, past_lens: torch.Tensor, block_table: torch.Tensor, *,
                 page_tokens: int, n_tokens: int, free_pages: torch.Tensor = None,
-                rope_delta: torch.Tensor = None) -> RaggedPlan:
+                free_start: torch.Tensor = None, rope_delta: torch.Tensor = None) -> RaggedPlan:
     """Block tables, slot map and positions of a step, from the requests' lengths.
 
     q_lens, past_lens int32 [B] on the device: new tokens and cached positions
     of each request.  block_table int32 [B, width] is filled in place with pages
-    of free_pages (int32 [n], in order) for the positions that need new ones;
-    without free_pages it must map every position already
+    of free_pages (int32 [n], in order, from entry free_start on: int32 [1] on
+    the device, to which a step adds counts[1:]) for the positions that need new
+    ones; without free_pages it must map every position already
     (KVPagePool.device_table).  n_tokens is the packed buffer's size: rows behind
     the last request get request -1, position 0 and slot -1.  rope_delta int64
     [B] or [B, 1] (rope_index) shifts the rotary positions.  Nothing is read
     back: counts[1] pages of the list were taken (more than its length, and
     0x903 in the device error word, when it was short)."""
     name = "ragged_plan"
-    dev = _ragged_device(name, q_lens, past_lens, block_table, free_pages, rope_delta)
+    dev = _ragged_device(name, q_lens, past_lens, block_table, free_pages, free_start, rope_delta)
     B, n = q_lens.numel(), int(n_tokens)
     if n < 0:
         raise ValueError(f"{name}: n_tokens={n}")
@@ -1128,9 +1129,11 @@ def ragged_plan(q_lens: torch.Tensor, past_lens: torch.Tensor, block_table: torc
     at_cu = at + 20 * n
     _ragged_call("q3_ragged_plan", dev, _ragged_ints(name, "q_lens", q_lens, torch.int32, B),
                  _ragged_ints(name, "past_lens", past_lens, torch.int32, B), B,
-                 block_table.data_ptr(), stride, width, page_tokens,
+                 block_table.data_ptr(), stride, width, int(page_tokens),
                  None if free_pages is None else
                  _ragged_ints(name, "free_pages", free_pages, torch.int32, n_free), n_free,
+                 None if free_start is None else
+                 _ragged_ints(name, "free_start", free_start, torch.int32, 1),
                  None if rope_delta is None else
                  _ragged_ints(name, "rope_delta", rope_delta, torch.int64, B), n, at_cu,
                  at_cu + 4 * (B + 1), at + 16 * n, at, at + 8 * n, at_cu + 4 * (2 * B + 1))
@@ -1157,6 +1160,7 @@ def qkv_norm_rope_ragged(qkv: torch.Tensor, q_norm_w: torch.Tensor, k_norm_w: to
     num_pages, heads, page_tokens, _ = _ragged_pool(name, k_pages, v_pages)
     if heads != Hkv:
         raise ValueError(f"{name}: the pool has {heads} K/V heads, Hkv is {Hkv}")
+    Hq, Hkv = int(Hq), int(Hkv)
     width = (Hq + 2 * Hkv) * HEAD_DIM
     _bf16(name, qkv, q_norm_w, k_norm_w)
     if qkv.dim() != 2 or qkv.shape[1] != width or qkv.stride(1) != 1:
@@ -1185,7 +1189,8 @@ def qkv_norm_rope_ragged(qkv: torch.Tensor, q_norm_w: torch.Tensor, k_norm_w: to
                  positions.data_ptr(), positions.stride(0) if len(pos_shape) == 2 else 0,
                  inv_freq.data_ptr(), _ragged_ints(name, "slots", slots, torch.int64, n),
                  out.data_ptr(), out_stride, k_pages.data_ptr(), v_pages.data_ptr(), n, Hq, Hkv,
-                 HEAD_DIM, page_tokens, num_pages, mrope_section[1], mrope_section[2], eps)
+                 HEAD_DIM, page_tokens, num_pages, int(mrope_section[1]), int(mrope_section[2]),
+                 float(eps))
     return out
 
 
@@ -1213,7 +1218,7 @@ def attn_decode_ragged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Te
                  v_pages.data_ptr(), out.data_ptr(), out_stride, B, Hq, Hkv, D,
                  block_table.data_ptr(), table_stride, width, page_tokens, num_pages,
                  _ragged_ints(name, "kv_lens", kv_lens, torch.int32, B),
-                 HEAD_DIM ** -0.5 if scale is None else scale, ws.data_ptr(), nbytes)
+                 HEAD_DIM ** -0.5 if scale is None else float(scale), ws.data_ptr(), nbytes)
     return out
 
 
@@ -1246,7 +1251,7 @@ def attn_prefill_ragged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.T
                  block_table.data_ptr(), table_stride, width, page_tokens, num_pages,
                  _ragged_ints(name, "cu_q", cu_q, torch.int32, B + 1),
                  _ragged_ints(name, "kv_lens", kv_lens, torch.int32, B), 1 if causal else 0,
-                 HEAD_DIM ** -0.5 if scale is None else scale, ws.data_ptr(), nbytes)
+                 HEAD_DIM ** -0.5 if scale is None else float(scale), ws.data_ptr(), nbytes)
     return out
 
 

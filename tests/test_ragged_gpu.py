@@ -414,3 +414,129 @@ def test_prefill_in_a_graph_with_new_lengths():
         want, tol = ora.attention(q[:m], k, v, table, lens, qs)
         ora.check("replayed", out[:m], want, tol)
         assert bool((out[m:] == 3).all())
+
+
+# ------------------------------------------------------- the operators together
+def test_plan_continues_the_free_list():
+    t = i32([[4, -1, -1], [5, -1, -1]])
+    free, start = i32([9, 8, 7, 6]), i32([0])
+    past = i32([64, 60])
+    for step, taken in ((0, 2), (1, 0)):
+        p = ops.ragged_plan(i32([1, 5]), past, t, page_tokens=64, n_tokens=6, free_pages=free,
+                            free_start=start)
+        assert p.counts.tolist() == [6, taken]
+        past, start = p.kv_lens.clone(), start + p.counts[1:]
+    assert t.tolist() == [[4, 9, -1], [5, 8, -1]] and start.tolist() == [2]
+    p = ops.ragged_plan(i32([100, 100]), past, t, page_tokens=64, n_tokens=200, free_pages=free,
+                        free_start=start)
+    assert t.tolist() == [[4, 9, 7], [5, 8, 6]] and p.counts.tolist() == [200, 2]
+    ops.ragged_plan(i32([1]), i32([192]), i32([[1, 2, 3, -1]]), page_tokens=64, n_tokens=1,
+                    free_pages=free, free_start=i32([4]))
+    assert ops.device_error() == 0x903                    # the list is used up
+
+
+def test_serve_a_mixed_batch():
+    """Prompts (one with an image), then steps that mix decoding requests with a
+    new request's prompt: every step's q, cache rows and attention against the
+    64-bit forms, pages handed out on the device."""
+    Hq, Hkv, page, W = 8, 2, 64, 6
+    width = (Hq + 2 * Hkv) * 128
+    qw, kw = 1 + rnd(128, seed=1, std=0.2), 1 + rnd(128, seed=2, std=0.2)
+    ids = torch.randperm(40, generator=torch.Generator().manual_seed(5)).tolist()
+    kp = torch.full((40, Hkv, page, 128), math.nan, dtype=BF16, device=DEV)
+    vp = torch.full_like(kp, math.nan)
+    table = torch.full((4, W), -1, dtype=torch.int32, device=DEV)
+    free, start = i32(ids), i32([0])
+    ref_table, ref_free = [[-1] * W for _ in range(4)], list(ids)
+    past = [0, 0, 0, 0]
+    # request 1's prompt: 3 text tokens, a 4 x 6 image after merging 8 x 12, 5 text tokens
+    types = torch.tensor([[0] * 3 + [1] * 24 + [0] * 5], device=DEV)
+    mm_pos, mm_delta = ops.rope_index(types, torch.tensor([[1, 8, 12]], device=DEV))
+    delta = torch.zeros(4, dtype=torch.int64, device=DEV)
+    # (new tokens per request); decoding requests first, then prompts
+    steps = [[60, 32, 0, 0], [1, 1, 130, 0], [1, 1, 1, 0], [1, 1, 1, 7], [1, 1, 1, 1], [1, 0, 1, 1]]
+    for n_step, q_lens in enumerate(steps):
+        n = sum(q_lens) + 3                                # three padding rows
+        plan = ops.ragged_plan(i32(q_lens), i32(past), table, page_tokens=page, n_tokens=n,
+                               free_pages=free, free_start=start, rope_delta=delta)
+        want = ora.plan(q_lens, past, ref_table, page, n, ref_free, delta.tolist())
+        del ref_free[:want[5][1]]
+        for name, x in zip(plan._fields, want):
+            assert getattr(plan, name).tolist() == x, (n_step, name)
+        assert table.tolist() == ref_table
+        start += plan.counts[1:]
+        qkv = rnd(n, width, seed=100 + n_step)
+        pos = plan.positions.expand(3, n).contiguous()
+        if n_step == 0:                                    # the image's own positions
+            pos[:, 60:92] = mm_pos[:, 0]
+            delta[1] = mm_delta[0, 0]
+        q = ops.qkv_norm_rope_ragged(qkv.to(DEV), qw.to(DEV), kw.to(DEV), pos, INV.to(DEV),
+                                     plan.slots, kp, vp, Hq=Hq, Hkv=Hkv)
+        live = sum(q_lens)
+        wq, wk, wv, tq, tk = ora.norm_rope(qkv, qw, kw, pos.cpu(), INV, Hq, Hkv)
+        ora.check("q", q[:live], wq[:live], tq[:live])
+        s = plan.slots[:live].cpu()
+        ora.check("k", kp.cpu()[s // page, :, s % page], wk[:live], tk[:live])
+        assert torch.equal(vp.cpu()[s // page, :, s % page], wv[:live].to(BF16))
+        # the requests with one token through decode, the others through prefill
+        first = next((b for b, m in enumerate(q_lens) if m != 1), 4)
+        out = torch.full((n, Hq, 128), 3.0, dtype=BF16, device=DEV)
+        if first:
+            ops.attn_decode_ragged(q[:first], kp, vp, table[:first], plan.kv_lens[:first],
+                                   out=out[:first])
+        ops.attn_prefill_ragged(q, kp, vp, table[first:], plan.cu_q[first:], plan.kv_lens[first:],
+                                out=out)
+        total = [a + b for a, b in zip(q_lens, past)]
+        wo, to = ora.attention(q[:live].cpu(), kp.cpu(), vp.cpu(), ref_table,
+                               [x if m else 0 for x, m in zip(total, q_lens)], q_lens)
+        ora.check(f"step {n_step}", out[:live], wo, to)
+        assert bool((out[live:] == 3).all())
+        past = total
+    assert past == [65, 36, 134, 9]
+
+
+def test_decode_steps_in_one_graph_grow_their_tables():
+    """plan -> norm + rotary + slots -> attention -> lengths + 1, captured once
+    and replayed across page borders."""
+    B, Hq, Hkv, page, W = 3, 4, 1, 64, 5
+    width = (Hq + 2 * Hkv) * 128
+    qw, kw = (1 + rnd(128, seed=1, std=0.2)).to(DEV), (1 + rnd(128, seed=2, std=0.2)).to(DEV)
+    kp = rnd(24, Hkv, page, 128, seed=3).to(DEV)
+    vp = rnd(24, Hkv, page, 128, seed=4).to(DEV)
+    past0 = [62, 128, 1]
+    table = i32([[3, -1, -1, -1, -1], [5, 6, -1, -1, -1], [7, -1, -1, -1, -1]])
+    free = [20, 21, 22, 23, 0, 1, 2, 9]
+    ones, past, start, dfree = i32([1] * B), i32(past0), i32([0]), i32(free)
+    x, inv = torch.zeros(B, width, dtype=BF16, device=DEV), INV.to(DEV)
+
+    def step():
+        p = ops.ragged_plan(ones, past, table, page_tokens=page, n_tokens=B, free_pages=dfree,
+                            free_start=start)
+        q = ops.qkv_norm_rope_ragged(x, qw, kw, p.positions, inv, p.slots, kp, vp, Hq=Hq, Hkv=Hkv)
+        o = ops.attn_decode_ragged(q, kp, vp, table, p.kv_lens)
+        past.copy_(p.kv_lens)
+        start.add_(p.counts[1:])
+        return q, o
+    keep = [t.clone() for t in (past, start, table, kp, vp)]
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.synchronize()
+    for t, k in zip((past, start, table, kp, vp), keep):
+        t.copy_(k)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        q, o = step()
+    ref = table.tolist()
+    left, lens = list(free), list(past0)
+    for i in range(140):
+        x.copy_(rnd(B, width, seed=1000 + i))
+        g.replay()
+        *_, counts = ora.plan([1] * B, lens, ref, page, B, left)
+        del left[:counts[1]]
+        lens = [n + 1 for n in lens]
+        if i % 35 == 0 or i == 139:
+            assert past.tolist() == lens and table.tolist() == ref
+            wo, to = ora.attention(q.cpu(), kp.cpu(), vp.cpu(), ref, lens, [1] * B)
+            ora.check(f"replay {i}", o, wo, to)
+    assert left == free[int(start):]

@@ -23,7 +23,7 @@ def refused(name, args, text, status=_lib.Q3_ERR_INVALID):
 
 def plan_args(**kw):
     a = dict(q=ONE, past=ONE, B=4, table=ONE, stride=8, width=8, page=64, free=ONE, n_free=3,
-             delta=None, n=16, cu=ONE, kv=ONE, req=ONE, pos=ONE, slots=ONE, counts=ONE, s=None)
+             start=None, delta=None, n=16, cu=ONE, kv=ONE, req=ONE, pos=ONE, slots=ONE, counts=ONE, s=None)
     a.update(kw)
     return list(a.values())
 
@@ -33,7 +33,7 @@ def plan_args(**kw):
     (dict(B=-1), b"B=-1"), (dict(B=8193), b"8192"), (dict(n=-1), b"n_tokens"),
     (dict(n=1 << 31), b"n_tokens"), (dict(page=0), b"page_tokens"), (dict(page=96), b"page_tokens"),
     (dict(width=0), b"width"), (dict(stride=7), b"stride"), (dict(width=1 << 25, stride=1 << 25), b"32-bit"),
-    (dict(free=None), b"free list"), (dict(n_free=-1), b"free list"), (dict(pos=ctypes.c_void_p(20)), b"misaligned")])
+    (dict(free=None), b"free list"), (dict(free=None, n_free=0, start=ONE), b"free list"), (dict(n_free=-1), b"free list"), (dict(pos=ctypes.c_void_p(20)), b"misaligned")])
 def test_plan_refusals(kw, text):
     refused("q3_ragged_plan", plan_args(**kw), text)
 
