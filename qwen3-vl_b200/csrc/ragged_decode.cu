@@ -24,10 +24,16 @@
 // its counters would tie the workspace to one stream.
 //
 // A producer warp streams K and V tiles by TMA into a ring of 32 KB stages; four
-// consumer warps take 16 positions of each: S = Q K^T by mma.sync with the pair's query heads as the rows (8, or 16
-// when Hq / Hkv > 8), the softmax above per row, O += P V with P rounded to
-// bf16 (2^-9 relative and independent per key, below the bf16 rounding of the
+// consumer warps take 16 positions of each: S = Q K^T by mma.sync with the pair's
+// query heads as the rows (8, or 16 when Hq / Hkv > 8), the softmax above per
+// row, O += P V with P rounded to bf16 (at most 2^-8 of each p and independent
+// per key, which an average over keys shrinks below the bf16 rounding of the
 // output; the sum l takes the unrounded p).
+// Measured on B200: 32 requests of 257 to 32768 positions, 32/8 heads, 885 MB:
+// 140 us, 6.3 TB/s (0.98 of a copy; with eight consumer warps 149, their merge
+// and registers cost more than they gave); 8 requests in a 2048 bucket 10.2 us;
+// one request of 700 positions, 4/1 heads, 5.6 us, about half of it the chain
+// lengths -> table -> first tile and the join.
 #include <math.h>
 
 #include "common.cuh"
@@ -87,7 +93,6 @@ __device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
 __device__ __forceinline__ uint32_t kv_at(int r, int c) {
   return (c >> 3) * kHalf + r * 128 + (((c & 7) ^ (r & 7)) << 4);
 }
-
 
 // Length of request b, inside what its table row can hold.
 __device__ __forceinline__ int req_len(const RaggedDecodeParams& p, int b, bool* bad) {
@@ -599,6 +604,9 @@ extern "C" int q3_attn_decode_ragged(const void* q, int64_t q_stride, const void
                  (int64_t)table_width * page_tokens < (1ll << 31),
              "q3_attn_decode_ragged: table width %d, stride %lld, %lld pages", table_width,
              (long long)table_stride, (long long)num_pages);
+  Q3_REQUIRE((int64_t)table_width * page_tokens / kTile * Hkv < (1ll << 31),
+             "q3_attn_decode_ragged: %d pages of %d positions and %d K/V heads pass 32-bit tiles",
+             table_width, page_tokens, Hkv);
   Q3_REQUIRE(num_pages * Hkv * page_tokens < (1ll << 31),
              "q3_attn_decode_ragged: the pool is too large for 32-bit TMA rows");
   Q3_REQUIRE(q_stride >= (int64_t)Hq * kD && out_stride >= (int64_t)Hq * kD &&

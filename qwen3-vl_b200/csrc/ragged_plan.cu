@@ -17,6 +17,10 @@
 // tokens and of the new pages by binary search, so there is one launch and no
 // grid-wide wait: a token whose page is new reads the free list, not the table
 // entry that another CTA may be writing.
+//
+// Bound by latency: one chain of loads (lengths, then table or list), scans and
+// stores.  Measured on B200 in a graph: 8 requests of one token 4.5 us, 1024
+// requests with 79718 tokens (1.6 MB written) 8.0 us.
 #include "common.cuh"
 
 namespace q3 {

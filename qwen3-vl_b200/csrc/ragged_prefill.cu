@@ -26,6 +26,9 @@
 // the six-prompt case had 12 % more tiles on one SM than on average).  An item cut in the middle leaves fp32 pieces (O, base, sum)
 // in the workspace and a second kernel joins them in CTA order: a 512-token
 // chunk on a 32k cache fills every SM (its 64 items alone would fill 64).
+// Measured on B200, 32/8 heads: that chunk 262 us (1040 TFLOP/s at the clock the
+// power cap leaves in a long run, 1.66 GHz and 61 % of the tensor pipe under
+// ncu); six prompts of 1100 to 4096 tokens 485 us (965).
 #include <math.h>
 
 #include "common.cuh"
@@ -209,8 +212,8 @@ __device__ __forceinline__ int64_t places(const RaggedPrefillParams& p, const Re
   return s + (int64_t)i * kItemCost;
 }
 // A cut at place `pos` of an item of nt tiles, as a tile boundary 0..nt: the first
-// places are the item's fixed cost, and a cut within `snap` tiles of an edge moves to the
-// nearer one.
+// places are the item's fixed cost, and a cut within `snap` tiles of an edge
+// moves to the nearer one.
 __device__ __forceinline__ int cut_tile(int64_t pos, int nt, int snap) {
   if (pos >= nt + kItemCost) return nt;
   const int t = (int)max64(pos - kItemCost, 0);

@@ -540,3 +540,110 @@ def test_decode_steps_in_one_graph_grow_their_tables():
             wo, to = ora.attention(q.cpu(), kp.cpu(), vp.cpu(), ref, lens, [1] * B)
             ora.check(f"replay {i}", o, wo, to)
     assert left == free[int(start):]
+
+
+def test_pages_past_4_gib():
+    """Rows whose byte and element offsets pass 32 bits: written by the norm +
+    rotary call, read by both attentions."""
+    Hq, Hkv, page, pages = 4, 1, 256, 1 << 17              # 8.6 GB each for K and V
+    kp = torch.empty(pages, Hkv, page, 128, dtype=BF16, device=DEV)
+    vp = torch.empty_like(kp)
+    ids = [pages - 1, 66000, 3, pages - 2]
+    n = 700
+    table = i32([ids])
+    qkv = rnd(n, (Hq + 2) * 128, seed=21)
+    qw, kw = 1 + rnd(128, seed=1, std=0.2), 1 + rnd(128, seed=2, std=0.2)
+    plan = ops.ragged_plan(i32([n]), i32([0]), table, page_tokens=page, n_tokens=n)
+    q = ops.qkv_norm_rope_ragged(qkv.to(DEV), qw.to(DEV), kw.to(DEV), plan.positions, INV.to(DEV),
+                                 plan.slots, kp, vp, Hq=Hq, Hkv=Hkv)
+    k4, v4 = kp[torch.tensor(ids, device=DEV)].cpu(), vp[torch.tensor(ids, device=DEV)].cpu()
+    _, wk, wv, _, tk = ora.norm_rope(qkv, qw, kw, torch.arange(n), INV, Hq, Hkv)
+    ora.check("k", k4[:3, 0].reshape(-1, 128)[:n], wk[:, 0], tk[:, 0])
+    assert torch.equal(v4[:3, 0].reshape(-1, 128)[:n], wv[:, 0].to(BF16))
+    want, tol = ora.attention(q.cpu(), k4, v4, [[0, 1, 2, 3]], [n], [n])
+    ora.check("prefill", ops.attn_prefill_ragged(q, kp, vp, table, plan.cu_q, plan.kv_lens), want, tol)
+    ora.check("decode", ops.attn_decode_ragged(q[-1:], kp, vp, table, plan.kv_lens), want[-1:], tol[-1:])
+
+
+def test_calls_captured_without_a_call_before():
+    """A process may capture first: nothing is set up on the stream or allocated
+    outside torch's graph pool."""
+    import os
+    import subprocess
+    import sys
+    code = """
+import sys, torch
+sys.path[:0] = ['qwen3-vl_b200', '.']
+from q3vl import ops
+from tests import ragged_oracle as ora
+k, v, table = ora.make_pool([300, 70], 2, 64, stale=0.0)
+q = torch.randn(5, 8, 128).to(torch.bfloat16)
+d = 'cuda:0'
+a = [t.to(d) for t in (q, k, v, torch.tensor(table, dtype=torch.int32))]
+cu = torch.tensor([0, 2, 5], dtype=torch.int32, device=d)
+kv = torch.tensor([300, 70], dtype=torch.int32, device=d)
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    x = ops.attn_prefill_ragged(*a, cu, kv)
+    y = ops.attn_decode_ragged(a[0][:2], *a[1:], kv)
+    p = ops.ragged_plan(kv, kv, a[3], page_tokens=64, n_tokens=370)
+g.replay()
+torch.cuda.synchronize()
+w, t = ora.attention(q, k, v, table, [300, 70], [2, 3])
+ora.check('prefill', x, w, t)
+w, t = ora.attention(q[:2], k, v, table, [300, 70], [1, 1])
+ora.check('decode', y, w, t)
+print('fine', p.cu_q.tolist())
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "fine [0, 300, 370]" in r.stdout, r.stderr[-2000:]
+
+
+def test_wrapper_refusals():
+    q, k, v, table = decode_case([100, 30], 8, 2, 64, stale=0.0)
+    a = [q.to(DEV), k.to(DEV), v.to(DEV), i32(table)]
+    kv, cu = i32([100, 30]), i32([0, 1, 2])
+
+    def bad(err, f, *args, **kw):
+        with pytest.raises(err):
+            f(*args, **kw)
+    d, pf = ops.attn_decode_ragged, ops.attn_prefill_ragged
+    bad(TypeError, d, a[0].float(), *a[1:], kv)
+    bad(TypeError, d, *a, kv.long())
+    bad(ValueError, d, *a, kv[:1])
+    bad(TypeError, d, *a[:3], a[3].long(), kv)
+    bad(ValueError, d, *a[:3], a[3][:1], kv)
+    bad(ValueError, d, a[0], a[1], a[2][:1], a[3], kv)
+    bad(ValueError, d, a[0], a[1].transpose(0, 1), a[2].transpose(0, 1), a[3], kv)
+    bad(ValueError, d, a[0][..., :64], *a[1:], kv)
+    bad(ValueError, d, a[0].transpose(1, 2).contiguous().transpose(1, 2), *a[1:], kv)
+    bad(ValueError, d, *a, kv, out=torch.empty(2, 4, 128, dtype=BF16, device=DEV))
+    bad(TypeError, d, *a, kv, out=torch.empty(2, 8, 128, device=DEV))
+    bad(RuntimeError, d, *a, kv.cpu())
+    bad(RuntimeError, d, a[0][:, :7], *a[1:], kv)           # 7 query heads over 2
+    bad(RuntimeError, d, a[0][:1].expand(2, 8, 128), *a[1:], kv)  # rows that overlap
+    bad(ValueError, pf, *a, cu[:2], kv)
+    bad(RuntimeError, pf, *a, cu, kv, scale=0.0)
+    bad(ValueError, ops.ragged_plan, kv, kv[:1], a[3], page_tokens=64, n_tokens=2)
+    bad(ValueError, ops.ragged_plan, kv, kv, a[3], page_tokens=64, n_tokens=-1)
+    bad(RuntimeError, ops.ragged_plan, kv, kv, a[3], page_tokens=100, n_tokens=2)
+    bad(ValueError, ops.ragged_plan, kv, kv, a[3], page_tokens=64, n_tokens=2,
+        rope_delta=torch.zeros(3, dtype=torch.int64, device=DEV))
+    n = 3
+    qkv, w = rnd(n, 12 * 128).to(DEV), torch.ones(128, dtype=BF16, device=DEV)
+    pos, sl = torch.arange(n, device=DEV), torch.arange(n, device=DEV)
+    f = lambda **kw: ops.qkv_norm_rope_ragged(                                  # noqa: E731
+        kw.get("qkv", qkv), w, w, kw.get("pos", pos), kw.get("inv", INV.to(DEV)), kw.get("sl", sl),
+        a[1], a[2], Hq=kw.get("Hq", 8), Hkv=kw.get("Hkv", 2), out=kw.get("out"))
+    f()
+    bad(ValueError, f, Hkv=1)
+    bad(ValueError, f, Hq=7)
+    bad(ValueError, f, pos=pos[:2])
+    bad(ValueError, f, pos=pos.expand(2, n))
+    bad(ValueError, f, pos=pos.int())
+    bad(ValueError, f, inv=INV[:32].to(DEV))
+    bad(TypeError, f, sl=sl.int())
+    bad(ValueError, f, sl=sl[:2])
+    bad(ValueError, f, out=torch.empty(n, 7, 128, dtype=BF16, device=DEV))
+    torch.cuda.synchronize()

@@ -66,7 +66,8 @@ def decode_args(**kw):
     (dict(q=None), b"null"), (dict(ws=None), b"null"), (dict(page=32), b"page_tokens"),
     (dict(width=0), b"table width"), (dict(stride=4), b"stride"), (dict(pages=0), b"pages"),
     (dict(pages=1 << 25), b"too large"), (dict(qs=1000), b"strides"), (dict(os=1028), b"strides"),
-    (dict(k=ODD), b"misaligned"), (dict(nb=100), b"workspace of 100")])
+    (dict(k=ODD), b"misaligned"), (dict(nb=100), b"workspace of 100"),
+    (dict(Hq=1024, Hkv=1024, width=1 << 22, stride=1 << 22), b"32-bit tiles")])
 def test_decode_refusals(kw, text):
     refused("q3_attn_decode_ragged", decode_args(**kw), text)
 
@@ -316,3 +317,33 @@ def test_prefill_refuses_more_than_16_heads_a_group_and_accepts_empty_calls():
             _lib.Q3_ERR_UNSUPPORTED)
     assert _lib.raw("q3_attn_prefill_ragged")(*prefill_args(B=0, q=None)) == 0
     assert _lib.raw("q3_attn_prefill_ragged")(*prefill_args(n=0, q=None)) == 0
+
+
+def test_calls_run_on_the_tensors_own_device(monkeypatch):
+    """A call whose tensors are on device 1 while device 0 is current switches to
+    device 1 and passes its current stream."""
+    seen, at = [], [0]
+
+    class Guard:
+        def __init__(self, dev):
+            self.dev = dev
+
+        def __enter__(self):
+            self.old, at[0] = at[0], self.dev
+
+        def __exit__(self, *a):
+            at[0] = self.old
+
+    def entry(*args):
+        seen.append((at[0],) + args)
+        return 0
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: at[0])
+    monkeypatch.setattr(torch.cuda, "device", Guard)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda d: 100 + d, raising=False)
+    monkeypatch.setattr(_lib, "raw", lambda name: entry)
+    ops._ragged_call("q3_x", 0, 7)
+    ops._ragged_call("q3_x", 1, 8)
+    assert seen == [(0, 7, 100), (1, 8, 101)] and at == [0]
+    monkeypatch.setattr(_lib, "raw", lambda name: lambda *a: _lib.Q3_ERR_INVALID)
+    with pytest.raises(_lib.Q3Error):
+        ops._ragged_call("q3_x", 0, 7)
