@@ -26,9 +26,9 @@
 // the six-prompt case had 12 % more tiles on one SM than on average).  An item cut in the middle leaves fp32 pieces (O, base, sum)
 // in the workspace and a second kernel joins them in CTA order: a 512-token
 // chunk on a 32k cache fills every SM (its 64 items alone would fill 64).
-// Measured on B200, 32/8 heads: that chunk 262 us (1040 TFLOP/s at the clock the
+// Measured on B200, 32/8 heads: that chunk 256 us (1065 TFLOP/s at the clock the
 // power cap leaves in a long run, 1.66 GHz and 61 % of the tensor pipe under
-// ncu); six prompts of 1100 to 4096 tokens 485 us (965).
+// ncu); six prompts of 1100 to 4096 tokens 469 us (997).
 #include <math.h>
 
 #include "common.cuh"
@@ -181,18 +181,21 @@ __device__ __forceinline__ int n_tiles(const RaggedPrefillParams& p, const Req& 
   const int x = p.causal ? r.past + min(r.q_len, (i + 1) * 2 * p.T) : r.L;
   return x <= kN ? 1 : (x + kN - 1) / kN;
 }
-// sum over i in [0, n) of floor((a i + b) / m), by Euclid's division steps
-__device__ __forceinline__ int64_t floor_sum(int64_t n, int64_t m, int64_t a, int64_t b) {
+// sum over i in [0, n) of floor((a i + b) / m), by Euclid's division steps, in
+// words of type U that hold a n + b
+template <typename U>
+__device__ __forceinline__ int64_t floor_sum(U n, U m, U a, U b) {
   int64_t s = 0;
   while (n > 0) {
-    s += (n - 1) * n / 2 * (a / m) + n * (b / m);
-    a %= m;
-    b %= m;
-    const int64_t y = a * n + b;
+    const U qa = a / m, qb = b / m;
+    s += (int64_t)(n - 1) * (int64_t)n / 2 * (int64_t)qa + (int64_t)n * (int64_t)qb;
+    a -= qa * m;
+    b -= qb * m;
+    const U y = a * n + b;
     if (y < m) break;
     n = y / m;
     b = y - n * m;
-    const int64_t t = m;
+    const U t = m;
     m = a;
     a = t;
   }
@@ -206,7 +209,11 @@ __device__ __forceinline__ int64_t places(const RaggedPrefillParams& p, const Re
   int64_t s = 0;
   if (full > 0) {
     const int one = r.past >= kN ? 0 : min(full, (kN - r.past) / S);  // those with one tile
-    s = one + floor_sum(full - one, kN, S, (int64_t)r.past + (int64_t)(one + 1) * S + kN - 1);
+    const int64_t n1 = full - one, b1 = (int64_t)r.past + (int64_t)(one + 1) * S + kN - 1;
+    // 32-bit divisions where S n + b fits (prompts of up to 4 million tokens)
+    s = one + (n1 < (1 << 22) && b1 < (1 << 30)
+                   ? floor_sum<uint32_t>((uint32_t)n1, kN, (uint32_t)S, (uint32_t)b1)
+                   : floor_sum<uint64_t>((uint64_t)n1, kN, (uint64_t)S, (uint64_t)b1));
   }
   if (i > full && n > 0) s += n_tiles(p, r, n - 1);
   return s + (int64_t)i * kItemCost;
@@ -232,17 +239,7 @@ struct Walk {
   int64_t pos, u, left;  // place inside the item, of the item, places left
   __device__ __forceinline__ bool next(const RaggedPrefillParams& p, Piece& w) {
     while (left > 0) {
-      const int64_t end = min64(pos + left, nt + kItemCost);
-      w.t0 = cut_tile(pos, nt, snap);
-      w.t1 = cut_tile(end, nt, snap);
-      w.r = r;
-      w.b = b;
-      w.kvh = kvh;
-      w.item = item;
-      w.nt = nt;
-      w.u = u;
-      left -= end - pos;
-      if (end == nt + kItemCost) {
+      if (pos == nt + kItemCost) {  // the next item
         u += nt + kItemCost;
         pos = 0;
         if (++item == n) {
@@ -251,20 +248,28 @@ struct Walk {
             kvh = 0;
             bool bad = false;
             do {
-              if (++b >= p.B) {
-                left = 0;
-                break;
-              }
+              if (++b >= p.B) return false;
               r = load_req(p, b, &bad);
               n = n_items(p, r);
             } while (n == 0);
           }
         }
         nt = n_tiles(p, r, item);
-      } else {
-        pos = end;
       }
-      if (w.t0 < w.t1) return true;
+      const int64_t end = min64(pos + left, nt + kItemCost);
+      w.t0 = cut_tile(pos, nt, snap);
+      w.t1 = cut_tile(end, nt, snap);
+      left -= end - pos;
+      pos = end;
+      if (w.t0 < w.t1) {
+        w.r = r;
+        w.b = b;
+        w.kvh = kvh;
+        w.item = item;
+        w.nt = nt;
+        w.u = u;
+        return true;
+      }
     }
     return false;
   }
@@ -371,9 +376,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (w < warp) before += s_warp[w];
     U += s_warp[w];
   }
-  const int64_t nc = min64(gridDim.x, U);  // CTAs that get places
+  // CTA k's range [U k / nc, U (k + 1) / nc) by one division of U (in 32 bits
+  // where it fits) and remainders below 2^18
   const int c = blockIdx.x;
-  const int64_t u0 = c < nc ? U * c / nc : U, u1 = c < nc ? U * (c + 1) / nc : U;
+  const uint32_t nc = (uint32_t)min64(gridDim.x, U);  // CTAs that get places
+  const int64_t share = nc == 0 ? 0 : U >> 32 ? U / nc : (int64_t)((uint32_t)U / nc);
+  const uint32_t rest = (uint32_t)(U - share * nc);
+  auto cut = [&](uint32_t k) { return share * k + (rest * k) / nc; };
+  const int64_t u0 = c < (int)nc ? cut(c) : U, u1 = c < (int)nc ? cut(c + 1) : U;
   if (u0 < u1 && before <= u0 && u0 < before + mine) {
     int64_t at = before;
     for (int b = b0; b < b1; ++b) {
@@ -381,8 +391,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int n = n_items(p, r);
       const int64_t per_head = places(p, r, n), all = per_head * p.Hkv;
       if (u0 < at + all) {
-        const int kvh = (int)((u0 - at) / per_head);
-        const int64_t rem = u0 - at - kvh * per_head;
+        const int64_t off = u0 - at;
+        const int kvh = (int)(all >> 32 ? off / per_head : (uint32_t)off / (uint32_t)per_head);
+        const int64_t rem = off - kvh * per_head;
         int lo = 0, hi = n;  // places(lo) <= rem < places(hi)
         while (hi - lo > 1) {
           const int mid = (lo + hi) >> 1;
@@ -395,7 +406,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         s_walk.item = lo;
         s_walk.n = n;
         s_walk.nt = n_tiles(p, r, lo);
-        s_walk.snap = (int)min64(U / nc / 8, 2);
+        s_walk.snap = (int)min64(share >> 3, 2);
         s_walk.pos = rem - places(p, r, lo);
         s_walk.u = u0 - s_walk.pos;
         s_walk.left = u1 - u0;
@@ -416,19 +427,20 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool ok = true;
       if (lane == 0) p.ws_desc[c] = make_int4(-1, 0, 0, 0);
       while (ok && !*abort_flag && walk.next(p, w)) {
-        if (w.t0 == 0 && w.t1 < w.nt) {
-          // the item goes on in the next CTAs: find the last of them
-          int last = c;
-          for (int k0 = c + 1; k0 < nc; k0 += 32) {
-            const int k = k0 + lane;
-            const int64_t pos = U * k / nc - w.u;
-            const bool in = k < nc && cut_tile(pos, w.nt, walk.snap) < w.nt;
-            const int n = __popc(__ballot_sync(0xffffffffu, in));
-            last += n;
-            if (n < 32) break;
+        // this lane's 64-key block of 16 tiles at a time: its first row in the pool, or
+        // -1 (page_tokens % 64 == 0: a block never straddles); loaded ahead of Q
+        auto block_row = [&](int j) {
+          const int64_t key = ((int64_t)2 * j + lane) * 64;
+          if (key >= w.r.L || 2 * j + lane >= 2 * w.t1) return -1;
+          int pg = p.table[w.b * p.table_stride + (uint32_t)key / (uint32_t)p.page_tokens];
+          if (pg < 0 || pg >= p.num_pages) {  // recorded, page 0 read in its place
+            report_timeout(p.err, 0x932);
+            pg = 0;
           }
-          if (lane == 0) p.ws_desc[c] = make_int4(w.b, w.kvh, w.item, last);
-        }
+          return (int)(((int64_t)pg * p.Hkv + w.kvh) * p.page_tokens +
+                       (uint32_t)key % (uint32_t)p.page_tokens);
+        };
+        int row = block_row(w.t0);
         if (ic >= 1 && !warp_ok(q_empty, (ic - 1) & 1, p.err, 0x93b)) { ok = false; break; }
         if (lane == 0) {
           const int rows = p.T * p.G;  // rows of a tile that hold a (token, head) pair
@@ -442,23 +454,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         ++ic;
-        int row = 0;  // this lane's 64-key block: its first row in the pool, or -1
         for (int j = w.t0; j < w.t1; ++j, ++T) {
           const int s = T & 1, k = (2 * (j - w.t0)) & 31;
-          if (k == 0) {
-            // 16 tiles' pages at once (page_tokens % 64 == 0: a block never straddles)
-            const int64_t key = ((int64_t)2 * j + lane) * 64;
-            row = -1;
-            if (key < w.r.L && (2 * j + lane) < 2 * w.t1) {
-              int pg = p.table[w.b * p.table_stride + (uint32_t)key / (uint32_t)p.page_tokens];
-              if (pg < 0 || pg >= p.num_pages) {  // recorded, page 0 read in its place
-                report_timeout(p.err, 0x932);
-                pg = 0;
-              }
-              row = (int)(((int64_t)pg * p.Hkv + w.kvh) * p.page_tokens +
-                          (uint32_t)key % (uint32_t)p.page_tokens);
-            }
-          }
+          if (k == 0 && j > w.t0) row = block_row(j);
           // blocks past the last position are masked: any valid rows do
           const int ya = max(__shfl_sync(0xffffffffu, row, k), 0);
           const int yb0 = __shfl_sync(0xffffffffu, row, k + 1);
@@ -500,6 +498,18 @@ __global__ void __launch_bounds__(kThreads, 1)
           } else {
             nv = T + 1;
           }
+        }
+        if (w.t0 == 0 && w.t1 < w.nt) {
+          // the item goes on in the next CTAs: find the last of them
+          int last = c;
+          for (uint32_t k0 = c + 1; k0 < nc; k0 += 32) {
+            const uint32_t k = k0 + lane;
+            const bool in = k < nc && cut_tile(cut(min(k, nc)) - w.u, w.nt, walk.snap) < w.nt;
+            const int n = __popc(__ballot_sync(0xffffffffu, in));
+            last += n;
+            if (n < 32) break;
+          }
+          if (lane == 0) p.ws_desc[c] = make_int4(w.b, w.kvh, w.item, last);
         }
       }
       if (!ok) {
