@@ -1076,18 +1076,14 @@ def _ragged_pool(name: str, k_pages: torch.Tensor, v_pages: torch.Tensor):
     return shape
 
 
-def _ragged_table(name: str, t: torch.Tensor, B: int):
-    """Row stride and width of an int32 [B, width] block table."""
-    shape = t.shape
-    if t.dtype == torch.int32 and len(shape) == 2 and shape[0] == B and t.is_contiguous():
-        return shape[1], shape[1]
+def _ragged_table(name: str, t: torch.Tensor, B: int) -> int:
+    """Row stride of an int32 [B, width] block table."""
     if t.dtype != torch.int32:
         raise TypeError(f"{name}: block_table must be int32, got {t.dtype}")
     if t.dim() != 2 or t.shape[0] != B or (t.stride(1) != 1 and t.shape[1] > 1):
         raise ValueError(f"{name}: block_table must be [{B}, width] with dense rows, got "
                          f"{tuple(t.shape)} with strides {t.stride()}")
-    width = t.shape[1]
-    return (t.stride(0) if B > 1 else width), width
+    return t.stride(0) if B > 1 else t.shape[1]
 
 
 def _ragged_ints(name: str, what: str, t: torch.Tensor, dtype, n: int) -> int:
@@ -1097,6 +1093,32 @@ def _ragged_ints(name: str, what: str, t: torch.Tensor, dtype, n: int) -> int:
     if t.numel() != n:
         raise ValueError(f"{name}: {what} must have {n} entries, got {t.numel()}")
     return t.data_ptr()
+
+
+def _ragged_attn(name: str, q, k_pages, v_pages, block_table, kv_lens, out, B: int):
+    """Checks what both attentions take; (device, q stride, table stride, out, its stride)."""
+    bf16, i32 = torch.bfloat16, torch.int32
+    dev, qs, ks, ts = q.get_device(), q.shape, k_pages.shape, block_table.shape
+    if (out is None and len(qs) == 3 and len(ks) == 4 and len(ts) == 2 and qs[2] == HEAD_DIM and
+            ks[3] == HEAD_DIM and v_pages.shape == ks and ts[0] == B and kv_lens.numel() == B and
+            dev >= 0 and k_pages.get_device() == dev and v_pages.get_device() == dev and
+            block_table.get_device() == dev and kv_lens.get_device() == dev and
+            q.dtype is bf16 and k_pages.dtype is bf16 and v_pages.dtype is bf16 and
+            block_table.dtype is i32 and kv_lens.dtype is i32 and q.is_contiguous() and
+            k_pages.is_contiguous() and v_pages.is_contiguous() and
+            block_table.is_contiguous() and kv_lens.is_contiguous()):
+        # the dense call in one pass
+        stride = qs[1] * HEAD_DIM
+        return dev, stride, ts[1], torch.empty_like(q), stride
+    _ragged_device(name, q, k_pages, v_pages, block_table, kv_lens, out)
+    _ragged_pool(name, k_pages, v_pages)
+    if len(qs) != 3:
+        raise ValueError(f"{name}: q must be [rows, heads, 128], got {tuple(qs)}")
+    q_stride = _ragged_rows(name, "q", q)
+    table_stride = _ragged_table(name, block_table, B)
+    _ragged_ints(name, "kv_lens", kv_lens, i32, B)
+    out, out_stride = _ragged_out(name, out, q, q_stride)
+    return dev, q_stride, table_stride, out, out_stride
 
 
 def ragged_plan(q_lens: torch.Tensor, past_lens: torch.Tensor, block_table: torch.Tensor, *,
@@ -1115,28 +1137,32 @@ def ragged_plan(q_lens: torch.Tensor, past_lens: torch.Tensor, block_table: torc
     back: counts[1] pages of the list were taken (more than its length, and
     0x903 in the device error word, when it was short)."""
     name = "ragged_plan"
+    i32 = torch.int32
     dev = _ragged_device(name, q_lens, past_lens, block_table, free_pages, free_start, rope_delta)
     B, n = q_lens.numel(), int(n_tokens)
     if n < 0:
         raise ValueError(f"{name}: n_tokens={n}")
-    stride, width = _ragged_table(name, block_table, B)
-    n_free = 0 if free_pages is None else free_pages.numel()
+    stride = _ragged_table(name, block_table, B)
+    at_free = at_start = at_delta = None
+    n_free = 0
+    if free_pages is not None:
+        n_free = free_pages.numel()
+        at_free = _ragged_ints(name, "free_pages", free_pages, i32, n_free)
+    if free_start is not None:
+        at_start = _ragged_ints(name, "free_start", free_start, i32, 1)
+    if rope_delta is not None:
+        at_delta = _ragged_ints(name, "rope_delta", rope_delta, torch.int64, B)
     # one allocation for the six results (the 64-bit ones first, for alignment)
     buf = q_lens.new_empty(5 * n + 2 * B + 3)
     positions, slots, requests, cu_q, kv_lens, counts = buf.split_with_sizes(
         (2 * n, 2 * n, n, B + 1, B, 2))
     at = buf.data_ptr()
     at_cu = at + 20 * n
-    _ragged_call("q3_ragged_plan", dev, _ragged_ints(name, "q_lens", q_lens, torch.int32, B),
-                 _ragged_ints(name, "past_lens", past_lens, torch.int32, B), B,
-                 block_table.data_ptr(), stride, width, int(page_tokens),
-                 None if free_pages is None else
-                 _ragged_ints(name, "free_pages", free_pages, torch.int32, n_free), n_free,
-                 None if free_start is None else
-                 _ragged_ints(name, "free_start", free_start, torch.int32, 1),
-                 None if rope_delta is None else
-                 _ragged_ints(name, "rope_delta", rope_delta, torch.int64, B), n, at_cu,
-                 at_cu + 4 * (B + 1), at + 16 * n, at, at + 8 * n, at_cu + 4 * (2 * B + 1))
+    _ragged_call("q3_ragged_plan", dev, _ragged_ints(name, "q_lens", q_lens, i32, B),
+                 _ragged_ints(name, "past_lens", past_lens, i32, B), B, block_table.data_ptr(),
+                 stride, block_table.shape[1], int(page_tokens), at_free, n_free, at_start,
+                 at_delta, n, at_cu, at_cu + 4 * (B + 1), at + 16 * n, at, at + 8 * n,
+                 at_cu + 4 * (2 * B + 1))
     return RaggedPlan(cu_q, kv_lens, requests, positions.view(torch.int64),
                       slots.view(torch.int64), counts)
 
@@ -1204,20 +1230,16 @@ def attn_decode_ragged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Te
     device: request b attends to positions [0, kv_lens[b]), and a length of 0
     gives zeros.  Hq / Hkv is any whole number up to 16."""
     name = "attn_decode_ragged"
-    dev = _ragged_device(name, q, k_pages, v_pages, block_table, kv_lens, out)
-    num_pages, Hkv, page_tokens, _ = _ragged_pool(name, k_pages, v_pages)
-    if q.dim() != 3:
-        raise ValueError(f"{name}: q must be [B, Hq, 128], got {tuple(q.shape)}")
-    B, Hq, D = q.shape
-    q_stride = _ragged_rows(name, "q", q)
-    table_stride, width = _ragged_table(name, block_table, B)
-    out, out_stride = _ragged_out(name, out, q, q_stride)
+    B, Hq = q.shape[0], q.shape[1]
+    dev, q_stride, table_stride, out, out_stride = _ragged_attn(name, q, k_pages, v_pages,
+                                                                block_table, kv_lens, out, B)
+    num_pages, Hkv, page_tokens, D = k_pages.shape
     nbytes = _lib.raw("q3_attn_decode_ragged_workspace_bytes")(Hq, Hkv)
     ws = q.new_empty(nbytes, dtype=torch.uint8)
     _ragged_call("q3_attn_decode_ragged", dev, q.data_ptr(), q_stride, k_pages.data_ptr(),
                  v_pages.data_ptr(), out.data_ptr(), out_stride, B, Hq, Hkv, D,
-                 block_table.data_ptr(), table_stride, width, page_tokens, num_pages,
-                 _ragged_ints(name, "kv_lens", kv_lens, torch.int32, B),
+                 block_table.data_ptr(), table_stride, block_table.shape[1], page_tokens,
+                 num_pages, kv_lens.data_ptr(),
                  HEAD_DIM ** -0.5 if scale is None else float(scale), ws.data_ptr(), nbytes)
     return out
 
@@ -1235,22 +1257,20 @@ def attn_prefill_ragged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.T
     through slices of cu_q, kv_lens and block_table.  A query that sees nothing
     gives zeros.  Hq / Hkv is any whole number up to 16; scale is positive."""
     name = "attn_prefill_ragged"
-    dev = _ragged_device(name, q, k_pages, v_pages, block_table, cu_q, kv_lens, out)
-    num_pages, Hkv, page_tokens, _ = _ragged_pool(name, k_pages, v_pages)
-    if q.dim() != 3:
-        raise ValueError(f"{name}: q must be [n, Hq, 128], got {tuple(q.shape)}")
-    n, Hq, D = q.shape
     B = kv_lens.numel()
-    q_stride = _ragged_rows(name, "q", q)
-    table_stride, width = _ragged_table(name, block_table, B)
-    out, out_stride = _ragged_out(name, out, q, q_stride)
+    dev, q_stride, table_stride, out, out_stride = _ragged_attn(name, q, k_pages, v_pages,
+                                                                block_table, kv_lens, out, B)
+    n, Hq, D = q.shape
+    num_pages, Hkv, page_tokens, _ = k_pages.shape
+    if cu_q.get_device() != dev:
+        raise RuntimeError(f"{name}: cu_q must be on the other tensors' CUDA device")
     nbytes = _lib.raw("q3_attn_prefill_ragged_workspace_bytes")()
     ws = q.new_empty(nbytes, dtype=torch.uint8)
     _ragged_call("q3_attn_prefill_ragged", dev, q.data_ptr(), q_stride, k_pages.data_ptr(),
                  v_pages.data_ptr(), out.data_ptr(), out_stride, n, B, Hq, Hkv, D,
-                 block_table.data_ptr(), table_stride, width, page_tokens, num_pages,
-                 _ragged_ints(name, "cu_q", cu_q, torch.int32, B + 1),
-                 _ragged_ints(name, "kv_lens", kv_lens, torch.int32, B), 1 if causal else 0,
+                 block_table.data_ptr(), table_stride, block_table.shape[1], page_tokens,
+                 num_pages, _ragged_ints(name, "cu_q", cu_q, torch.int32, B + 1),
+                 kv_lens.data_ptr(), 1 if causal else 0,
                  HEAD_DIM ** -0.5 if scale is None else float(scale), ws.data_ptr(), nbytes)
     return out
 
