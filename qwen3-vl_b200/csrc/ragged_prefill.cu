@@ -19,16 +19,21 @@
 // S, and O is rescaled in place only when a row's maximum has grown by 2^8.
 //
 // Bound by the tensor pipe and the softmax (4 * 128 flops per visible pair).
-// The lengths are only known on the device, so the 128-key tiles of all items,
-// plus two places per item for its fixed cost, form one list that is cut into
-// equal ranges, one per SM; a cut within 2 tiles of an item's edge moves there (a
-// split costs about as much as a tile; with cuts moved by up to 1/16 of a range
-// the six-prompt case had 12 % more tiles on one SM than on average).  An item cut in the middle leaves fp32 pieces (O, base, sum)
-// in the workspace and a second kernel joins them in CTA order: a 512-token
-// chunk on a 32k cache fills every SM (its 64 items alone would fill 64).
-// Measured on B200, 32/8 heads: that chunk 256 us (1065 TFLOP/s at the clock the
-// power cap leaves in a long run, 1.66 GHz and 61 % of the tensor pipe under
-// ncu); six prompts of 1100 to 4096 tokens 469 us (997).
+// The lengths are only known on the device, so the keys of all items, plus two
+// tiles' worth per item for its fixed cost, form one list that is cut into equal
+// ranges, one per SM (fewer when the list has fewer tiles than SMs).  A cut inside
+// an item goes to the nearest tile boundary, and within 2 tiles of the item's edge
+// to the edge (a split costs about as much as a tile; with cuts moved by up to 1/16
+// of a range the six-prompt case had 12 % more tiles on one SM than on average).
+// Counting keys instead of tiles makes a request's sum a polynomial: with tiles it
+// was a floor sum and a search, 16300 against 2900 cycles before the first load at
+// 10/2 heads.  An item cut in the middle leaves fp32 pieces (O, base, sum) in the
+// workspace and a second kernel joins them in CTA order: a 512-token chunk on a 32k
+// cache fills every SM (its 64 items alone would fill 64).
+// Measured on B200, 32/8 heads: that chunk 256 to 268 us by device (1065 to 1017
+// TFLOP/s at the clock the power cap leaves in a long run, 1.66 GHz and 61 % of the
+// tensor pipe under ncu); six prompts of 1100 to 4096 tokens 469 to 480 us (997 to
+// 975); four prompts of up to 100 tokens at 4/1 heads 11.6 us.
 #include <math.h>
 
 #include "common.cuh"
@@ -62,7 +67,7 @@ constexpr float kLazyLog2 = 16.0f;
 constexpr int kMaxB = 65536;
 constexpr int kMaxGrid = 512;
 constexpr int kPieceRows = 2 * kM;
-constexpr int kItemCost = 2;              // places of the work list an item takes besides its tiles
+constexpr int kItemCost = 2 * kN;         // places of the work list an item takes besides its keys
 
 struct RaggedPrefillParams {
   __nv_bfloat16* out;
@@ -157,9 +162,10 @@ __device__ __forceinline__ void regs_inc() {
 // ---------------------------------------------------------------------------
 // The work list.  Request b has n = ceil(q_len / 2T) items per K/V head; item i
 // has tiles(i) = max(1, ceil(x / 128)) key tiles, x = the positions its last
-// query sees.  Every item takes tiles(i) + kItemCost places in the list (loading
-// its queries, an epilogue and a first tile that moves the base cost about 5000
-// cycles; a tile takes about 3200).
+// query sees.  An item takes x + kItemCost places in the list: its keys, whose
+// sum over items is a polynomial (tiles would be a sum of roundings), and a fixed
+// cost (loading its queries, an epilogue and a first tile that moves the base
+// take about 5000 cycles; a tile takes about 3200).
 // ---------------------------------------------------------------------------
 struct Req {
   int q0, q_len, L, past;  // first packed row, queries, cached positions, L - q_len
@@ -181,49 +187,39 @@ __device__ __forceinline__ int n_tiles(const RaggedPrefillParams& p, const Req& 
   const int x = p.causal ? r.past + min(r.q_len, (i + 1) * 2 * p.T) : r.L;
   return x <= kN ? 1 : (x + kN - 1) / kN;
 }
-// sum over i in [0, n) of floor((a i + b) / m), by Euclid's division steps, in
-// words of type U that hold a n + b
-template <typename U>
-__device__ __forceinline__ int64_t floor_sum(U n, U m, U a, U b) {
-  int64_t s = 0;
-  while (n > 0) {
-    const U qa = a / m, qb = b / m;
-    s += (int64_t)(n - 1) * (int64_t)n / 2 * (int64_t)qa + (int64_t)n * (int64_t)qb;
-    a -= qa * m;
-    b -= qb * m;
-    const U y = a * n + b;
-    if (y < m) break;
-    n = y / m;
-    b = y - n * m;
-    const U t = m;
-    m = a;
-    a = t;
-  }
-  return s;
+// places of item i, and of items [0, i) of one K/V head (a request whose tokens
+// outnumber its positions counts as if it had none before them)
+__device__ __forceinline__ int weight(const RaggedPrefillParams& p, const Req& r, int i) {
+  if (!p.causal) return r.L + kItemCost;
+  return max(r.past, 0) + min(r.q_len, (i + 1) * 2 * p.T) + kItemCost;
 }
-// places that items [0, i) of one K/V head take
-__device__ __forceinline__ int64_t places(const RaggedPrefillParams& p, const Req& r, int i) {
-  if (!p.causal) return (int64_t)i * (n_tiles(p, r, 0) + kItemCost);
-  const int n = n_items(p, r), S = 2 * p.T;
-  const int full = min(i, n - 1);  // items whose last query is (k + 1) * 2T
-  int64_t s = 0;
-  if (full > 0) {
-    const int one = r.past >= kN ? 0 : min(full, (kN - r.past) / S);  // those with one tile
-    const int64_t n1 = full - one, b1 = (int64_t)r.past + (int64_t)(one + 1) * S + kN - 1;
-    // 32-bit divisions where S n + b fits (prompts of up to 4 million tokens)
-    s = one + (n1 < (1 << 22) && b1 < (1 << 30)
-                   ? floor_sum<uint32_t>((uint32_t)n1, kN, (uint32_t)S, (uint32_t)b1)
-                   : floor_sum<uint64_t>((uint64_t)n1, kN, (uint64_t)S, (uint64_t)b1));
-  }
-  if (i > full && n > 0) s += n_tiles(p, r, n - 1);
-  return s + (int64_t)i * kItemCost;
+__device__ __forceinline__ int64_t places(const RaggedPrefillParams& p, const Req& r, int n, int i) {
+  if (!p.causal) return (int64_t)i * (r.L + kItemCost);
+  const int64_t base = (int64_t)max(r.past, 0) + kItemCost;
+  const int64_t full = i < n ? i : max(n - 1, 0);  // items that end at (k + 1) * 2T
+  const int64_t s = full * base + (int64_t)p.T * full * (full + 1);
+  return i > full ? s + base + r.q_len : s;
 }
-// A cut at place `pos` of an item of nt tiles, as a tile boundary 0..nt: the first
-// places are the item's fixed cost, and a cut within `snap` tiles of an edge
-// moves to the nearer one.
-__device__ __forceinline__ int cut_tile(int64_t pos, int nt, int snap) {
-  if (pos >= nt + kItemCost) return nt;
-  const int t = (int)max64(pos - kItemCost, 0);
+// The item (of n) at place `rem` of one K/V head's items: the root of places(i) =
+// rem in fp32, corrected by the exact sums.
+__device__ __forceinline__ int item_at(const RaggedPrefillParams& p, const Req& r, int n,
+                                       int64_t rem) {
+  if (n == 1) return 0;
+  const float h = (float)max(r.past, 0) + (float)(kItemCost + p.T), T = (float)p.T;
+  const float d = h * h + 4.f * T * (float)rem;
+  const float x = p.causal ? __fdividef(d * rsqrtf(d) - h, 2.f * T)
+                           : __fdividef((float)rem, (float)(r.L + kItemCost));
+  int i = min(max((int)x, 0), n - 1);
+  while (i > 0 && places(p, r, n, i) > rem) --i;
+  while (i + 1 < n && places(p, r, n, i + 1) <= rem) ++i;
+  return i;
+}
+// A cut at place `pos` of an item of `w` places and nt tiles, as a tile boundary
+// 0..nt: the nearest one, and within `snap` tiles of an edge the edge.  Cuts of
+// the list are at least a tile apart, so those inside an item stay apart.
+__device__ __forceinline__ int cut_tile(int64_t pos, int w, int nt, int snap) {
+  if (pos >= w) return nt;
+  const int t = min((int)(max64(pos - kItemCost + kN / 2, 0) / kN), nt);
   if (t < snap && 2 * t < nt) return 0;
   return nt - t < snap ? nt : t;
 }
@@ -235,12 +231,12 @@ struct Piece {
 };
 struct Walk {
   Req r;
-  int b, kvh, item, n, nt, snap;
+  int b, kvh, item, n, nt, places, snap;
   int64_t pos, u, left;  // place inside the item, of the item, places left
   __device__ __forceinline__ bool next(const RaggedPrefillParams& p, Piece& w) {
     while (left > 0) {
-      if (pos == nt + kItemCost) {  // the next item
-        u += nt + kItemCost;
+      if (pos == places) {  // the next item
+        u += places;
         pos = 0;
         if (++item == n) {
           item = 0;
@@ -255,10 +251,11 @@ struct Walk {
           }
         }
         nt = n_tiles(p, r, item);
+        places = weight(p, r, item);
       }
-      const int64_t end = min64(pos + left, nt + kItemCost);
-      w.t0 = cut_tile(pos, nt, snap);
-      w.t1 = cut_tile(end, nt, snap);
+      const int64_t end = min64(pos + left, places);
+      w.t0 = cut_tile(pos, places, nt, snap);
+      w.t1 = cut_tile(end, places, nt, snap);
       left -= end - pos;
       pos = end;
       if (w.t0 < w.t1) {
@@ -354,7 +351,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   bool bad = false;
   for (int b = b0; b < b1; ++b) {
     const Req r = load_req(p, b, &bad);
-    mine += places(p, r, n_items(p, r));
+    const int n = n_items(p, r);
+    mine += places(p, r, n, n);
   }
   mine *= p.Hkv;
   if (bad && blockIdx.x == 0) report_timeout(p.err, 0x931);
@@ -379,7 +377,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   // CTA k's range [U k / nc, U (k + 1) / nc) by one division of U (in 32 bits
   // where it fits) and remainders below 2^18
   const int c = blockIdx.x;
-  const uint32_t nc = (uint32_t)min64(gridDim.x, U);  // CTAs that get places
+  const uint32_t nc = (uint32_t)min64(gridDim.x, U / kN);  // CTAs that get places, a tile or more
   const int64_t share = nc == 0 ? 0 : U >> 32 ? U / nc : (int64_t)((uint32_t)U / nc);
   const uint32_t rest = (uint32_t)(U - share * nc);
   auto cut = [&](uint32_t k) { return share * k + (rest * k) / nc; };
@@ -389,25 +387,21 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int b = b0; b < b1; ++b) {
       const Req r = load_req(p, b, &bad);
       const int n = n_items(p, r);
-      const int64_t per_head = places(p, r, n), all = per_head * p.Hkv;
+      const int64_t per_head = places(p, r, n, n), all = per_head * p.Hkv;
       if (u0 < at + all) {
         const int64_t off = u0 - at;
         const int kvh = (int)(all >> 32 ? off / per_head : (uint32_t)off / (uint32_t)per_head);
         const int64_t rem = off - kvh * per_head;
-        int lo = 0, hi = n;  // places(lo) <= rem < places(hi)
-        while (hi - lo > 1) {
-          const int mid = (lo + hi) >> 1;
-          if (places(p, r, mid) <= rem) lo = mid;
-          else hi = mid;
-        }
+        const int item = item_at(p, r, n, rem);
         s_walk.r = r;
         s_walk.b = b;
         s_walk.kvh = kvh;
-        s_walk.item = lo;
+        s_walk.item = item;
         s_walk.n = n;
-        s_walk.nt = n_tiles(p, r, lo);
-        s_walk.snap = (int)min64(share >> 3, 2);
-        s_walk.pos = rem - places(p, r, lo);
+        s_walk.nt = n_tiles(p, r, item);
+        s_walk.places = weight(p, r, item);
+        s_walk.snap = (int)min64(share / (8 * kN), 2);
+        s_walk.pos = rem - places(p, r, n, item);
         s_walk.u = u0 - s_walk.pos;
         s_walk.left = u1 - u0;
         break;
@@ -504,7 +498,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           int last = c;
           for (uint32_t k0 = c + 1; k0 < nc; k0 += 32) {
             const uint32_t k = k0 + lane;
-            const bool in = k < nc && cut_tile(cut(min(k, nc)) - w.u, w.nt, walk.snap) < w.nt;
+            const bool in =
+                k < nc && cut_tile(cut(min(k, nc)) - w.u, walk.places, w.nt, walk.snap) < w.nt;
             const int n = __popc(__ballot_sync(0xffffffffu, in));
             last += n;
             if (n < 32) break;
@@ -761,19 +756,23 @@ __global__ void __launch_bounds__(kThreads, 1)
         // piece that began inside its item has the even slot.
         const int64_t slot = 2 * c + (w.t0 == 0 ? 1 : 0);
         const int r256 = t * kM + row;
-        p.ws_ml[(slot * 2) * kPieceRows + r256] = m_used;
-        p.ws_ml[(slot * 2 + 1) * kPieceRows + r256] = l;
+        if (live) {
+          p.ws_ml[(slot * 2) * kPieceRows + r256] = m_used;
+          p.ws_ml[(slot * 2 + 1) * kPieceRows + r256] = l;
+        }
         float4* dst = reinterpret_cast<float4*>(p.ws_o) + slot * 32 * kPieceRows + r256;
 #pragma unroll
         for (int cc = 0; cc < kD / 32; ++cc) {
           uint32_t r32[32];
           tmem_ld_32cols(o_col + cc * 32, r32);
           tc_wait_ld();
+          if (live) {
 #pragma unroll
-          for (int d = 0; d < 8; ++d)
-            dst[(cc * 8 + d) * kPieceRows] =
-                make_float4(__uint_as_float(r32[4 * d]), __uint_as_float(r32[4 * d + 1]),
-                            __uint_as_float(r32[4 * d + 2]), __uint_as_float(r32[4 * d + 3]));
+            for (int d = 0; d < 8; ++d)
+              dst[(cc * 8 + d) * kPieceRows] =
+                  make_float4(__uint_as_float(r32[4 * d]), __uint_as_float(r32[4 * d + 1]),
+                              __uint_as_float(r32[4 * d + 2]), __uint_as_float(r32[4 * d + 3]));
+          }
         }
       }
       tc_fence_before();
@@ -793,47 +792,76 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // Joins the pieces of the item that CTA c left unfinished: slots 2c+1, 2(c+1),
-// ..., 2*last, in that order.  One thread per row of the item and 16 dims.
-constexpr int kJoinD4 = 4;  // float4 columns per CTA
-__global__ void __launch_bounds__(kPieceRows) ragged_prefill_join(RaggedPrefillParams p) {
-  pdl_launch();
-  pdl_wait();
-  const int c = blockIdx.x, d40 = blockIdx.y * kJoinD4, r256 = threadIdx.x;
-  const int4 d = p.ws_desc[c];
-  if (d.x < 0) return;
-  const int t = r256 / kM, row = r256 - t * kM;
-  const int tok_in = row / p.G, head_in = row - tok_in * p.G;
-  const int tok = (2 * d.z + t) * p.T + tok_in;
-  bool bad = false;
-  const Req r = load_req(p, d.x, &bad);
-  if (row >= p.T * p.G || tok >= r.q_len) return;
-  const int n = d.w - c + 1;
-  auto slot = [&](int i) { return (int64_t)(i == 0 ? 2 * c + 1 : 2 * (c + i)); };
+// ..., 2*last, in that order.  Eight CTAs per item, 16 dims each.  With few pieces
+// (two is the usual case) a thread takes one of the 256 rows; with many pieces of
+// few rows (nine queries on a 17k cache) the warps share the pieces of 32 rows at
+// a time: 50 -> 21 us for that call, whose 130 pieces a thread took one by one.
+constexpr int kJoinD4 = 4;      // float4 columns (of 32) at a time
+constexpr int kJoinWarps = 8;
+// the workspace slot of piece i of the item that CTA c left unfinished
+__device__ __forceinline__ int64_t piece_slot(int c, int i) {
+  return i == 0 ? 2 * c + 1 : 2 * (c + i);
+}
+struct JoinRow {
+  int c, first, step, n, r256;  // pieces first, first + step, ... below n of row r256
+};
+// The row's maximum over the pieces, and sums and dims 4 d40 .. relative to it.
+// Loads of two pieces are issued before any is used (four take 126 registers,
+// and CTAs without an item then leave more slowly).
+constexpr int kJoinBatch = 2;
+__device__ __forceinline__ float join_max(const RaggedPrefillParams& p, const JoinRow& j) {
   float M = -INFINITY;
-#pragma unroll 4
-  for (int i = 0; i < n; ++i) M = fmaxf(M, p.ws_ml[slot(i) * 2 * kPieceRows + r256]);
-  float4 a[kJoinD4];
+  for (int i0 = j.first; i0 < j.n; i0 += kJoinBatch * j.step) {
+    float m[kJoinBatch];
+#pragma unroll
+    for (int u = 0; u < kJoinBatch; ++u) {
+      const int i = min(i0 + u * j.step, j.n - 1);  // the last again: no change
+      m[u] = p.ws_ml[piece_slot(j.c, i) * 2 * kPieceRows + j.r256];
+    }
+#pragma unroll
+    for (int u = 0; u < kJoinBatch; ++u) M = fmaxf(M, m[u]);
+  }
+  return M;
+}
+__device__ __forceinline__ float join_sum(const RaggedPrefillParams& p, const JoinRow& j, float M,
+                                          int d40, float4 (&a)[kJoinD4]) {
 #pragma unroll
   for (int k = 0; k < kJoinD4; ++k) a[k] = make_float4(0.f, 0.f, 0.f, 0.f);
   float l = 0.f;
-#pragma unroll 2
-  for (int i = 0; i < n; ++i) {
-    const float mi = p.ws_ml[slot(i) * 2 * kPieceRows + r256];
-    const float f = mi == -INFINITY ? 0.f : ex2_approx(mi - M);
-    l = fmaf(f, p.ws_ml[(slot(i) * 2 + 1) * kPieceRows + r256], l);
-    const float4* src = reinterpret_cast<const float4*>(p.ws_o) + slot(i) * 32 * kPieceRows + r256;
+  for (int i0 = j.first; i0 < j.n; i0 += kJoinBatch * j.step) {
+    float m[kJoinBatch], li[kJoinBatch];
+    float4 x[kJoinBatch][kJoinD4];
 #pragma unroll
-    for (int k = 0; k < kJoinD4; ++k) {
-      const float4 x = src[(d40 + k) * kPieceRows];
-      a[k].x = fmaf(f, x.x, a[k].x);
-      a[k].y = fmaf(f, x.y, a[k].y);
-      a[k].z = fmaf(f, x.z, a[k].z);
-      a[k].w = fmaf(f, x.w, a[k].w);
+    for (int u = 0; u < kJoinBatch; ++u) {
+      const int i = i0 + u * j.step;
+      const int64_t slot = piece_slot(j.c, min(i, j.n - 1));
+      const float* ml = p.ws_ml + slot * 2 * kPieceRows + j.r256;
+      m[u] = i < j.n ? ml[0] : -INFINITY;
+      li[u] = ml[kPieceRows];
+      const float4* src =
+          reinterpret_cast<const float4*>(p.ws_o) + (slot * 32 + d40) * kPieceRows + j.r256;
+#pragma unroll
+      for (int k = 0; k < kJoinD4; ++k) x[u][k] = src[k * kPieceRows];
+    }
+#pragma unroll
+    for (int u = 0; u < kJoinBatch; ++u) {
+      const float f = m[u] == -INFINITY ? 0.f : ex2_approx(m[u] - M);
+      if (f == 0.f) continue;  // a piece of which the row sees nothing, or none
+      l = fmaf(f, li[u], l);
+#pragma unroll
+      for (int k = 0; k < kJoinD4; ++k) {
+        a[k].x = fmaf(f, x[u][k].x, a[k].x);
+        a[k].y = fmaf(f, x[u][k].y, a[k].y);
+        a[k].z = fmaf(f, x[u][k].z, a[k].z);
+        a[k].w = fmaf(f, x[u][k].w, a[k].w);
+      }
     }
   }
+  return l;
+}
+__device__ __forceinline__ void join_store(__nv_bfloat16* dst, const float4 (&a)[kJoinD4],
+                                           float l) {
   const float inv = l > 0.f ? 1.f / l : 0.f;
-  __nv_bfloat16* dst = p.out + (int64_t)(r.q0 + tok) * p.out_stride +
-                       (int64_t)(d.y * p.G + head_in) * kD + d40 * 4;
 #pragma unroll
   for (int k = 0; k < kJoinD4; k += 2) {
     uint4 u;
@@ -842,6 +870,72 @@ __global__ void __launch_bounds__(kPieceRows) ragged_prefill_join(RaggedPrefillP
     u.z = pack_bf16x2(a[k + 1].x * inv, a[k + 1].y * inv);
     u.w = pack_bf16x2(a[k + 1].z * inv, a[k + 1].w * inv);
     *reinterpret_cast<uint4*>(dst + k * 4) = u;
+  }
+}
+__global__ void __launch_bounds__(kJoinWarps * 32) ragged_prefill_join(RaggedPrefillParams p) {
+  __shared__ float s_m[kJoinWarps][32], s_l[kJoinWarps][32];
+  __shared__ float4 s_acc[kJoinWarps][kJoinD4][32];
+  pdl_launch();
+  pdl_wait();
+  const int c = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int d40 = blockIdx.y * kJoinD4;
+  const int4 d = p.ws_desc[c];
+  if (d.x < 0) return;
+  const int n = d.w - c + 1;
+  bool bad = false;
+  const Req r = load_req(p, d.x, &bad);
+  // rows of query tile t that hold a token of the request
+  auto live_rows = [&](int t) {
+    return max(min(r.q_len - (2 * d.z + t) * p.T, p.T), 0) * p.G;
+  };
+  auto out_of = [&](int r256) {
+    const int t = r256 / kM, row = r256 - t * kM, tok_in = row / p.G;
+    return p.out + (int64_t)(r.q0 + (2 * d.z + t) * p.T + tok_in) * p.out_stride +
+           (int64_t)(d.y * p.G + row - tok_in * p.G) * kD + d40 * 4;
+  };
+  float4 a[kJoinD4];
+  // A thread with its row's n pieces takes about 430 n cycles (its loads wait in
+  // turn); eight warps take 54 n + 1500 for each of the blocks of 32 live rows.
+  const int blocks = (live_rows(0) + 31) / 32 + (live_rows(1) + 31) / 32;
+  if (blocks * (n + 28) >= 8 * n) {
+    const int r256 = threadIdx.x;
+    if (r256 % kM >= live_rows(r256 / kM)) return;
+    const JoinRow j{c, 0, 1, n, r256};
+    const float l = join_sum(p, j, join_max(p, j), d40, a);
+    join_store(out_of(r256), a, l);
+    return;
+  }
+#pragma unroll 1
+  for (int r0 = 0; r0 < kPieceRows; r0 += 32) {  // lane = row
+    const int live = live_rows(r0 / kM) - r0 % kM;
+    if (live <= 0) continue;
+    const JoinRow j{c, warp, kJoinWarps, n, r0 + lane};
+    s_m[warp][lane] = join_max(p, j);
+    __syncthreads();
+    float M = s_m[0][lane];
+#pragma unroll
+    for (int i = 1; i < kJoinWarps; ++i) M = fmaxf(M, s_m[i][lane]);
+    s_l[warp][lane] = join_sum(p, j, M, d40, a);
+#pragma unroll
+    for (int k = 0; k < kJoinD4; ++k) s_acc[warp][k][lane] = a[k];
+    __syncthreads();
+    if (warp == 0 && lane < live) {  // the warps' sums in order
+      float l = s_l[0][lane];
+#pragma unroll
+      for (int i = 1; i < kJoinWarps; ++i) {
+        l += s_l[i][lane];
+#pragma unroll
+        for (int k = 0; k < kJoinD4; ++k) {
+          const float4 x = s_acc[i][k][lane];
+          a[k].x += x.x;
+          a[k].y += x.y;
+          a[k].z += x.z;
+          a[k].w += x.w;
+        }
+      }
+      join_store(out_of(r0 + lane), a, l);
+    }
+    __syncthreads();
   }
 }
 
@@ -931,6 +1025,6 @@ extern "C" int q3_attn_prefill_ragged(const void* q, int64_t q_stride, const voi
   rc = launch_ex(ragged_prefill_kernel, grid, dim3(kThreads), kSmem, (cudaStream_t)stream, 1, tq,
                  tk, tv, p);
   if (rc) return rc;
-  return launch_ex(ragged_prefill_join, dim3(grid.x, kD / 4 / kJoinD4), dim3(kPieceRows), 0,
+  return launch_ex(ragged_prefill_join, dim3(grid.x, kD / 4 / kJoinD4), dim3(kJoinWarps * 32), 0,
                    (cudaStream_t)stream, 1, p);
 }

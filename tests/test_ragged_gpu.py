@@ -325,6 +325,22 @@ def test_prefill(q_lens, pasts, Hq, Hkv, page, causal):
     assert torch.equal(got, ops.attn_prefill_ragged(*args, causal=causal))
 
 
+@pytest.mark.parametrize("q_lens,pasts,Hq,Hkv,page", [
+    ([9], [17000], 8, 1, 128), ([1, 2], [9000, 4000], 4, 1, 64), ([31, 260], [5000, 1778], 6, 1, 256),
+    ([16], [12345], 16, 1, 192)])
+def test_prefill_of_few_rows_with_many_pieces(q_lens, pasts, Hq, Hkv, page):
+    """One item cut over most SMs: the rows' bases rise from piece to piece."""
+    q, k, v, table, cu, lens = prefill_case(q_lens, pasts, Hq, Hkv, page, seed=21)
+    for b, n in enumerate(lens):                    # keys grow along the request
+        for j in range(-(-n // page)):
+            k[table[b][j]] *= 0.25 + 2.0 * j * page / n
+    want, tol = ora.attention(q, k, v, table, lens, q_lens)
+    args = (q.to(DEV), k.to(DEV), v.to(DEV), i32(table), i32(cu), i32(lens))
+    got = ops.attn_prefill_ragged(*args)
+    ora.check("prefill", got, want, tol)
+    assert torch.equal(got, ops.attn_prefill_ragged(*args))
+
+
 def test_prefill_matches_the_one_start_kernel():
     B, S, Hq, Hkv, page, start = 2, 300, 8, 2, 128, 128
     q, k, v, table, cu, lens = prefill_case([S] * B, [start] * B, Hq, Hkv, page, stale=0.0)

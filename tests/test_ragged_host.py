@@ -3,6 +3,7 @@ touches a device, the Python wrappers' refusals, and the plan's 64-bit form
 against the page allocator's own tables."""
 import ctypes
 
+import numpy as np
 import pytest
 import torch
 
@@ -176,19 +177,7 @@ def test_decode_division_covers_every_tile_once(lens, Hkv, grid):
     assert not per or max(per) - min(per) <= 1
 
 
-def floor_sum(n, m, a, b):
-    s = 0
-    while n > 0:
-        s += (n - 1) * n // 2 * (a // m) + n * (b // m)
-        a, b = a % m, b % m
-        y = a * n + b
-        if y < m:
-            break
-        n, b, m, a = y // m, y % m, a, m
-    return s
-
-
-ITEM_COST = 2          # places of the list an item takes besides its tiles
+ITEM_COST = 256        # places of the list an item takes besides its keys
 
 
 def n_tiles(T, q, L, i, causal=True):
@@ -196,36 +185,65 @@ def n_tiles(T, q, L, i, causal=True):
     return 1 if x <= 128 else -(-x // 128)
 
 
+def weight(T, q, L, i, causal=True):
+    return (max(L - q, 0) + min(q, (i + 1) * 2 * T) if causal else L) + ITEM_COST
+
+
 def places(T, q, L, i, causal=True):
     """Places of items [0, i), as the kernel sums them in closed form."""
     if not causal:
-        return i * (n_tiles(T, q, L, 0, False) + ITEM_COST)
-    n, S, past = -(-q // (2 * T)), 2 * T, L - q
-    full, s = min(i, n - 1), 0
-    if full > 0:
-        one = 0 if past >= 128 else min(full, (128 - past) // S)
-        s = one + floor_sum(full - one, 128, S, past + (one + 1) * S + 127)
-    if i > full and n > 0:
-        s += n_tiles(T, q, L, n - 1)
-    return s + i * ITEM_COST
+        return i * (L + ITEM_COST)
+    n, base = -(-q // (2 * T)), max(L - q, 0) + ITEM_COST
+    full = i if i < n else max(n - 1, 0)
+    s = full * base + T * full * (full + 1)
+    return s + base + q if i > full else s
 
 
-def test_places_in_closed_form():
+def item_at(T, q, L, rem, causal=True):
+    """The kernel's fp32 root and its correction."""
+    f = np.float32
+    n = -(-q // (2 * T))
+    h = f(max(L - q, 0)) + f(ITEM_COST + T)
+    x = (np.sqrt(h * h + f(4) * f(T) * f(rem)) - h) / (f(2) * f(T)) if causal else \
+        f(rem) / f(L + ITEM_COST)
+    i = min(max(int(x), 0), n - 1)
+    steps = 0
+    while i > 0 and places(T, q, L, i, causal) > rem:
+        i, steps = i - 1, steps + 1
+    while i + 1 < n and places(T, q, L, i + 1, causal) <= rem:
+        i, steps = i + 1, steps + 1
+    return i, steps
+
+
+def test_places_in_closed_form_and_the_item_of_a_place():
     import random
     r = random.Random(2)
-    for _ in range(400):
+    for _ in range(300):
         T = r.choice([128, 64, 42, 32, 25, 21, 18, 16, 10, 8])
-        q, past = r.randint(0, 900), r.choice([0, 1, 63, 64, 127, 128, 129, 5000, -3, -400])
+        q, past = r.randint(1, 900), r.choice([0, 1, 63, 64, 127, 128, 129, 5000, -3, -400])
         L = max(0, q + past)
         n = -(-q // (2 * T))
-        for i in range(n + 1):
-            assert places(T, q, L, i) == sum(n_tiles(T, q, L, k) + ITEM_COST for k in range(i))
+        for causal in (True, False):
+            sums = [sum(weight(T, q, L, k, causal) for k in range(i)) for i in range(n + 1)]
+            assert [places(T, q, L, i, causal) for i in range(n + 1)] == sums
+            for _ in range(20):
+                rem = r.randrange(sums[-1])
+                i, steps = item_at(T, q, L, rem, causal)
+                assert sums[i] <= rem < sums[i + 1] and steps <= 2
+    # prompts of millions of tokens: the fp32 root stays within a few items
+    for T, q, past in ((8, 3_000_000, 0), (32, 10_000_000, 5), (128, 1_000_000, 900_000_000)):
+        L, n = q + past, -(-q // (2 * T))
+        for _ in range(50):
+            i = r.randrange(n)
+            rem = places(T, q, L, i) + r.choice([0, 1, 200])
+            got, steps = item_at(T, q, L, rem)
+            assert got == i and steps <= 64, (T, q, past, i, steps)
 
 
-def cut_tile(pos, nt, snap):
-    if pos >= nt + ITEM_COST:
+def cut_tile(pos, w, nt, snap):
+    if pos >= w:
         return nt
-    t = max(pos - ITEM_COST, 0)
+    t = min(max(pos - ITEM_COST + 64, 0) // 128, nt)
     if t < snap and 2 * t < nt:
         return 0
     return nt if nt - t < snap else t
@@ -237,21 +255,27 @@ def prefill_ranges(qs, Ls, T, Hkv, grid, causal=True):
     for b, (q, L) in enumerate(zip(qs, Ls)):
         for h in range(Hkv):
             for i in range(-(-q // (2 * T))):
-                nt = n_tiles(T, q, L, i, causal)
-                items.append(((b, h, i), nt, u))
-                u += nt + ITEM_COST
-    U, nc = u, min(grid, u)
-    snap = min(U // nc // 8, 2) if nc else 0
+                w = weight(T, q, L, i, causal)
+                items.append(((b, h, i), n_tiles(T, q, L, i, causal), u, w))
+                u += w
+    U, nc = u, min(grid, u // 128)
+    share = U // nc if nc else 0
+    rest = U - share * nc
+
+    def cut(k):
+        return share * k + rest * k // nc
+    snap = min(share // 1024, 2)
     pieces, desc, at = [], {}, 0
     for c in range(nc):
-        u0, u1 = U * c // nc, U * (c + 1) // nc
-        while items[at][2] + items[at][1] + ITEM_COST <= u0:
+        u0, u1 = cut(c), cut(c + 1)
+        assert u1 - u0 >= 128
+        while items[at][2] + items[at][3] <= u0:
             at += 1
         k = at
         while k < len(items) and items[k][2] < u1:
-            key, nt, base = items[k]
-            t0 = cut_tile(max(u0 - base, 0), nt, snap)
-            t1 = cut_tile(min(u1 - base, nt + ITEM_COST), nt, snap)
+            key, nt, base, w = items[k]
+            t0 = cut_tile(max(u0 - base, 0), w, nt, snap)
+            t1 = cut_tile(min(u1 - base, w), w, nt, snap)
             if t0 < t1:
                 pieces.append((c, key, t0, t1, nt))
                 if t0 == 0 and t1 < nt:
@@ -260,14 +284,14 @@ def prefill_ranges(qs, Ls, T, Hkv, grid, causal=True):
                         n = 0
                         for lane in range(32):
                             y = x + lane
-                            pos = U * y // nc - base
-                            n += y < nc and cut_tile(pos, nt, snap) < nt
+                            n += y < nc and cut_tile(cut(min(y, nc)) - base, w, nt, snap) < nt
                         last += n
                         if n < 32:
                             break
                         x += 32
                     desc[c] = (key, last)
             k += 1
+    assert not nc or cut(nc) == U
     return pieces, desc, items
 
 
@@ -288,7 +312,7 @@ def test_prefill_division_covers_every_tile_once():
                 pieces, desc, items = prefill_ranges(qs, Ls, T, Hkv, grid, causal)
                 seen = [(k, t) for _, k, t0, t1, _ in pieces for t in range(t0, t1)]
                 assert len(seen) == len(set(seen))
-                assert sorted(seen) == sorted((k, t) for k, nt, _ in items for t in range(nt))
+                assert sorted(seen) == sorted((k, t) for k, nt, *_ in items for t in range(nt))
                 join_check(pieces, desc)
 
 
