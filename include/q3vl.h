@@ -163,8 +163,8 @@ Q3_API int q3_attn_decode_paged(const void* q, const void* k_pages, const void* 
  * in request order, written to its row of block_table behind the pages of its
  * past positions (entries there are taken as empty); with NULL the table
  * already maps every position.  free_start (int32 [1] on the device, or NULL: 0)
- * is the list's first entry that no earlier call has taken; it is only read (a
- * step adds counts[1] to it).  Outputs: cu_q int32 [B + 1] first packed token
+ * is the list's first entry that no earlier call has taken, clamped to 0 ..
+ * n_free; it is only read (a step adds counts[1] to it).  Outputs: cu_q int32 [B + 1] first packed token
  * of each request; kv_lens int32 [B] = past + q; counts int32 [2] = {packed
  * tokens, pages taken}; for each of n_tokens packed rows requests int32,
  * positions int64 (cache position + rope_delta[b], rope_delta int64 [B] or
@@ -177,9 +177,10 @@ Q3_API int q3_attn_decode_paged(const void* q, const void* k_pages, const void* 
 Q3_API int q3_ragged_plan(const int32_t* q_lens, const int32_t* past_lens, int B,
                           int32_t* block_table, int64_t table_stride, int table_width,
                           int page_tokens, const int32_t* free_pages, int n_free,
-                          const int32_t* free_start, const int64_t* rope_delta, int64_t n_tokens, int32_t* cu_q,
-                          int32_t* kv_lens, int32_t* requests, int64_t* positions, int64_t* slots,
-                          int32_t* counts, q3_stream_t stream);
+                          const int32_t* free_start, const int64_t* rope_delta,
+                          int64_t n_tokens, int32_t* cu_q, int32_t* kv_lens, int32_t* requests,
+                          int64_t* positions, int64_t* slots, int32_t* counts,
+                          q3_stream_t stream);
 
 /* Per-head QK-RMSNorm, rotary positions and the K/V write of packed tokens
  * (model_fused.py:107-129, :244-246; M-RoPE of transformers 5.5.0
@@ -191,7 +192,8 @@ Q3_API int q3_ragged_plan(const int32_t* q_lens, const int32_t* past_lens, int B
  * go to position slots[i] % page_tokens of page slots[i] / page_tokens.  fp32
  * throughout with one rounding at the end (angles reduced in fp64).  A token
  * whose slot is -1 is padding: nothing of it is written.  A slot outside the
- * pool is recorded (0x911) and its token skipped. */
+ * pool is recorded (0x911) and its token skipped.  q_out may be qkv itself (the
+ * q part of its rows). */
 Q3_API int q3_qkv_norm_rope_ragged(const void* qkv, int64_t qkv_stride, const void* q_norm_w,
                                    const void* k_norm_w, const int64_t* positions,
                                    int64_t pos_axis_stride, const float* inv_freq,
@@ -203,7 +205,7 @@ Q3_API int q3_qkv_norm_rope_ragged(const void* qkv, int64_t qkv_stride, const vo
 /* Attention of one new token per request (model_fused.py:248-262 at S = 1):
  * q, out bf16 [B, Hq, 128] with row strides (elements; out_stride a multiple
  * of 8); request b attends to positions [0, kv_lens[b]) (int32 [B] on the
- * device); kv_lens[b] = 0 gives zeros.  Hq / Hkv <= 16.  Rows of the pools at
+ * device); kv_lens[b] = 0 gives zeros; out may be q itself.  Hq / Hkv <= 16.  Rows of the pools at
  * or past kv_lens[b] may hold anything, NaN included.  The work is divided
  * over the SMs by length on the device; partial results meet in the workspace
  * (q3_attn_decode_ragged_workspace_bytes, 16-byte aligned; no state is kept in
@@ -224,7 +226,8 @@ Q3_API int q3_attn_decode_ragged(const void* q, int64_t q_stride, const void* k_
  * ascending, cu_q[0] need not be 0), its query i sits at position kv_lens[b] -
  * q_len + i and, with causal != 0, sees positions up to its own; otherwise all
  * kv_lens[b].  A query that sees nothing gives zeros; rows outside
- * [cu_q[0], cu_q[B]) are not written.  Hq / Hkv <= 16, scale > 0.  Rows of the
+ * [cu_q[0], cu_q[B]) are not written; out may be q itself.  Hq / Hkv <= 16,
+ * scale > 0.  Rows of the
  * pools at or past kv_lens[b] may hold anything; rows before it must be finite
  * (a masked key of the same request still meets a zero probability).  Workspace
  * as for q3_attn_decode_ragged.  Lengths outside the table or the packed rows

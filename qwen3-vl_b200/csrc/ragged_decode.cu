@@ -532,8 +532,10 @@ __global__ void __launch_bounds__(kJoinWarps * 32) ragged_decode_join(RaggedDeco
     const int64_t piece = (int64_t)(i == 0 ? 2 * c + 1 : 2 * (c + i)) * p.G + row;
     const float2 ml = *reinterpret_cast<const float2*>(p.ws_ml + piece * 2);
     const float4 x = *reinterpret_cast<const float4*>(p.ws_acc + piece * kD + lane * 4);
-    const float m_new = fmaxf(M, ml.x);  // a piece has at least one position: finite
-    const float f0 = ex2_approx(M - m_new), f1 = ex2_approx(ml.x - m_new);
+    const float m_new = fmaxf(M, ml.x);
+    // -inf where every score of the pieces so far passed fp32's lowest value
+    const float base = m_new == -INFINITY ? 0.f : m_new;
+    const float f0 = ex2_approx(M - base), f1 = ex2_approx(ml.x - base);
     M = m_new;
     l = fmaf(f1, ml.y, l * f0);
     a.x = fmaf(f1, x.x, a.x * f0);

@@ -194,9 +194,10 @@ __global__ void __launch_bounds__(kPlanThreads) ragged_plan_kernel(PlanParams p)
 extern "C" int q3_ragged_plan(const int32_t* q_lens, const int32_t* past_lens, int B,
                               int32_t* block_table, int64_t table_stride, int table_width,
                               int page_tokens, const int32_t* free_pages, int n_free,
-                              const int32_t* free_start, const int64_t* rope_delta, int64_t n_tokens, int32_t* cu_q,
-                              int32_t* kv_lens, int32_t* requests, int64_t* positions,
-                              int64_t* slots, int32_t* counts, q3_stream_t stream) {
+                              const int32_t* free_start, const int64_t* rope_delta,
+                              int64_t n_tokens, int32_t* cu_q, int32_t* kv_lens,
+                              int32_t* requests, int64_t* positions, int64_t* slots,
+                              int32_t* counts, q3_stream_t stream) {
   using namespace q3;
   Q3_REQUIRE(cu_q && counts && (n_tokens == 0 || (requests && positions && slots)) &&
                  (B == 0 || (q_lens && past_lens && block_table && kv_lens)),
@@ -215,8 +216,8 @@ extern "C" int q3_ragged_plan(const int32_t* q_lens, const int32_t* past_lens, i
   Q3_REQUIRE(n_free >= 0 && (free_pages || (n_free == 0 && !free_start)),
              "q3_ragged_plan: free list");
   Q3_REQUIRE(aligned(q_lens, 4) && aligned(past_lens, 4) && aligned(block_table, 4) &&
-                 aligned(free_pages, 4) && aligned(free_start, 4) && aligned(rope_delta, 8) && aligned(cu_q, 4) &&
-                 aligned(kv_lens, 4) && aligned(requests, 4) && aligned(positions, 8) &&
+                 aligned(free_pages, 4) && aligned(free_start, 4) && aligned(rope_delta, 8) &&
+                 aligned(cu_q, 4) && aligned(kv_lens, 4) && aligned(requests, 4) && aligned(positions, 8) &&
                  aligned(slots, 8) && aligned(counts, 4),
              "q3_ragged_plan: misaligned pointer");
   const size_t smem = (size_t)2 * (B + 1) * sizeof(int32_t);
@@ -226,8 +227,7 @@ extern "C" int q3_ragged_plan(const int32_t* q_lens, const int32_t* past_lens, i
                                        2 * (kPlanMaxB + 1) * (int)sizeof(int32_t)));
   const int64_t want = (max64(n_tokens, B + 1) + kPlanThreads - 1) / kPlanThreads;
   PlanParams p{q_lens, past_lens, block_table, table_stride, free_pages, free_start, rope_delta,
-               cu_q,
-               kv_lens, requests, positions, slots, counts, n_tokens, B, table_width,
+               cu_q, kv_lens, requests, positions, slots, counts, n_tokens, B, table_width,
                page_tokens, n_free, device_error_word()};
   return launch_ex(ragged_plan_kernel, dim3((unsigned)min64(want, num_sms())),
                    dim3(kPlanThreads), smem, (cudaStream_t)stream, 1, p);

@@ -1177,9 +1177,9 @@ def qkv_norm_rope_ragged(qkv: torch.Tensor, q_norm_w: torch.Tensor, k_norm_w: to
     qkv bf16 [n, (Hq + 2 Hkv) * 128]; positions int64 [n] (text) or [3, n]
     (time, height, width, interleaved by mrope_section); inv_freq f32 [64];
     slots int64 [n] (RaggedPlan.slots; distinct, or -1 for a padding token, of
-    which nothing is written).  Returns q [n, Hq, 128].  Computed in
-    fp32 and rounded once, without the bf16 tables and rounding points of
-    qkv_norm_rope, so the last bit of a value may differ from it."""
+    which nothing is written).  Returns q [n, Hq, 128]; out may be the q part of
+    qkv.  Computed in fp32 and rounded once, without the bf16 tables and rounding
+    points of qkv_norm_rope, so the last bit of a value may differ from it."""
     name = "qkv_norm_rope_ragged"
     dev = _ragged_device(name, qkv, q_norm_w, k_norm_w, positions, inv_freq, slots, k_pages,
                          v_pages, out)
@@ -1228,11 +1228,12 @@ def attn_decode_ragged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Te
     q bf16 [B, Hq, 128] (any row stride); k_pages / v_pages [num_pages, Hkv,
     page_tokens, 128]; block_table int32 [B, width]; kv_lens int32 [B] on the
     device: request b attends to positions [0, kv_lens[b]), and a length of 0
-    gives zeros.  Hq / Hkv is any whole number up to 16."""
+    gives zeros.  Hq / Hkv is any whole number up to 16; out may be q."""
     name = "attn_decode_ragged"
-    B, Hq = q.shape[0], q.shape[1]
+    B = q.shape[0] if q.dim() else 0
     dev, q_stride, table_stride, out, out_stride = _ragged_attn(name, q, k_pages, v_pages,
                                                                 block_table, kv_lens, out, B)
+    Hq = q.shape[1]
     num_pages, Hkv, page_tokens, D = k_pages.shape
     nbytes = _lib.raw("q3_attn_decode_ragged_workspace_bytes")(Hq, Hkv)
     ws = q.new_empty(nbytes, dtype=torch.uint8)
@@ -1255,7 +1256,8 @@ def attn_prefill_ragged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.T
     kv_lens[b] - 1; with causal each query sees positions up to its own.  Rows of
     out outside [cu_q[0], cu_q[B]) are not written, so a part of a batch goes
     through slices of cu_q, kv_lens and block_table.  A query that sees nothing
-    gives zeros.  Hq / Hkv is any whole number up to 16; scale is positive."""
+    gives zeros.  Hq / Hkv is any whole number up to 16; scale is positive; out
+    may be q."""
     name = "attn_prefill_ragged"
     B = kv_lens.numel()
     dev, q_stride, table_stride, out, out_stride = _ragged_attn(name, q, k_pages, v_pages,

@@ -433,6 +433,48 @@ def test_prefill_in_a_graph_with_new_lengths():
 
 
 # ------------------------------------------------------- the operators together
+def test_scores_below_the_lowest_fp32_value():
+    """Keys whose scores pass fp32 count for nothing, whole pieces of them too."""
+    L, hidden, Hq, Hkv, page = 30000, 20032, 4, 1, 64
+    q, k, v, table = decode_case([L], Hq, Hkv, page, seed=5)
+    q.fill_(1e20)                                   # products of -1e40
+    k[table[0][:hidden // page]] = -1e20
+    for j, pg in enumerate(table[0][hidden // page:]):
+        k[pg, :, :min(page, L - hidden - j * page)] = 0.0
+    want, tol = ora.attention(q, k, v, [table[0][hidden // page:]], [L - hidden], [1])
+    args = (q.to(DEV), k.to(DEV), v.to(DEV), i32(table))
+    ora.check("decode", ops.attn_decode_ragged(*args, i32([L])), want, tol)
+    ora.check("prefill", ops.attn_prefill_ragged(*args, i32([0, 1]), i32([L])), want, tol)
+    # nothing but such keys and one plain one at the end
+    want = v[table[0][hidden // page], :, :1].double().expand(1, Hq, 128)
+    tol = 2 * ora.BF16_HALF * want.abs() + 1e-30
+    ora.check("decode", ops.attn_decode_ragged(*args, i32([hidden + 1])), want, tol)
+
+
+def test_results_in_place_of_q():
+    q_lens, pasts, Hq, Hkv, page = [70, 1, 300], [5, 900, 64], 8, 2, 64
+    q, k, v, table, cu, lens = prefill_case(q_lens, pasts, Hq, Hkv, page, seed=6)
+    rest = (k.to(DEV), v.to(DEV), i32(table))
+    buf = q.to(DEV)
+    want = ops.attn_prefill_ragged(buf, *rest, i32(cu), i32(lens))
+    got = ops.attn_prefill_ragged(buf, *rest, i32(cu), i32(lens), out=buf)
+    assert got is buf and torch.equal(got, want)
+    buf = q[:3].to(DEV)
+    want = ops.attn_decode_ragged(buf, *rest, i32(lens))
+    assert torch.equal(ops.attn_decode_ragged(buf, *rest, i32(lens), out=buf), want)
+    # the q part of packed qkv rows, heads of a token shared by several warps
+    Hq, Hkv = 32, 8
+    qkv = rnd(9, (Hq + 2 * Hkv) * 128, seed=7).to(DEV)
+    w = torch.ones(128, dtype=BF16, device=DEV)
+    pools = torch.zeros(4, 1, Hkv, 64, 128, dtype=BF16, device=DEV)
+    pos = torch.arange(9, device=DEV)
+    args = (w, w, pos, INV.to(DEV), pos)
+    want = ops.qkv_norm_rope_ragged(qkv, *args, pools[0], pools[1], Hq=Hq, Hkv=Hkv)
+    part = qkv.view(9, Hq + 2 * Hkv, 128)[:, :Hq]
+    ops.qkv_norm_rope_ragged(qkv, *args, pools[2], pools[3], Hq=Hq, Hkv=Hkv, out=part)
+    assert torch.equal(part, want) and torch.equal(pools[:2], pools[2:])
+
+
 def test_plan_continues_the_free_list():
     t = i32([[4, -1, -1], [5, -1, -1]])
     free, start = i32([9, 8, 7, 6]), i32([0])
@@ -633,6 +675,8 @@ def test_wrapper_refusals():
     bad(ValueError, d, a[0], a[1], a[2][:1], a[3], kv)
     bad(ValueError, d, a[0], a[1].transpose(0, 1), a[2].transpose(0, 1), a[3], kv)
     bad(ValueError, d, a[0][..., :64], *a[1:], kv)
+    bad(ValueError, d, a[0].flatten(), *a[1:], kv)
+    bad(ValueError, pf, a[0].flatten(), *a[1:], cu, kv)
     bad(ValueError, d, a[0].transpose(1, 2).contiguous().transpose(1, 2), *a[1:], kv)
     bad(ValueError, d, *a, kv, out=torch.empty(2, 4, 128, dtype=BF16, device=DEV))
     bad(TypeError, d, *a, kv, out=torch.empty(2, 8, 128, device=DEV))
