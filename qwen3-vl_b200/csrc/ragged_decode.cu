@@ -18,8 +18,7 @@
 // (32 requests of 257 to 32768 positions or one of 700), where one CTA or one
 // fixed number of splits per pair leaves SMs idle behind the longest request.
 // A pair inside one CTA is written directly; the pieces of a pair that spans
-// CTAs go to the workspace in fp32 and a second kernel joins them in CTA order
-// (the same order every time).  The second kernel costs about 2 us; the
+// CTAs go to the workspace in fp32 and a second kernel joins them in a fixed order.  The second kernel costs about 2 us; the
 // last-arriving-CTA join that would save it was slower in attn_decode.cu, and
 // its counters would tie the workspace to one stream.
 //
@@ -71,8 +70,11 @@ struct RaggedDecodeParams {
   const int32_t* kv_lens;
   float* ws_acc;   // [2 * grid][G][128] unnormalised pieces
   float* ws_ml;    // [2 * grid][G][2]   running max (log2 units) and sum
-  int2* ws_desc;   // [grid] {pair whose first piece ends CTA c's range or -1, last CTA of it}
-  int B, Hkv, G, page_tokens, num_pages, capacity;
+  // [grid] of the pair that goes on behind CTA c's range: {the pair, its last CTA};
+  // of one that began before it, if the split join will look: {-2 - (its first CTA),
+  // its last CTA}; else {-1, -1}
+  int2* ws_desc;
+  int B, Hkv, G, page_tokens, num_pages, capacity, split;
   float scale_log2;
   int* err;
 };
@@ -298,17 +300,23 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
       }
-      if (w.t0 == 0 && w.t1 < w.nt) {
-        // the pair goes on in the next CTAs: the last is the one with its last
-        // tile, the largest k with cut(k) <= that tile
-        int last = c;
-        for (uint32_t k0 = c + 1; k0 < nc; k0 += 32) {
-          const uint32_t k = k0 + lane;
-          const int n = __popc(__ballot_sync(0xffffffffu, k < nc && cut(k) <= u + w.nt - 1));
-          last += n;
-          if (n < 32) break;
-        }
-        if (lane == 0) p.ws_desc[c] = make_int2(w.b * p.Hkv + w.kvh, last);
+      if (w.t1 < w.nt && (w.t0 == 0 || p.split)) {
+        // the pair goes on in the next CTAs (this is the CTA's last piece): its
+        // first and last CTA have the largest k with cut(k) <= its first, last tile
+        auto holder = [&](int from, int64_t tile) {
+          int at = from;
+          for (uint32_t k0 = from + 1; k0 < nc; k0 += 32) {
+            const uint32_t k = k0 + lane;
+            const int n = __popc(__ballot_sync(0xffffffffu, k < nc && cut(k) <= tile));
+            at += n;
+            if (n < 32) break;
+          }
+          return at;
+        };
+        const int64_t first = u - w.t0;
+        const int last = holder(c, first + w.nt - 1);
+        const int id = w.t0 == 0 ? w.b * p.Hkv + w.kvh : -2 - holder(0, first);
+        if (lane == 0) p.ws_desc[c] = make_int2(id, last);
       }
       u += w.t1 - w.t0;
     }
@@ -511,24 +519,98 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// Joins the pieces of the pair whose first piece ends CTA c's range: pieces
-// 2c+1, 2(c+1), 2(c+2), ..., 2*last.  One CTA per (c, query head of the pair).
-constexpr int kJoinWarps = 8;
 constexpr int kMaxGrid = 512;
-__global__ void __launch_bounds__(kJoinWarps * 32) ragged_decode_join(RaggedDecodeParams p) {
-  __shared__ float2 s_ml[kJoinWarps];
-  __shared__ __align__(16) float s_acc[kJoinWarps][kD];
+// Few long requests leave pairs of up to a piece per SM, which one CTA would take
+// warp by warp.  Above kFewPieces the CTAs of a pair's first kJoinParts CTAs take 16
+// dims each and a warp eight pieces at a time.  Launched (SPLIT) for up to a pair per
+// 8 SMs when the table can hold more than kFewPieces tiles: one request of 3000,
+// 8000, 30000 positions, 4/1 heads, 7.0, 9.5, 11.7 -> 5.9, 7.1, 8.7 us, two of 11312,
+// 6/1, 12.2 -> 8.4; one of 700, with few pieces all the same, 5.4 -> 5.5.  Twelve
+// requests of 3000 have 13 pieces a pair: 8.1 us without the split, 8.8 with it.
+constexpr int kFewPieces = 16;
+constexpr int kJoinParts = 8;
+template <int W>
+__device__ __forceinline__ void join_many(const RaggedDecodeParams& p, int c0, int n, int part,
+                                          int row) {
+  __shared__ float2 s_ml[W];
+  __shared__ float s_acc[W][kD / kJoinParts];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, d0 = part * (kD / kJoinParts);
+  float M = -INFINITY, l = 0.f;
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
+  for (int i = warp * 8 + (lane >> 2); i < n; i += W * 8) {
+    const int64_t piece = (int64_t)(i == 0 ? 2 * c0 + 1 : 2 * (c0 + i)) * p.G + row;
+    const float2 ml = *reinterpret_cast<const float2*>(p.ws_ml + piece * 2);
+    const float4 x =
+        *reinterpret_cast<const float4*>(p.ws_acc + piece * kD + d0 + (lane & 3) * 4);
+    const float m_new = fmaxf(M, ml.x);
+    const float base = m_new == -INFINITY ? 0.f : m_new;
+    const float f0 = ex2_approx(M - base), f1 = ex2_approx(ml.x - base);
+    M = m_new;
+    l = fmaf(f1, ml.y, l * f0);
+    a.x = fmaf(f1, x.x, a.x * f0);
+    a.y = fmaf(f1, x.y, a.y * f0);
+    a.z = fmaf(f1, x.z, a.z * f0);
+    a.w = fmaf(f1, x.w, a.w * f0);
+  }
+#pragma unroll
+  for (int o = 4; o < 32; o <<= 1) {  // the lanes that hold the same dims
+    const float m_new = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    const float f = ex2_approx(M - (m_new == -INFINITY ? 0.f : m_new));
+    M = m_new;
+    l *= f;
+    l += __shfl_xor_sync(0xffffffffu, l, o);
+    a = make_float4(a.x * f, a.y * f, a.z * f, a.w * f);
+    a.x += __shfl_xor_sync(0xffffffffu, a.x, o);
+    a.y += __shfl_xor_sync(0xffffffffu, a.y, o);
+    a.z += __shfl_xor_sync(0xffffffffu, a.z, o);
+    a.w += __shfl_xor_sync(0xffffffffu, a.w, o);
+  }
+  if (lane < 4) *reinterpret_cast<float4*>(&s_acc[warp][lane * 4]) = a;
+  if (lane == 0) s_ml[warp] = make_float2(M, l);
+  __syncthreads();
+  if (threadIdx.x < kD / kJoinParts) {
+    float Ma = -INFINITY;
+    for (int i = 0; i < W; ++i) Ma = fmaxf(Ma, s_ml[i].x);
+    float x = 0.f, ls = 0.f;
+    for (int i = 0; i < W; ++i) {
+      const float f = s_ml[i].x == -INFINITY ? 0.f : ex2_approx(s_ml[i].x - Ma);
+      x = fmaf(f, s_acc[i][threadIdx.x], x);
+      ls = fmaf(f, s_ml[i].y, ls);
+    }
+    const int pair = p.ws_desc[c0].x, b = pair / p.Hkv, kvh = pair - b * p.Hkv;
+    p.out[b * p.out_stride + (int64_t)(kvh * p.G + row) * kD + d0 + threadIdx.x] = f2bf(x / ls);
+  }
+}
+// Joins the pieces of the pair whose first piece ends CTA c's range: pieces
+// 2c+1, 2(c+1), 2(c+2), ..., 2*last.  One CTA per (c, query head of the pair), of
+// four warps with more than 8 heads per K/V head, so that more of the grid waits on
+// the SMs beside the first kernel (3 short requests at 32/2 heads 7.6 -> 6.8 us; 16
+// long ones at 24/2 20.0 -> 20.6), and for the same reason it is kept to 32 registers
+// (with 40 the case of 32 long requests took 143 us for 140).
+template <int W, bool SPLIT>  // warps
+__global__ void __launch_bounds__(W * 32) ragged_decode_join(RaggedDecodeParams p) {
+  __shared__ float2 s_ml[W];
+  __shared__ __align__(16) float s_acc[W][kD];
   pdl_launch();
   pdl_wait();
   const int c = blockIdx.x, row = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int2 d = p.ws_desc[c];
-  if (d.x < 0) return;
+  if (SPLIT ? d.x == -1 : d.x < 0) return;
+  if constexpr (SPLIT) {
+    const int c0 = d.x < 0 ? -2 - d.x : c;
+    if (d.y - c0 + 1 > kFewPieces) {
+      if (c - c0 < kJoinParts) join_many<W>(p, c0, d.y - c0 + 1, c - c0, row);
+      return;
+    }
+    if (c != c0) return;
+  }
   const int n = d.y - c + 1;  // pieces, at most the first kernel's grid
   // a warp's pieces against a running maximum, then the warps'
   float M = -INFINITY, l = 0.f;
   float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-  for (int i = warp; i < n; i += kJoinWarps) {
+  for (int i = warp; i < n; i += W) {
     const int64_t piece = (int64_t)(i == 0 ? 2 * c + 1 : 2 * (c + i)) * p.G + row;
     const float2 ml = *reinterpret_cast<const float2*>(p.ws_ml + piece * 2);
     const float4 x = *reinterpret_cast<const float4*>(p.ws_acc + piece * kD + lane * 4);
@@ -549,10 +631,10 @@ __global__ void __launch_bounds__(kJoinWarps * 32) ragged_decode_join(RaggedDeco
   if (threadIdx.x < kD) {
     float Ma = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < kJoinWarps; ++i) Ma = fmaxf(Ma, s_ml[i].x);
+    for (int i = 0; i < W; ++i) Ma = fmaxf(Ma, s_ml[i].x);
     float x = 0.f, ls = 0.f;
 #pragma unroll
-    for (int i = 0; i < kJoinWarps; ++i) {
+    for (int i = 0; i < W; ++i) {
       const float f = s_ml[i].x == -INFINITY ? 0.f : ex2_approx(s_ml[i].x - Ma);
       x = fmaf(f, s_acc[i][threadIdx.x], x);
       ls = fmaf(f, s_ml[i].y, ls);
@@ -629,10 +711,12 @@ extern "C" int q3_attn_decode_ragged(const void* q, int64_t q_stride, const void
   rc = make_tmap_2d(&tv, v_pages, rows, kD, kTile, 64);
   if (rc) return rc;
   uint8_t* ws = (uint8_t*)workspace;
+  const int split = (int64_t)B * Hkv * 8 <= decode_grid() &&
+                    (int64_t)table_width * page_tokens > kFewPieces * kTile;
   RaggedDecodeParams p{(const __nv_bfloat16*)q, q_stride, (__nv_bfloat16*)out, out_stride,
                        block_table, table_stride, kv_lens, (float*)ws, (float*)(ws + off_ml),
                        (int2*)(ws + off_desc), B, Hkv, G, page_tokens, (int)num_pages,
-                       table_width * page_tokens, scale * 1.4426950408889634f,
+                       table_width * page_tokens, split, scale * 1.4426950408889634f,
                        device_error_word()};
   static bool attr_set[64] = {false};
   int dev = 0;
@@ -652,6 +736,8 @@ extern "C" int q3_attn_decode_ragged(const void* q, int64_t q_stride, const void
              : launch_ex(ragged_decode_kernel<false>, grid, dim3(kThreads), Cfg<false>::kSmem,
                          (cudaStream_t)stream, 1, tk, tv, p);
   if (rc) return rc;
-  return launch_ex(ragged_decode_join, dim3(grid.x, (unsigned)G), dim3(kJoinWarps * 32), 0,
+  auto join = G > 8 ? (split ? ragged_decode_join<4, true> : ragged_decode_join<4, false>)
+                    : (split ? ragged_decode_join<8, true> : ragged_decode_join<8, false>);
+  return launch_ex(join, dim3(grid.x, (unsigned)G), dim3(G > 8 ? 128 : 256), 0,
                    (cudaStream_t)stream, 1, p);
 }

@@ -215,7 +215,8 @@ def decode_case(lens, Hq, Hkv, page, seed=0, stale=math.nan, std=1.5, **kw):
     ([1000, 17], 3, 1, 192), ([130, 4097, 64], 10, 2, 128), ([257, 1], 16, 2, 64),
     ([1500, 66, 0], 16, 1, 64), ([900, 31], 24, 2, 256), ([40, 2000], 9, 1, 64),
     ([5] * 300, 8, 2, 64), ([0] * 40 + [3000] + [0] * 40 + [1], 8, 4, 64),
-    ([30000], 4, 1, 256), ([0, 0, 0], 8, 2, 64)])
+    ([30000], 4, 1, 256), ([0, 0, 0], 8, 2, 64), ([9000, 100, 0, 2500], 12, 1, 64),
+    ([1100], 2, 1, 64), ([3] * 17 + [20000], 1, 1, 128), ([7000, 1, 9000], 16, 2, 64)])
 def test_decode(lens, Hq, Hkv, page):
     q, k, v, table = decode_case(lens, Hq, Hkv, page, seed=len(lens))
     want, tol = ora.attention(q, k, v, table, lens, [1] * len(lens))

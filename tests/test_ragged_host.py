@@ -124,7 +124,7 @@ def decode_ranges(lens, Hkv, grid):
     units = [(b * Hkv + h, t, n) for b, n in enumerate(tiles) for h in range(Hkv) for t in range(n)]
     U = len(units)
     nc = min(grid, U)
-    out, desc = [], {}
+    out, desc, owner = [], {}, {}
     for c in range(nc):
         u = u0 = U * c // nc
         u1 = U * (c + 1) // nc
@@ -134,6 +134,13 @@ def decode_ranges(lens, Hkv, grid):
             out.append((c, pair, t0, t1, n))
             if t0 == 0 and t1 < n:
                 desc[c] = (pair, ((u + n) * nc - 1) // U)
+                owner[pair] = c
+            elif t1 < n:
+                # what the split join reads in the CTAs between: the pair's first
+                # CTA (the largest k with cut(k) <= its first tile) and its last
+                first = u - t0
+                assert owner[pair] == ((first + 1) * nc - 1) // U
+                assert desc[owner[pair]] == (pair, ((first + n) * nc - 1) // U)
             u += t1 - t0
         assert u == u1 and u0 <= u1
     return out, desc
