@@ -29,11 +29,13 @@
 // per key, which an average over keys shrinks below the bf16 rounding of the
 // output; the sum l takes the unrounded p).
 // Measured on B200: 32 requests of 257 to 32768 positions, 32/8 heads, 885 MB:
-// 140 us, 6.3 TB/s (0.98 of a copy; with eight consumer warps 149, their merge
-// and registers cost more than they gave); 8 requests in a 2048 bucket 10.2 us;
-// one request of 700 positions, 4/1 heads, 5.6 us, about half of it the chain
-// lengths -> table -> first tile and the join.
+// 133 us, 6.7 TB/s (1.03 of a copy, which also writes; two tiles a step: with one
+// 140, and then with eight consumer warps 149); 8 requests in a 2048 bucket 10.2 us,
+// of which the 24 MB take 3.5; one request of 700 positions, 4/1 heads, 5.6 us,
+// about half of it the chain lengths -> table -> first tile and 2 us the join.
 #include <math.h>
+
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -355,37 +357,55 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int e = 0; e < (WIDE ? 4 : 2); ++e) o[i][e] = 0.f;
       float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 
-      for (int t = w.t0; t < w.t1; ++t, ++it) {
-        const int s = it % C::kStages;
-        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&full[s], (it / C::kStages) & 1, p.err, 0x924));
-        if (!ok) continue;
-        const uint32_t sK = ring + s * kStage, sV = sK + 2 * kHalf;
-        const int pos0 = t * kTile + band * 16;
-        // ---- S = Q K^T: 16 rows x 16 positions (two n-tiles of 8) ----
-        float sc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+      // NT tiles in one step: two are independent work for a warp that has its
+      // scheduler to itself
+      auto step = [&](auto nt_c, int t) {
+        constexpr int NT = decltype(nt_c)::value;
+        uint32_t sK[NT];
 #pragma unroll
-        for (int ks = 0; ks < 8; ++ks) {
-          uint32_t kf[4];
-          const int r = band * 16 + (lane & 7) + ((lane >> 4) << 3);
-          ldsm4(kf, sK + kv_at(r, ks * 2 + ((lane >> 3) & 1)));
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            if constexpr (WIDE)
-              mma_bf16_16816(sc[j], qf[ks][0], qf[ks][1], qf[ks][2], qf[ks][3], kf[2 * j],
-                             kf[2 * j + 1]);
-            else
-              mma_bf16_16816(sc[j], qf[ks][0], 0u, qf[ks][1], 0u, kf[2 * j], kf[2 * j + 1]);
-          }
+        for (int u = 0; u < NT; ++u) {
+          const int s = (it + u) % C::kStages;
+          if (ok)
+            ok = __all_sync(0xffffffffu,
+                            mbar_wait(&full[s], ((it + u) / C::kStages) & 1, p.err, 0x924));
+          sK[u] = ring + s * kStage;
         }
-        const bool tail = pos0 + 16 > w.L;
+        if (!ok) return;
+        // ---- S = Q K^T: 16 rows x 16 positions of each tile (two n-tiles of 8) ----
+        float sc[NT][2][4];
+#pragma unroll
+        for (int u = 0; u < NT; ++u)
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sc[u][j][e] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < 8; ++ks)
+#pragma unroll
+          for (int u = 0; u < NT; ++u) {
+            uint32_t kf[4];
+            const int r = band * 16 + (lane & 7) + ((lane >> 4) << 3);
+            ldsm4(kf, sK[u] + kv_at(r, ks * 2 + ((lane >> 3) & 1)));
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              if constexpr (WIDE)
+                mma_bf16_16816(sc[u][j], qf[ks][0], qf[ks][1], qf[ks][2], qf[ks][3], kf[2 * j],
+                               kf[2 * j + 1]);
+              else
+                mma_bf16_16816(sc[u][j], qf[ks][0], 0u, qf[ks][1], 0u, kf[2 * j], kf[2 * j + 1]);
+            }
+          }
+        const int pos0 = t * kTile + band * 16;  // of the first tile
+        const bool tail = pos0 + (NT - 1) * kTile + 16 > w.L;
         if (tail) {
           // V rows past the end hold whatever the page held before: 0 * V must
           // be 0, so this warp's rows there become zeros (the ring's next copy
           // into the stage is ordered behind the fence and the release below)
+          const uint32_t sV = sK[NT - 1] + 2 * kHalf;
 #pragma unroll
           for (int i = lane; i < 16 * 16; i += 32) {
             const int r = band * 16 + (i >> 4);
-            if (t * kTile + r >= w.L)
+            if ((t + NT - 1) * kTile + r >= w.L)
               asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(sV + kv_at(r, i & 15)),
                            "r"(0u)
                            : "memory");
@@ -393,18 +413,22 @@ __global__ void __launch_bounds__(kThreads, 1)
           __syncwarp();
         }
         // ---- running max and sum per row; P as the A operand of P V ----
-        uint32_t pa[4] = {0u, 0u, 0u, 0u};
+        uint32_t pa[NT][4];
 #pragma unroll
         for (int hh = 0; hh < (WIDE ? 2 : 1); ++hh) {
-          float x[4];
+          float x[NT][4];
+          float mx = -INFINITY;
 #pragma unroll
-          for (int j = 0; j < 2; ++j)
+          for (int u = 0; u < NT; ++u) {
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int pos = pos0 + j * 8 + 2 * t4 + e;
-              x[j * 2 + e] = pos < w.L ? sc[j][hh * 2 + e] * p.scale_log2 : -INFINITY;
-            }
-          float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const int pos = pos0 + u * kTile + j * 8 + 2 * t4 + e;
+                x[u][j * 2 + e] = pos < w.L ? sc[u][j][hh * 2 + e] * p.scale_log2 : -INFINITY;
+              }
+            mx = fmaxf(mx, fmaxf(fmaxf(x[u][0], x[u][1]), fmaxf(x[u][2], x[u][3])));
+          }
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
           const float m_new = fmaxf(m[hh], mx);
@@ -412,9 +436,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           const float corr = ex2_approx(m[hh] - base);
           float rs = 0.f;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            x[e] = ex2_approx(x[e] - base);
-            rs += x[e];
+          for (int u = 0; u < NT; ++u) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              x[u][e] = ex2_approx(x[u][e] - base);
+              rs += x[u][e];
+            }
+            pa[u][hh] = pack_bf16x2(x[u][0], x[u][1]);
+            pa[u][2 + hh] = pack_bf16x2(x[u][2], x[u][3]);
           }
           l[hh] = l[hh] * corr + rs;
           m[hh] = m_new;
@@ -423,31 +452,40 @@ __global__ void __launch_bounds__(kThreads, 1)
             o[d][hh * 2] *= corr;
             o[d][hh * 2 + 1] *= corr;
           }
-          pa[hh] = pack_bf16x2(x[0], x[1]);
-          pa[2 + hh] = pack_bf16x2(x[2], x[3]);
         }
         // ---- O += P V ----
 #pragma unroll
-        for (int ip = 0; ip < 8; ++ip) {
-          uint32_t vf[4];
-          const int r = band * 16 + (lane & 7) + (((lane >> 3) & 1) << 3);
-          ldsm4t(vf, sV + kv_at(r, ip * 2 + (lane >> 4)));
+        for (int ip = 0; ip < 8; ++ip)
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            float(&oo)[WIDE ? 4 : 2] = o[2 * ip + j];
-            if constexpr (WIDE) {
-              mma_bf16_16816(oo, pa[0], pa[1], pa[2], pa[3], vf[2 * j], vf[2 * j + 1]);
-            } else {
-              float d4[4] = {oo[0], oo[1], 0.f, 0.f};
-              mma_bf16_16816(d4, pa[0], 0u, pa[2], 0u, vf[2 * j], vf[2 * j + 1]);
-              oo[0] = d4[0];
-              oo[1] = d4[1];
+          for (int u = 0; u < NT; ++u) {
+            uint32_t vf[4];
+            const int r = band * 16 + (lane & 7) + (((lane >> 3) & 1) << 3);
+            ldsm4t(vf, sK[u] + 2 * kHalf + kv_at(r, ip * 2 + (lane >> 4)));
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              float(&oo)[WIDE ? 4 : 2] = o[2 * ip + j];
+              if constexpr (WIDE) {
+                mma_bf16_16816(oo, pa[u][0], pa[u][1], pa[u][2], pa[u][3], vf[2 * j],
+                               vf[2 * j + 1]);
+              } else {
+                float d4[4] = {oo[0], oo[1], 0.f, 0.f};
+                mma_bf16_16816(d4, pa[u][0], 0u, pa[u][2], 0u, vf[2 * j], vf[2 * j + 1]);
+                oo[0] = d4[0];
+                oo[1] = d4[1];
+              }
             }
           }
-        }
         if (tail) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
-        if (lane == 0) mbar_arrive(&empty[s]);
+        if (lane == 0)
+#pragma unroll
+          for (int u = 0; u < NT; ++u) mbar_arrive(&empty[(it + u) % C::kStages]);
+      };
+      int t = w.t0;
+      for (; t + 1 < w.t1; t += 2, it += 2) step(std::integral_constant<int, 2>(), t);
+      if (t < w.t1) {
+        step(std::integral_constant<int, 1>(), t);
+        ++it;
       }
 
       // ---- merge the warps; write the output or this CTA's piece ----
@@ -587,7 +625,7 @@ __device__ __forceinline__ void join_many(const RaggedDecodeParams& p, int c0, i
 // four warps with more than 8 heads per K/V head, so that more of the grid waits on
 // the SMs beside the first kernel (3 short requests at 32/2 heads 7.6 -> 6.8 us; 16
 // long ones at 24/2 20.0 -> 20.6), and for the same reason it is kept to 32 registers
-// (with 40 the case of 32 long requests took 143 us for 140).
+// (with 40 the case of 32 long requests took 3 us longer).
 template <int W, bool SPLIT>  // warps
 __global__ void __launch_bounds__(W * 32) ragged_decode_join(RaggedDecodeParams p) {
   __shared__ float2 s_ml[W];
