@@ -1039,6 +1039,18 @@ def _ragged_call(name: str, dev: int, *args) -> None:
         _lib.check(rc, name)
 
 
+_ragged_ws_bytes: dict = {}
+
+
+def _ragged_workspace(q: torch.Tensor, dev: int, name: str, *args):
+    """A call's workspace and its size, which depends on the device and args only."""
+    nbytes = _ragged_ws_bytes.get((dev, name, args))
+    if nbytes is None:
+        with torch.cuda.device(dev):
+            nbytes = _ragged_ws_bytes[dev, name, args] = _lib.raw(name)(*args)
+    return q.new_empty(nbytes, dtype=torch.uint8), nbytes
+
+
 def _ragged_rows(name: str, what: str, t: torch.Tensor) -> int:
     """Row stride of a bf16 [rows, heads, 128] tensor whose rows are dense."""
     rows, heads, d = t.shape
@@ -1235,8 +1247,7 @@ def attn_decode_ragged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Te
                                                                 block_table, kv_lens, out, B)
     Hq = q.shape[1]
     num_pages, Hkv, page_tokens, D = k_pages.shape
-    nbytes = _lib.raw("q3_attn_decode_ragged_workspace_bytes")(Hq, Hkv)
-    ws = q.new_empty(nbytes, dtype=torch.uint8)
+    ws, nbytes = _ragged_workspace(q, dev, "q3_attn_decode_ragged_workspace_bytes", Hq, Hkv)
     _ragged_call("q3_attn_decode_ragged", dev, q.data_ptr(), q_stride, k_pages.data_ptr(),
                  v_pages.data_ptr(), out.data_ptr(), out_stride, B, Hq, Hkv, D,
                  block_table.data_ptr(), table_stride, block_table.shape[1], page_tokens,
@@ -1266,8 +1277,7 @@ def attn_prefill_ragged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.T
     num_pages, Hkv, page_tokens, _ = k_pages.shape
     if cu_q.get_device() != dev:
         raise RuntimeError(f"{name}: cu_q must be on the other tensors' CUDA device")
-    nbytes = _lib.raw("q3_attn_prefill_ragged_workspace_bytes")()
-    ws = q.new_empty(nbytes, dtype=torch.uint8)
+    ws, nbytes = _ragged_workspace(q, dev, "q3_attn_prefill_ragged_workspace_bytes")
     _ragged_call("q3_attn_prefill_ragged", dev, q.data_ptr(), q_stride, k_pages.data_ptr(),
                  v_pages.data_ptr(), out.data_ptr(), out_stride, n, B, Hq, Hkv, D,
                  block_table.data_ptr(), table_stride, block_table.shape[1], page_tokens,

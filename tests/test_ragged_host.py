@@ -378,3 +378,29 @@ def test_calls_run_on_the_tensors_own_device(monkeypatch):
     monkeypatch.setattr(_lib, "raw", lambda name: lambda *a: _lib.Q3_ERR_INVALID)
     with pytest.raises(_lib.Q3Error):
         ops._ragged_call("q3_x", 0, 7)
+
+
+def test_workspace_sizes_are_asked_on_the_tensors_device(monkeypatch):
+    at, asked = [0], []
+
+    class Guard:
+        def __init__(self, dev):
+            self.dev = dev
+
+        def __enter__(self):
+            self.old, at[0] = at[0], self.dev
+
+        def __exit__(self, *a):
+            at[0] = self.old
+
+    def size(*args):
+        asked.append((at[0],) + args)
+        return 64 + at[0]
+    monkeypatch.setattr(torch.cuda, "device", Guard)
+    monkeypatch.setattr(_lib, "raw", lambda name: size)
+    monkeypatch.setattr(ops, "_ragged_ws_bytes", {})
+    q = torch.zeros(1)
+    for dev, args in ((0, (8, 2)), (1, (8, 2)), (0, (8, 2)), (0, (4, 2))):
+        ws, n = ops._ragged_workspace(q, dev, "q3_x", *args)
+        assert n == 64 + dev and ws.dtype == torch.uint8 and ws.numel() == n
+    assert asked == [(0, 8, 2), (1, 8, 2), (0, 4, 2)] and at == [0]
