@@ -34,16 +34,12 @@ SECTION = (24, 20, 20)
 EPS = 1e-6
 
 
-_loaded = []
-
-
 def _ops():
-    """q3vl.ops, imported by the first call (a user's program imports it once)."""
-    if not _loaded:
-        sys.path.insert(0, os.path.abspath("qwen3-vl_b200"))
-        from q3vl import ops
-        _loaded.append(ops)
-    return _loaded[0]
+    path = os.path.abspath("qwen3-vl_b200")
+    if path not in sys.path:
+        sys.path.insert(0, path)
+    from q3vl import ops
+    return ops
 
 
 # --------------------------------------------------------------------------
