@@ -846,7 +846,9 @@ __device__ __forceinline__ float join_sum(const RaggedPrefillParams& p, const Jo
 #pragma unroll
     for (int u = 0; u < kJoinBatch; ++u) {
       const float f = m[u] == -INFINITY ? 0.f : ex2_approx(m[u] - M);
-      if (f == 0.f) continue;  // a piece of which the row sees nothing, or none
+      // a piece of which the row sees nothing, or none; but a NaN score, which no
+      // maximum shows, has made its piece's sum and O NaN, and the row is NaN
+      if (f == 0.f && li[u] == li[u]) continue;
       l = fmaf(f, li[u], l);
 #pragma unroll
       for (int k = 0; k < kJoinD4; ++k) {
