@@ -206,7 +206,9 @@ Q3_API int q3_qkv_norm_rope_ragged(const void* qkv, int64_t qkv_stride, const vo
  * q, out bf16 [B, Hq, 128] with row strides (elements; out_stride a multiple
  * of 8); request b attends to positions [0, kv_lens[b]) (int32 [B] on the
  * device); kv_lens[b] = 0 gives zeros; out may be q itself.  Hq / Hkv <= 16.  Rows of the pools at
- * or past kv_lens[b] may hold anything, NaN included.  The work is divided
+ * or past kv_lens[b] may hold anything, NaN included.  A key whose score passes
+ * fp32's lowest value counts for nothing; a query with no other key gives zeros,
+ * one with a NaN score NaN.  The work is divided
  * over the SMs by length on the device; partial results meet in the workspace
  * (q3_attn_decode_ragged_workspace_bytes, 16-byte aligned; no state is kept in
  * it between calls, but two calls that may overlap need one each).  A length
@@ -225,7 +227,8 @@ Q3_API int q3_attn_decode_ragged(const void* q, int64_t q_stride, const void* k_
  * request b owns rows cu_q[b] .. cu_q[b+1] - 1 (int32 [B + 1] on the device,
  * ascending, cu_q[0] need not be 0), its query i sits at position kv_lens[b] -
  * q_len + i and, with causal != 0, sees positions up to its own; otherwise all
- * kv_lens[b].  A query that sees nothing gives zeros; rows outside
+ * kv_lens[b].  A query that sees nothing gives zeros, as does one all of whose
+ * scores pass fp32's lowest value; one with a NaN score gives NaN.  Rows outside
  * [cu_q[0], cu_q[B]) are not written; out may be q itself.  Hq / Hkv <= 16,
  * scale > 0.  Rows of the
  * pools at or past kv_lens[b] may hold anything; rows before it must be finite

@@ -98,6 +98,10 @@ __device__ __forceinline__ uint32_t kv_at(int r, int c) {
   return (c >> 3) * kHalf + r * 128 + (((c & 7) ^ (r & 7)) << 4);
 }
 
+// x / l; 0 where l is 0: every score of the row passed fp32's lowest value, no key
+// counts, and the row is zeros as one that sees no key.  A NaN sum stays NaN.
+__device__ __forceinline__ float over_sum(float x, float l) { return l == 0.f ? 0.f : x / l; }
+
 // Length of request b, inside what its table row can hold.
 __device__ __forceinline__ int req_len(const RaggedDecodeParams& p, int b, bool* bad) {
   const int L = p.kv_lens[b];
@@ -535,7 +539,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           ls = fmaf(f, ml[i].y, ls);
         }
         if (whole) {
-          const float inv = 1.0f / ls;
+          const float inv = over_sum(1.0f, ls);
           *reinterpret_cast<uint2*>(p.out + w.b * p.out_stride +
                                     (int64_t)(w.kvh * p.G + row) * kD + d) =
               make_uint2(pack_bf16x2(a.x * inv, a.y * inv), pack_bf16x2(a.z * inv, a.w * inv));
@@ -617,7 +621,8 @@ __device__ __forceinline__ void join_many(const RaggedDecodeParams& p, int c0, i
       ls = fmaf(f, s_ml[i].y, ls);
     }
     const int pair = p.ws_desc[c0].x, b = pair / p.Hkv, kvh = pair - b * p.Hkv;
-    p.out[b * p.out_stride + (int64_t)(kvh * p.G + row) * kD + d0 + threadIdx.x] = f2bf(x / ls);
+    p.out[b * p.out_stride + (int64_t)(kvh * p.G + row) * kD + d0 + threadIdx.x] =
+        f2bf(over_sum(x, ls));
   }
 }
 // Joins the pieces of the pair whose first piece ends CTA c's range: pieces
@@ -678,7 +683,8 @@ __global__ void __launch_bounds__(W * 32) ragged_decode_join(RaggedDecodeParams 
       ls = fmaf(f, s_ml[i].y, ls);
     }
     const int b = d.x / p.Hkv, kvh = d.x - b * p.Hkv;
-    p.out[b * p.out_stride + (int64_t)(kvh * p.G + row) * kD + threadIdx.x] = f2bf(x / ls);
+    p.out[b * p.out_stride + (int64_t)(kvh * p.G + row) * kD + threadIdx.x] =
+        f2bf(over_sum(x, ls));
   }
 }
 
