@@ -222,6 +222,22 @@ Q3_API int q3_attn_decode_ragged(const void* q, int64_t q_stride, const void* k_
                                  int64_t num_pages, const int32_t* kv_lens, float scale,
                                  void* workspace, size_t workspace_bytes, q3_stream_t stream);
 
+/* The same over packed rows, so that a slot of the batch may be idle in a step:
+ * q, out [n_tokens, Hq, 128], cu_q int32 [B + 1] on the device (q3_ragged_plan).
+ * Request b's row is cu_q[b] when it has exactly one token, cu_q[b + 1] =
+ * cu_q[b] + 1.  One without a token is left out.  One with more tokens, or whose
+ * row lies outside [0, n_tokens), is recorded (0x925) and left out.  Rows of out
+ * that belong to no such request are not written.  (In the call above row b is
+ * request b's, whether it brings a token or not.) */
+Q3_API int q3_attn_decode_ragged_packed(const void* q, int64_t q_stride, const void* k_pages,
+                                        const void* v_pages, void* out, int64_t out_stride,
+                                        int64_t n_tokens, int B, int Hq, int Hkv, int head_dim,
+                                        const int32_t* block_table, int64_t table_stride,
+                                        int table_width, int page_tokens, int64_t num_pages,
+                                        const int32_t* cu_q, const int32_t* kv_lens, float scale,
+                                        void* workspace, size_t workspace_bytes,
+                                        q3_stream_t stream);
+
 /* Attention of packed prompt chunks (model_fused.py:248-262 at S > 1) on
  * tcgen05: q, out bf16 [n_tokens, Hq, 128] with row strides (multiples of 8);
  * request b owns rows cu_q[b] .. cu_q[b+1] - 1 (int32 [B + 1] on the device,

@@ -7,6 +7,8 @@
 //   out[b, h] = softmax(q[b, h] . K_b^T * scale) V_b over positions
 //   [0, kv_lens[b]), K/V head h / (Hq / Hkv), position t in page
 //   table[b, t / page_tokens]; a request of length 0 gives zeros.
+// With cu_q the requests' rows are packed: request b's is cu_q[b], and a request that
+// brings no token in this step has none.
 // One pass with a running maximum and sum (fp32, log2 units):
 //   m' = max(m, s),  l' = l 2^(m-m') + 2^(s-m'),  o' = o 2^(m-m') + 2^(s-m') v.
 //
@@ -72,9 +74,9 @@ struct RaggedDecodeParams {
   const int32_t* kv_lens;
   float* ws_acc;   // [2 * grid][G][128] unnormalised pieces
   float* ws_ml;    // [2 * grid][G][2]   running max (log2 units) and sum
-  // [grid] of the pair that goes on behind CTA c's range: {the pair, its last CTA};
-  // of one that began before it, if the split join will look: {-2 - (its first CTA),
-  // its last CTA}; else {-1, -1}
+  // [grid] of the pair that goes on behind CTA c's range: {its row of out * Hkv + its
+  // K/V head, its last CTA}; of one that began before it, if the split join will
+  // look: {-2 - (its first CTA), its last CTA}; else {-1, -1}
   int2* ws_desc;
   int B, Hkv, G, page_tokens, num_pages, capacity, split;
   float scale_log2;
@@ -102,10 +104,40 @@ __device__ __forceinline__ uint32_t kv_at(int r, int c) {
 // counts, and the row is zeros as one that sees no key.  A NaN sum stays NaN.
 __device__ __forceinline__ float over_sum(float x, float l) { return l == 0.f ? 0.f : x / l; }
 
-// Length of request b, inside what its table row can hold.
-__device__ __forceinline__ int req_len(const RaggedDecodeParams& p, int b, bool* bad) {
+// Row of request b in q and out: b, or with packed rows cu_q[b].  A type of its own,
+// so that the other form does not pay for it (8 requests in a 2048 bucket 10.3 us,
+// 10.7 with the choice made at run time).
+template <bool PACKED>
+struct Rows {
+  __device__ __forceinline__ int find(int b, int*) const { return b; }
+  __device__ __forceinline__ int at(int b) const { return b; }
+};
+template <>
+struct Rows<true> {
+  const int32_t* cu_q;  // [B + 1]
+  int n;                // packed rows
+  // -1 without a token.  More than one, or rows outside the packed ones, are not
+  // for this call (0x925).
+  __device__ __forceinline__ int find(int b, int* bad) const {
+    const int first = cu_q[b], end = cu_q[b + 1];
+    if (first == end) return -1;
+    if (first < 0 || first >= n || end != first + 1) {
+      *bad = 0x925;
+      return -1;
+    }
+    return first;
+  }
+  // of a request that has tiles
+  __device__ __forceinline__ int at(int b) const { return cu_q[b]; }
+};
+
+// Length of request b, inside what its table row can hold; 0 without a token.
+template <bool PACKED>
+__device__ __forceinline__ int req_len(const RaggedDecodeParams& p, const Rows<PACKED>& rows, int b,
+                                       int* bad) {
   const int L = p.kv_lens[b];
-  if (L < 0 || L > p.capacity) *bad = true;
+  if (PACKED && rows.find(b, bad) < 0) return 0;
+  if (L < 0 || L > p.capacity) *bad = 0x921;
   return min(max(L, 0), p.capacity);
 }
 
@@ -116,15 +148,17 @@ struct Piece {
 struct Walk {
   int b, kvh, tile, nt, L;
   int64_t left;
-  __device__ __forceinline__ bool next(const RaggedDecodeParams& p, Piece& w) {
+  template <bool PACKED>
+  __device__ __forceinline__ bool next(const RaggedDecodeParams& p, const Rows<PACKED>& rows,
+                                       Piece& w) {
     if (left <= 0) return false;
-    bool bad = false;
+    int bad = 0;
     while (tile >= nt) {  // the next pair that has tiles
       tile = 0;
       if (nt > 0 && ++kvh < p.Hkv) break;
       kvh = 0;
       if (++b >= p.B) return false;
-      L = req_len(p, b, &bad);
+      L = req_len(p, rows, b, &bad);
       nt = (L + kTile - 1) / kTile;
     }
     w.b = b;
@@ -140,10 +174,11 @@ struct Walk {
   }
 };
 
-template <bool WIDE>
+template <bool WIDE, bool PACKED>
 __global__ void __launch_bounds__(kThreads, 1)
     ragged_decode_kernel(const __grid_constant__ CUtensorMap tmK,
-                         const __grid_constant__ CUtensorMap tmV, RaggedDecodeParams p) {
+                         const __grid_constant__ CUtensorMap tmV, RaggedDecodeParams p,
+                         Rows<PACKED> rows) {
   using C = Cfg<WIDE>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
@@ -183,13 +218,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto cut = [&](uint32_t k) { return share * k + (rest * k) / nc; };
   Walk walk;
   int64_t u0 = 0, off = 0;
-  bool bad = false;
+  int bad = 0;  // error code of a request this thread looked at
   walk.b = p.B;
   walk.nt = walk.L = walk.kvh = walk.tile = 0;
   walk.left = 0;
   if (p.B <= 32) {
     // one request per lane: every warp scans for itself
-    walk.L = lane < p.B ? req_len(p, lane, &bad) : 0;
+    walk.L = lane < p.B ? req_len(p, rows, lane, &bad) : 0;
     walk.nt = (walk.L + kTile - 1) / kTile;
     const int64_t mine = (int64_t)walk.nt * p.Hkv;
     int64_t incl = mine;
@@ -214,7 +249,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int per = (p.B + kThreads - 1) / kThreads;
     const int b0 = min((int)threadIdx.x * per, p.B), b1 = min(b0 + per, p.B);
     int64_t mine = 0;
-    for (int b = b0; b < b1; ++b) mine += (req_len(p, b, &bad) + kTile - 1) / kTile;
+    for (int b = b0; b < b1; ++b) mine += (req_len(p, rows, b, &bad) + kTile - 1) / kTile;
     mine *= p.Hkv;
     int64_t incl = mine;
 #pragma unroll
@@ -237,7 +272,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (before <= u0 && u0 < before + mine) {  // one thread's requests
         int64_t at = before;
         for (int b = b0; b < b1; ++b) {
-          const int L = req_len(p, b, &bad), nt = (L + kTile - 1) / kTile;
+          const int L = req_len(p, rows, b, &bad), nt = (L + kTile - 1) / kTile;
           const int64_t n = (int64_t)nt * p.Hkv;
           if (u0 < at + n) {
             s_start[0] = b;
@@ -258,7 +293,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       walk.L = s_start[3];
     }
   }
-  if (bad && c == 0) report_timeout(p.err, 0x921);
+  if (bad && c == 0) report_timeout(p.err, bad);
   if (walk.left > 0) {
     walk.kvh = (int)((uint32_t)off / (uint32_t)walk.nt);
     walk.tile = (int)off - walk.kvh * walk.nt;
@@ -271,7 +306,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = true;
     int64_t u = u0;  // first tile of the piece in the list
     if (lane == 0) p.ws_desc[c] = make_int2(-1, -1);
-    while (ok && walk.next(p, w)) {
+    while (ok && walk.next(p, rows, w)) {
       int pages = 0;  // this lane's entry of 32 tiles' pages
       for (int t = w.t0; t < w.t1; ++t, ++it) {
         const int k = (t - w.t0) & 31;
@@ -321,7 +356,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         };
         const int64_t first = u - w.t0;
         const int last = holder(c, first + w.nt - 1);
-        const int id = w.t0 == 0 ? w.b * p.Hkv + w.kvh : -2 - holder(0, first);
+        const int id = w.t0 == 0 ? rows.at(w.b) * p.Hkv + w.kvh : -2 - holder(0, first);
         if (lane == 0) p.ws_desc[c] = make_int2(id, last);
       }
       u += w.t1 - w.t0;
@@ -338,12 +373,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t ring = smem_u32(smem);
     bool ok = true;
     int it = 0;
-    while (walk.next(p, w)) {
+    while (walk.next(p, rows, w)) {
       // Q as the A operand: row g (and g + 8) = query head kvh * G + row
       uint32_t qf[8][WIDE ? 4 : 2];
       {
         const __nv_bfloat16* qh =
-            p.q + w.b * p.q_stride + (int64_t)(w.kvh * p.G) * kD + 2 * t4;
+            p.q + rows.at(w.b) * p.q_stride + (int64_t)(w.kvh * p.G) * kD + 2 * t4;
 #pragma unroll
         for (int ks = 0; ks < 8; ++ks)
 #pragma unroll
@@ -540,7 +575,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (whole) {
           const float inv = over_sum(1.0f, ls);
-          *reinterpret_cast<uint2*>(p.out + w.b * p.out_stride +
+          *reinterpret_cast<uint2*>(p.out + rows.at(w.b) * p.out_stride +
                                     (int64_t)(w.kvh * p.G + row) * kD + d) =
               make_uint2(pack_bf16x2(a.x * inv, a.y * inv), pack_bf16x2(a.z * inv, a.w * inv));
         } else {
@@ -554,10 +589,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     // requests with nothing cached: zeros
     const int Hq = p.Hkv * p.G;
-    for (int b = c; b < p.B; b += gridDim.x)
-      if (p.kv_lens[b] <= 0)
+    for (int b = c; b < p.B; b += gridDim.x) {
+      const int row = rows.find(b, &bad);
+      if (row >= 0 && p.kv_lens[b] <= 0)
         for (int i = threadIdx.x; i < Hq * kD / 8; i += kConsumers * 32)
-          reinterpret_cast<uint4*>(p.out + b * p.out_stride)[i] = make_uint4(0, 0, 0, 0);
+          reinterpret_cast<uint4*>(p.out + row * p.out_stride)[i] = make_uint4(0, 0, 0, 0);
+    }
   }
 }
 
@@ -620,8 +657,8 @@ __device__ __forceinline__ void join_many(const RaggedDecodeParams& p, int c0, i
       x = fmaf(f, s_acc[i][threadIdx.x], x);
       ls = fmaf(f, s_ml[i].y, ls);
     }
-    const int pair = p.ws_desc[c0].x, b = pair / p.Hkv, kvh = pair - b * p.Hkv;
-    p.out[b * p.out_stride + (int64_t)(kvh * p.G + row) * kD + d0 + threadIdx.x] =
+    const int pair = p.ws_desc[c0].x, r = pair / p.Hkv, kvh = pair - r * p.Hkv;
+    p.out[r * p.out_stride + (int64_t)(kvh * p.G + row) * kD + d0 + threadIdx.x] =
         f2bf(over_sum(x, ls));
   }
 }
@@ -682,8 +719,8 @@ __global__ void __launch_bounds__(W * 32) ragged_decode_join(RaggedDecodeParams 
       x = fmaf(f, s_acc[i][threadIdx.x], x);
       ls = fmaf(f, s_ml[i].y, ls);
     }
-    const int b = d.x / p.Hkv, kvh = d.x - b * p.Hkv;
-    p.out[b * p.out_stride + (int64_t)(kvh * p.G + row) * kD + threadIdx.x] =
+    const int r = d.x / p.Hkv, kvh = d.x - r * p.Hkv;
+    p.out[r * p.out_stride + (int64_t)(kvh * p.G + row) * kD + threadIdx.x] =
         f2bf(over_sum(x, ls));
   }
 }
@@ -699,29 +736,20 @@ size_t decode_ws(int G, size_t* off_ml, size_t* off_desc) {
   return n + decode_grid() * sizeof(int2);
 }
 
-}  // namespace
-}  // namespace q3
-
-extern "C" size_t q3_attn_decode_ragged_workspace_bytes(int Hq, int Hkv) {
-  if (Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || Hq / Hkv > 16) return 0;
-  size_t a, b;
-  return q3::decode_ws(Hq / Hkv, &a, &b);
-}
-
-extern "C" int q3_attn_decode_ragged(const void* q, int64_t q_stride, const void* k_pages,
-                                     const void* v_pages, void* out, int64_t out_stride, int B,
-                                     int Hq, int Hkv, int head_dim, const int32_t* block_table,
-                                     int64_t table_stride, int table_width, int page_tokens,
-                                     int64_t num_pages, const int32_t* kv_lens, float scale,
-                                     void* workspace, size_t workspace_bytes,
-                                     q3_stream_t stream) {
-  using namespace q3;
+// Both entry points (a kernel of each width); messages name the first.
+template <bool PACKED>
+int decode_ragged(const void* q, int64_t q_stride, const void* k_pages, const void* v_pages,
+                  void* out, int64_t out_stride, int64_t n_rows, int B, int Hq, int Hkv,
+                  int head_dim, const int32_t* block_table, int64_t table_stride, int table_width,
+                  int page_tokens, int64_t num_pages, const int32_t* kv_lens, float scale,
+                  void* workspace, size_t workspace_bytes, Rows<PACKED> rows_of_q,
+                  q3_stream_t stream) {
   Q3_REQUIRE(head_dim == kD, "q3_attn_decode_ragged: head_dim must be 128 (got %d)", head_dim);
   Q3_REQUIRE(B >= 0 && B <= kMaxB && Hq > 0 && Hkv > 0 && Hkv <= 1024 && Hq % Hkv == 0,
              "q3_attn_decode_ragged: bad shape B=%d Hq=%d Hkv=%d", B, Hq, Hkv);
   if (Hq / Hkv > 16)
     return fail(Q3_ERR_UNSUPPORTED, "q3_attn_decode_ragged: Hq/Hkv=%d above 16", Hq / Hkv);
-  if (B == 0) return Q3_OK;
+  if (B == 0 || n_rows == 0) return Q3_OK;
   Q3_REQUIRE(q && k_pages && v_pages && out && block_table && kv_lens && workspace,
              "q3_attn_decode_ragged: null pointer");
   Q3_REQUIRE(page_tokens > 0 && page_tokens % kTile == 0,
@@ -766,22 +794,61 @@ extern "C" int q3_attn_decode_ragged(const void* q, int64_t q_stride, const void
   int dev = 0;
   Q3_CUDA_CHECK(cudaGetDevice(&dev));
   if (dev < 0 || dev >= 64 || !attr_set[dev]) {
-    Q3_CUDA_CHECK(cudaFuncSetAttribute(ragged_decode_kernel<false>,
+    Q3_CUDA_CHECK(cudaFuncSetAttribute(ragged_decode_kernel<false, PACKED>,
                                        cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        Cfg<false>::kSmem));
-    Q3_CUDA_CHECK(cudaFuncSetAttribute(ragged_decode_kernel<true>,
+    Q3_CUDA_CHECK(cudaFuncSetAttribute(ragged_decode_kernel<true, PACKED>,
                                        cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        Cfg<true>::kSmem));
     if (dev >= 0 && dev < 64) attr_set[dev] = true;
   }
   const dim3 grid((unsigned)decode_grid());
-  rc = G > 8 ? launch_ex(ragged_decode_kernel<true>, grid, dim3(kThreads), Cfg<true>::kSmem,
-                         (cudaStream_t)stream, 1, tk, tv, p)
-             : launch_ex(ragged_decode_kernel<false>, grid, dim3(kThreads), Cfg<false>::kSmem,
-                         (cudaStream_t)stream, 1, tk, tv, p);
+  rc = G > 8 ? launch_ex(ragged_decode_kernel<true, PACKED>, grid, dim3(kThreads), Cfg<true>::kSmem,
+                         (cudaStream_t)stream, 1, tk, tv, p, rows_of_q)
+             : launch_ex(ragged_decode_kernel<false, PACKED>, grid, dim3(kThreads), Cfg<false>::kSmem,
+                         (cudaStream_t)stream, 1, tk, tv, p, rows_of_q);
   if (rc) return rc;
   auto join = G > 8 ? (split ? ragged_decode_join<4, true> : ragged_decode_join<4, false>)
                     : (split ? ragged_decode_join<8, true> : ragged_decode_join<8, false>);
   return launch_ex(join, dim3(grid.x, (unsigned)G), dim3(G > 8 ? 128 : 256), 0,
                    (cudaStream_t)stream, 1, p);
+}
+
+}  // namespace
+}  // namespace q3
+
+extern "C" size_t q3_attn_decode_ragged_workspace_bytes(int Hq, int Hkv) {
+  if (Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || Hq / Hkv > 16) return 0;
+  size_t a, b;
+  return q3::decode_ws(Hq / Hkv, &a, &b);
+}
+
+extern "C" int q3_attn_decode_ragged(const void* q, int64_t q_stride, const void* k_pages,
+                                     const void* v_pages, void* out, int64_t out_stride, int B,
+                                     int Hq, int Hkv, int head_dim, const int32_t* block_table,
+                                     int64_t table_stride, int table_width, int page_tokens,
+                                     int64_t num_pages, const int32_t* kv_lens, float scale,
+                                     void* workspace, size_t workspace_bytes,
+                                     q3_stream_t stream) {
+  return q3::decode_ragged(q, q_stride, k_pages, v_pages, out, out_stride, B, B, Hq, Hkv, head_dim,
+                           block_table, table_stride, table_width, page_tokens, num_pages, kv_lens,
+                           scale, workspace, workspace_bytes, q3::Rows<false>{}, stream);
+}
+
+extern "C" int q3_attn_decode_ragged_packed(
+    const void* q, int64_t q_stride, const void* k_pages, const void* v_pages, void* out,
+    int64_t out_stride, int64_t n_tokens, int B, int Hq, int Hkv, int head_dim,
+    const int32_t* block_table, int64_t table_stride, int table_width, int page_tokens,
+    int64_t num_pages, const int32_t* cu_q, const int32_t* kv_lens, float scale, void* workspace,
+    size_t workspace_bytes, q3_stream_t stream) {
+  using namespace q3;
+  Q3_REQUIRE(n_tokens >= 0 && n_tokens * max64(Hkv, 1) < (1ll << 31),
+             "q3_attn_decode_ragged_packed: n_tokens=%lld, %d K/V heads pass 32-bit rows",
+             (long long)n_tokens, Hkv);
+  Q3_REQUIRE(B == 0 || n_tokens == 0 || (cu_q && aligned(cu_q, 4)),
+             "q3_attn_decode_ragged_packed: cu_q is null or misaligned");
+  return decode_ragged(q, q_stride, k_pages, v_pages, out, out_stride, n_tokens, B, Hq, Hkv,
+                       head_dim, block_table, table_stride, table_width, page_tokens, num_pages,
+                       kv_lens, scale, workspace, workspace_bytes,
+                       Rows<true>{cu_q, (int)n_tokens}, stream);
 }

@@ -79,6 +79,8 @@ SIGNATURES: dict[str, tuple] = {
     "q3_attn_decode_ragged_workspace_bytes": (SZ, [I32, I32]),
     "q3_attn_decode_ragged": (I32, [P, I64, P, P, P, I64, I32, I32, I32, I32, P, I64, I32, I32,
                                     I64, P, F32, P, SZ, P]),
+    "q3_attn_decode_ragged_packed": (I32, [P, I64, P, P, P, I64, I64, I32, I32, I32, I32, P, I64,
+                                           I32, I32, I64, P, P, F32, P, SZ, P]),
     "q3_attn_prefill_ragged_workspace_bytes": (SZ, []),
     "q3_attn_prefill_ragged": (I32, [P, I64, P, P, P, I64, I64, I32, I32, I32, I32, P, I64, I32,
                                      I32, I64, P, P, I32, F32, P, SZ, P]),

@@ -1234,25 +1234,41 @@ def qkv_norm_rope_ragged(qkv: torch.Tensor, q_norm_w: torch.Tensor, k_norm_w: to
 
 def attn_decode_ragged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
                        block_table: torch.Tensor, kv_lens: torch.Tensor, scale: float = None,
-                       out: torch.Tensor = None) -> torch.Tensor:
+                       out: torch.Tensor = None, cu_q: torch.Tensor = None) -> torch.Tensor:
     """Attention of one new token per request over its own length of the pool.
 
     q bf16 [B, Hq, 128] (any row stride); k_pages / v_pages [num_pages, Hkv,
     page_tokens, 128]; block_table int32 [B, width]; kv_lens int32 [B] on the
     device: request b attends to positions [0, kv_lens[b]), and a length of 0
-    gives zeros.  Hq / Hkv is any whole number up to 16; out may be q."""
+    gives zeros.  Hq / Hkv is any whole number up to 16; out may be q.
+
+    Row b of q is request b's, so every request needs a row.  In a step where a
+    request may bring no token, cu_q (int32 [B + 1], RaggedPlan.cu_q) says whose
+    the rows of a packed q [n, Hq, 128] are: cu_q[b] is request b's when it has
+    one token, and one without a token is left out (with more, it is left out
+    and 0x925 recorded).  Other rows of out are not written."""
     name = "attn_decode_ragged"
-    B = q.shape[0] if q.dim() else 0
+    B = kv_lens.numel() if cu_q is not None else q.shape[0] if q.dim() else 0
     dev, q_stride, table_stride, out, out_stride = _ragged_attn(name, q, k_pages, v_pages,
                                                                 block_table, kv_lens, out, B)
     Hq = q.shape[1]
     num_pages, Hkv, page_tokens, D = k_pages.shape
+    scale = HEAD_DIM ** -0.5 if scale is None else float(scale)
     ws, nbytes = _ragged_workspace(q, dev, "q3_attn_decode_ragged_workspace_bytes", Hq, Hkv)
+    if cu_q is not None:
+        if cu_q.get_device() != dev:
+            raise RuntimeError(f"{name}: cu_q must be on the other tensors' CUDA device")
+        _ragged_call("q3_attn_decode_ragged_packed", dev, q.data_ptr(), q_stride,
+                     k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), out_stride,
+                     q.shape[0], B, Hq, Hkv, D, block_table.data_ptr(), table_stride,
+                     block_table.shape[1], page_tokens, num_pages,
+                     _ragged_ints(name, "cu_q", cu_q, torch.int32, B + 1), kv_lens.data_ptr(),
+                     scale, ws.data_ptr(), nbytes)
+        return out
     _ragged_call("q3_attn_decode_ragged", dev, q.data_ptr(), q_stride, k_pages.data_ptr(),
                  v_pages.data_ptr(), out.data_ptr(), out_stride, B, Hq, Hkv, D,
                  block_table.data_ptr(), table_stride, block_table.shape[1], page_tokens,
-                 num_pages, kv_lens.data_ptr(),
-                 HEAD_DIM ** -0.5 if scale is None else float(scale), ws.data_ptr(), nbytes)
+                 num_pages, kv_lens.data_ptr(), scale, ws.data_ptr(), nbytes)
     return out
 
 
