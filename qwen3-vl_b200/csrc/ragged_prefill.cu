@@ -420,7 +420,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       int T = 0, ic = 0, nk = 0, nv = 0, tails = 0;
       bool ok = true;
       if (lane == 0) p.ws_desc[c] = make_int4(-1, 0, 0, 0);
-      while (ok && !*abort_flag && walk.next(p, w)) {
+      // (one vote on the flag, which another warp may set between two lanes' reads)
+      while (ok && !__any_sync(0xffffffffu, *abort_flag != 0) && walk.next(p, w)) {
         // this lane's 64-key block of 16 tiles at a time: its first row in the pool, or
         // -1 (page_tokens % 64 == 0: a block never straddles); loaded ahead of Q
         auto block_row = [&](int j) {
