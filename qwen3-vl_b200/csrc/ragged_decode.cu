@@ -362,8 +362,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       u += w.t1 - w.t0;
     }
     // the copies issued land before the CTA may exit (the consumers wait for
-    // every one of them unless a wait ran out)
-    if (!ok && lane == 0)
+    // every one of them unless a wait ran out, theirs or this warp's)
+    if (lane == 0)
       for (int i = max(0, it - C::kStages); i < it; ++i)
         mbar_wait(&full[i % C::kStages], (i / C::kStages) & 1, nullptr, 0);
   } else {

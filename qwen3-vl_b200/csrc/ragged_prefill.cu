@@ -490,9 +490,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive(&v_full[s]);
-          } else {
-            nv = T + 1;
           }
+          nv = T + 1;
         }
         if (w.t0 == 0 && w.t1 < w.nt) {
           // the item goes on in the next CTAs: find the last of them
@@ -508,17 +507,17 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (lane == 0) p.ws_desc[c] = make_int4(w.b, w.kvh, w.item, last);
         }
       }
-      if (!ok) {
-        *abort_flag = 1;
-        // let the copies this warp issued land before the CTA exits
-        if (lane == 0) {
-          if (ic > 0) mbar_wait(q_full, (ic - 1) & 1, nullptr, 0);
-          for (int j = max(0, nk - 2); j < nk; ++j)
-            mbar_wait(&k_full[j & 1], (j >> 1) & 1, nullptr, 0);
-          for (int j = max(0, nv - 2); j < nv; ++j)
-            mbar_wait(&v_full[j & 1], (j >> 1) & 1, nullptr, 0);
-          if (tails > 0) mbar_wait(v_tail, (tails - 1) & 1, nullptr, 0);
-        }
+      if (!ok) *abort_flag = 1;
+      // The copies this warp issued land before the CTA exits.  They have when all went
+      // well; when a wait ran out, here or in another warp, the last ones of each
+      // barrier may not have.
+      if (lane == 0) {
+        if (ic > 0) mbar_wait(q_full, (ic - 1) & 1, nullptr, 0);
+        for (int j = max(0, nk - 2); j < nk; ++j)
+          mbar_wait(&k_full[j & 1], (j >> 1) & 1, nullptr, 0);
+        for (int j = max(0, nv - 2); j < nv; ++j)
+          mbar_wait(&v_full[j & 1], (j >> 1) & 1, nullptr, 0);
+        if (tails > 0) mbar_wait(v_tail, (tails - 1) & 1, nullptr, 0);
       }
     } else if (warp == 1) {
       // ------------------------------ MMA issuer --------------------------------
