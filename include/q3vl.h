@@ -170,8 +170,10 @@ Q3_API int q3_attn_decode_paged(const void* q, const void* k_pages, const void* 
  * positions int64 (cache position + rope_delta[b], rope_delta int64 [B] or
  * NULL) and slots int64 (page * page_tokens + offset).  Rows behind the last
  * request get request -1, position 0, slot -1.  Errors recorded: 0x901 a
- * negative length (taken as 0); 0x902 a position past the table (slot -1,
- * kv_lens clamped); 0x903 no page (free list short: counts[1] > n_free, table
+ * negative length (taken as 0); 0x902 a position past the table, cached ones
+ * included (slot -1, kv_lens clamped to the table: the attentions then place that
+ * request's queries too early, and its outputs are of no use; the other requests'
+ * are what they were); 0x903 no page (free list short: counts[1] > n_free, table
  * entry -1; or the table's entry negative; slot -1); 0x904 more tokens than
  * n_tokens (the last ones are dropped). */
 Q3_API int q3_ragged_plan(const int32_t* q_lens, const int32_t* past_lens, int B,

@@ -96,12 +96,13 @@ __global__ void __launch_bounds__(kPlanThreads) ragged_plan_kernel(PlanParams p)
   const int b0 = min(tid * per, p.B), b1 = min(b0 + per, p.B);
   const int P = p.page_tokens;
   const int64_t cap = (int64_t)p.width * P;
-  bool bad = false;
+  int bad = 0;
 
   int64_t mine = 0, total;
   for (int b = b0; b < b1; ++b) {
-    const int q = p.q_lens[b];
-    bad |= q < 0 || p.past[b] < 0;
+    const int q = p.q_lens[b], past = p.past[b];
+    if (q < 0 || past < 0) bad = 0x901;
+    else if (past > cap) bad = 0x902;  // clamped, with or without new tokens
     mine += max(q, 0);
   }
   int64_t at = block_scan(mine, &total);
@@ -111,7 +112,7 @@ __global__ void __launch_bounds__(kPlanThreads) ragged_plan_kernel(PlanParams p)
   }
   if (tid == 0) cu[p.B] = (int32_t)min64(total, p.n_tokens);
   if (blockIdx.x == 0) {
-    if (bad) report_timeout(p.err, 0x901);
+    if (bad) report_timeout(p.err, bad);
     if (tid == 0 && total > p.n_tokens) report_timeout(p.err, 0x904);
   }
   __syncthreads();
