@@ -19,8 +19,8 @@
 // entry that another CTA may be writing.
 //
 // Bound by latency: one chain of loads (lengths, then table or list), scans and
-// stores.  Measured on B200 in a graph: 8 requests of one token 4.5 us, 1024
-// requests with 79718 tokens (1.6 MB written) 8.0 us.
+// stores.  Measured on B200 in a graph: 8 requests of one token 4.2 us, 1024
+// requests with 79718 tokens (1.6 MB written) 7.9 us.
 #include "common.cuh"
 
 namespace q3 {

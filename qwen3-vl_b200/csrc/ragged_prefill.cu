@@ -30,10 +30,10 @@
 // 10/2 heads.  An item cut in the middle leaves fp32 pieces (O, base, sum) in the
 // workspace and a second kernel joins them in CTA order: a 512-token chunk on a 32k
 // cache fills every SM (its 64 items alone would fill 64).
-// Measured on B200, 32/8 heads: that chunk 256 to 268 us by device (1065 to 1017
+// Measured on B200, 32/8 heads: that chunk 256 to 272 us by device (1065 to 1002
 // TFLOP/s at the clock the power cap leaves in a long run, 1.66 GHz and 61 % of the
-// tensor pipe under ncu); six prompts of 1100 to 4096 tokens 469 to 480 us (997 to
-// 975); four prompts of up to 100 tokens at 4/1 heads 11.6 us.
+// tensor pipe under ncu); six prompts of 1100 to 4096 tokens 469 to 486 us (997 to
+// 962); four prompts of up to 100 tokens at 4/1 heads 11.4 us.
 #include <math.h>
 
 #include "common.cuh"
@@ -62,7 +62,8 @@ constexpr int kSmem = kOffBar + 256 + 1024;
 static_assert(kSmem + 1024 <= 227 * 1024, "shared memory (1 KB for the static part)");
 constexpr uint32_t kTmemCols = 512;       // S[0] S[1] O[0] O[1], 128 columns each
 // a row's base moves when its maximum has grown by more than 2^16: P, l and O are
-// relative to the base, and fp32 holds 2^16 times V for any |V| below 2^112
+// relative to the base, so over n keys O may reach n 2^16 |V|, which fp32 holds
+// while |V| is below 2^112 / n (2^97 at 32768 keys)
 constexpr float kLazyLog2 = 16.0f;
 constexpr int kMaxB = 65536;
 constexpr int kMaxGrid = 512;
@@ -91,7 +92,7 @@ __device__ __forceinline__ bool warp_ok(uint64_t* bar, uint32_t parity, int* err
 // The exponentials of keys 64 * HALF .. + 63 of a row against base m: their bf16
 // pairs and the sums of the unrounded values.  All on the MUFU pipe: with a
 // quarter of them as polynomials on the FMA pipe the six-prompt case took 561 us
-// against 520 (a thread's chain of instructions is what is long, not one pipe).
+// against 520, measured with an epilogue that has since been replaced.
 template <int HALF>
 __device__ __forceinline__ void half_exps(const uint32_t (&rr)[kN], float scale_log2, float m,
                                           float2 (&sum)[2], uint32_t (&pk)[32]) {

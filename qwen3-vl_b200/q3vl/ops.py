@@ -1237,7 +1237,7 @@ def attn_decode_ragged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Te
                        out: torch.Tensor = None, cu_q: torch.Tensor = None) -> torch.Tensor:
     """Attention of one new token per request over its own length of the pool.
 
-    q bf16 [B, Hq, 128] (any row stride); k_pages / v_pages [num_pages, Hkv,
+    q bf16 [B, Hq, 128] (even row stride); k_pages / v_pages [num_pages, Hkv,
     page_tokens, 128]; block_table int32 [B, width]; kv_lens int32 [B] on the
     device: request b attends to positions [0, kv_lens[b]), and a length of 0
     gives zeros.  Hq / Hkv is any whole number up to 16; out may be q.
@@ -1278,7 +1278,7 @@ def attn_prefill_ragged(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.T
                         out: torch.Tensor = None) -> torch.Tensor:
     """Attention of packed prompt chunks over the page pool, on tcgen05.
 
-    q bf16 [n, Hq, 128] (any row stride); cu_q int32 [B + 1]: request b owns rows
+    q bf16 [n, Hq, 128] (row stride a multiple of 8); cu_q int32 [B + 1]: request b owns rows
     cu_q[b] .. cu_q[b+1] - 1 of q, and its last one sits at position
     kv_lens[b] - 1; with causal each query sees positions up to its own.  Rows of
     out outside [cu_q[0], cu_q[B]) are not written, so a part of a batch goes
